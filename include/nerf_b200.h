@@ -358,6 +358,97 @@ NERF_API NerfStatus nerf_b200_composite(const NerfB200RayRecord* rays, uint32_t 
 NERF_API NerfStatus nerf_b200_adam(float* master, void* params_f16, void* grid_grad_f16, const float* mlp_grad, float* adam_m,
                                    float* adam_v, uint64_t n_grid, uint64_t n_params, const float scalars[5], uint32_t skip,
                                    float beta1, float beta2, float eps, void* stream);
+/* ---- dense layers and gradient norms (kernel-level, device pointers) ----
+ * What a stack of layers of any width needs beside the fixed field MLPs: a
+ * layer's forward and backward, and the gradient norm and clipping of the
+ * training step over any list of tensors.  One training step of such a stack
+ * is linear_forward per layer, linear_backward per layer, grad_clip, then
+ * nerf_b200_adam on the flat vector (n_grid = 0).  No counterpart in the
+ * reference, whose network is a fixed fused kernel.
+ * All calls are asynchronous on `stream`, of the current device; memory of
+ * another device or of the host is refused.  They can be captured into a
+ * graph: pointers and sizes are then fixed, contents are read at replay. */
+#define NERF_B200_F32  0u
+#define NERF_B200_F16  1u
+#define NERF_B200_BF16 2u
+#define NERF_B200_ACT_NONE    0u
+#define NERF_B200_ACT_RELU    1u /* z > 0 ? z : 0 */
+#define NERF_B200_ACT_SILU    2u /* z / (1 + exp(-z)) */
+#define NERF_B200_ACT_GELU    3u /* z (1 + erf(z / sqrt 2)) / 2 */
+#define NERF_B200_ACT_SIGMOID 4u /* 1 / (1 + exp(-z)) */
+/* Row-major matrices; ld_* are the values between two rows (0: tight). */
+typedef struct NerfB200Linear {
+    uint32_t n_rows;      /* may be 0                                             */
+    uint32_t n_in;
+    uint32_t n_out;
+    uint32_t dtype;       /* F16 or BF16: everything but dweight, dbias           */
+    uint32_t activation;
+    uint32_t grad_dtype;  /* of dweight and dbias: F32, or dtype                  */
+    uint32_t accumulate;  /* 1: backward adds to dweight and dbias                */
+    uint32_t reserved;    /* 0 */
+    uint64_t ld_x;        /* x [n_rows][n_in]                                     */
+    uint64_t ld_weight;   /* weight [n_out][n_in]                                 */
+    uint64_t ld_residual; /* residual [n_rows][n_out]; dx_residual [n_rows][n_in] */
+    uint64_t ld_y;        /* y [n_rows][n_out]                                    */
+    uint64_t ld_pre;      /* pre [n_rows][n_out]                                  */
+    uint64_t ld_dy;       /* dy [n_rows][n_out]                                   */
+    uint64_t ld_dx;       /* dx [n_rows][n_in]                                    */
+} NerfB200Linear;
+/* z = x weight^T + bias, y = act(z) + residual; pre = z where given (what the
+ * backward needs unless the activation is NONE).  bias [n_out], residual and
+ * pre may be NULL.  Products are summed in fp32, y and pre are rounded once.
+ * residual may be y itself; otherwise outputs overlap nothing.  Any alignment
+ * of the dtype is accepted; rows that start on 16-byte boundaries (pointer
+ * and ld) are the fast path.  error_word: one device uint32; bit 0 is set
+ * when a wait inside the kernel ran out after a second (outputs are then
+ * incomplete). */
+NERF_API NerfStatus nerf_b200_linear_forward(const NerfB200Linear* desc, const void* x, const void* weight, const void* bias,
+                                             const void* residual, void* y, void* pre, uint32_t* error_word, void* stream);
+/* dz = dy act'(pre); dx = dz weight + dx_residual; dweight [n_out][n_in]
+ * (tight) and dbias [n_out] are dz^T x and the column sums of dz, written or
+ * added to.  dx, dweight, dbias, dx_residual may be NULL (dx_residual may be
+ * dx itself, or dy where the widths agree: the gradient of the forward's
+ * residual is dy).  ReLU passes nothing where pre <= 0, whatever dy holds.
+ * dz is rounded to dtype before the two products (exact for NONE and RELU);
+ * dbias sums it before the rounding.  Sums are fp32 in a fixed order: the
+ * same inputs give the same bits.  workspace: 256-byte aligned,
+ * nerf_b200_linear_backward_workspace_bytes() of the same desc and device (0:
+ * invalid desc), contents irrelevant, one per call in flight: calls on
+ * different streams, and graphs that may run at once, need their own. */
+NERF_API uint64_t nerf_b200_linear_backward_workspace_bytes(const NerfB200Linear* desc);
+NERF_API NerfStatus nerf_b200_linear_backward(const NerfB200Linear* desc, const void* x, const void* weight, const void* pre,
+                                              const void* dy, const void* dx_residual, void* dx, void* dweight, void* dbias,
+                                              void* workspace, uint64_t workspace_bytes, uint32_t* error_word, void* stream);
+/* One gradient tensor: `count` contiguous values of dtype at grad, and for
+ * the clip where the clipped values go: out == grad for in place, or memory
+ * of its own, of out_dtype = dtype or F32. */
+typedef struct NerfB200GradTensor {
+    const void* grad;
+    void* out;
+    uint64_t count;      /* 0: skipped */
+    uint32_t dtype;
+    uint32_t out_dtype;
+} NerfB200GradTensor;
+typedef struct NerfB200GradNorm {
+    float norm;          /* sqrt(sum of squares of the finite values) / loss_scale  */
+    float scale;         /* what the clip multiplied by (1 after nerf_b200_grad_norm) */
+    uint32_t nonfinite;  /* 1: some value is infinite or NaN                        */
+    uint32_t reserved;
+} NerfB200GradNorm;
+/* The global norm over a host array of tensors (read during the call), into
+ * device memory `info`: the training step's rule, which leaves non-finite
+ * values out of the norm and reports them.  workspace: 16-byte aligned, as in
+ * the backward. */
+NERF_API uint64_t nerf_b200_grad_workspace_bytes(uint32_t n_tensors);
+NERF_API NerfStatus nerf_b200_grad_norm(const NerfB200GradTensor* tensors, uint32_t n_tensors, float loss_scale,
+                                        NerfB200GradNorm* info, void* workspace, uint64_t workspace_bytes, void* stream);
+/* The norm, then out = grad * (norm > max_norm ? max_norm / norm : 1).  With
+ * a non-finite value the scale is 1 and out = grad: the caller skips the
+ * update.  Outputs that overlap each other or another tensor's gradient are
+ * refused (a tensor may not be listed twice).  The loss scale stays in the
+ * gradients. */
+NERF_API NerfStatus nerf_b200_grad_clip(const NerfB200GradTensor* tensors, uint32_t n_tensors, float loss_scale, float max_norm,
+                                        NerfB200GradNorm* info, void* workspace, uint64_t workspace_bytes, void* stream);
 /* Occupancy maintenance of one step with an explicit mode (0 none, 1
  * warm-up init, 2 refresh) and frame; sigma holds the update window's
  * densities. */

@@ -237,6 +237,22 @@ class NerfB200SceneDesc(C.Structure):
     ]
 
 
+class NerfB200Linear(C.Structure):
+    _fields_ = [(n, C.c_uint32) for n in ("n_rows", "n_in", "n_out", "dtype", "activation", "grad_dtype", "accumulate", "reserved")] + [
+        (n, C.c_uint64) for n in ("ld_x", "ld_weight", "ld_residual", "ld_y", "ld_pre", "ld_dy", "ld_dx")]
+
+
+class NerfB200GradTensor(C.Structure):
+    _fields_ = [("grad", C.c_void_p), ("out", C.c_void_p), ("count", C.c_uint64), ("dtype", C.c_uint32), ("out_dtype", C.c_uint32)]
+
+
+class NerfB200GradNorm(C.Structure):
+    _fields_ = [("norm", C.c_float), ("scale", C.c_float), ("nonfinite", C.c_uint32), ("reserved", C.c_uint32)]
+
+
+NERF_B200_F32, NERF_B200_F16, NERF_B200_BF16 = 0, 1, 2
+NERF_B200_ACT_NONE, NERF_B200_ACT_RELU, NERF_B200_ACT_SILU, NERF_B200_ACT_GELU, NERF_B200_ACT_SIGMOID = range(5)
+
 P = C.c_void_p
 U32 = C.c_uint32
 U64 = C.c_uint64
@@ -303,6 +319,12 @@ B200_EXPORTS = {
     "nerf_b200_field_backward_noalloc": (S, [C.POINTER(NerfB200GridLayout), P, P, P, U32, P, P, P, P, P]),
     "nerf_b200_composite": (S, [P, U32, P, P, F32, F32, F32, P, P, P, P, P]),
     "nerf_b200_adam": (S, [P, P, P, P, P, P, U64, U64, P, U32, F32, F32, F32, P]),
+    "nerf_b200_linear_forward": (S, [P, P, P, P, P, P, P, P, P]),
+    "nerf_b200_linear_backward_workspace_bytes": (U64, [P]),
+    "nerf_b200_linear_backward": (S, [P, P, P, P, P, P, P, P, P, P, U64, P, P]),
+    "nerf_b200_grad_workspace_bytes": (U64, [U32]),
+    "nerf_b200_grad_norm": (S, [P, U32, F32, P, P, U64, P]),
+    "nerf_b200_grad_clip": (S, [P, U32, F32, F32, P, P, U64, P]),
     "nerf_b200_occupancy_update": (S, [P, P, P, U32, U32, U32, U32, F32, F32, P]),
 }
 ALL_EXPORTS = {**NERF_H_EXPORTS, **B200_EXPORTS}

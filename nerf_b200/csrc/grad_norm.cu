@@ -1,0 +1,432 @@
+// grad_norm.cu -- the global norm of many gradient tensors, and clipping to it.
+//
+//   norm = sqrt(sum of the squares of all finite values) / loss_scale
+//   out  = g * (norm > max_norm ? max_norm / norm : 1), unless a value is not finite
+// (the rule of the training step's statistics, over any list of tensors).
+//
+// The tensors are cut into chunks of 8192 values; every block of one resident
+// wave takes a contiguous range of chunks and leaves one fp64 partial sum, and
+// whoever needs the norm adds the partials in the same order, so the result
+// does not depend on the blocks' order of execution.  Both passes move each
+// byte once; the clip's second pass walks each range backwards, because the
+// chunks read last are the ones still in the L2 cache.
+#include <cuda_bf16.h>
+
+#include <algorithm>
+#include <cmath>
+#include <new>
+
+#include "../../include/nerf_b200.h"
+#include "common.cuh"
+
+namespace nb {
+namespace {
+
+constexpr uint32_t kChunk = 8192;
+constexpr uint32_t kThreads = 256;
+constexpr uint32_t kMaxBlocks = 1024;  // partial sums of one launch
+constexpr uint32_t kTable = 512;       // tensors of one launch
+
+struct GradEntry {
+    const void* g;
+    void* out;
+    uint64_t count;
+    uint32_t chunk0;  // first chunk of this tensor among the launch's
+    uint16_t type, out_type;
+};
+template <uint32_t CAP>
+struct GradTable {
+    uint32_t n, chunks, blocks;  // blocks: ranges that the chunks are dealt to
+    uint32_t pad;
+    GradEntry e[CAP];
+};
+struct GradPartial {
+    double sum;
+    uint32_t bad;
+    uint32_t pad;
+};
+struct GradInfo {
+    float norm, scale;
+    uint32_t nonfinite, reserved;
+};
+
+NB_DEV float2 unpack_bf(uint32_t v) { return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u)); }
+NB_DEV uint32_t pack_bf(float lo, float hi) {
+    __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<uint32_t*>(&h);
+}
+// The values of a 16-byte vector of a type: 4 fp32, 8 fp16 or bf16.
+template <uint32_t TYPE>
+struct Vec {
+    static constexpr uint32_t kN = TYPE == NERF_B200_F32 ? 4u : 8u;
+    static constexpr uint32_t kBytes = 16u / kN;
+    NB_DEV static void unpack(const uint4& u, float* v) {
+        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (TYPE == NERF_B200_F32) {
+                v[i] = __uint_as_float(w[i]);
+            } else {
+                const float2 f = TYPE == NERF_B200_F16 ? unpack_h2(w[i]) : unpack_bf(w[i]);
+                v[2 * i] = f.x;
+                v[2 * i + 1] = f.y;
+            }
+        }
+    }
+    NB_DEV static float one(const void* p, uint64_t i) {
+        if (TYPE == NERF_B200_F32) return static_cast<const float*>(p)[i];
+        const uint16_t h = static_cast<const uint16_t*>(p)[i];
+        return TYPE == NERF_B200_F16 ? h2f_bits(h) : __uint_as_float(static_cast<uint32_t>(h) << 16);
+    }
+};
+
+// Squares of fp32 and bf16 values leave the range of fp32 sums at both ends: a
+// batch whose sum does not lie well inside it is added again in fp64 (fp16
+// squares never leave it).
+template <uint32_t TYPE, uint32_t N>
+NB_DEV void add_squares(const float* v, double& sum, uint32_t& bad) {
+    float s = 0.0f;
+#pragma unroll
+    for (uint32_t i = 0; i < N; ++i) {
+        const bool fine = isfinite(v[i]);
+        bad |= fine ? 0u : 1u;
+        const float x = fine ? v[i] : 0.0f;
+        s = fmaf(x, x, s);
+    }
+    if (TYPE != NERF_B200_F16 && !(s >= 1e-25f && s <= 1e37f)) {
+#pragma unroll
+        for (uint32_t i = 0; i < N; ++i)
+            if (isfinite(v[i]) && v[i] != 0.0f) sum += static_cast<double>(v[i]) * v[i];
+        return;
+    }
+    sum += s;
+}
+
+template <uint32_t TYPE>
+NB_DEV void chunk_squares(const GradEntry& e, uint64_t e0, uint64_t e1, double& sum, uint32_t& bad) {
+    constexpr uint32_t V = Vec<TYPE>::kN, B = Vec<TYPE>::kBytes;
+    const uint64_t addr = reinterpret_cast<uint64_t>(e.g) + e0 * B;
+    const uint64_t head = min(e1 - e0, static_cast<uint64_t>(((16u - (addr & 15u)) & 15u) / B));
+    const uint64_t n_vec = (e1 - e0 - head) / V, tail0 = e0 + head + n_vec * V;
+    const uint4* q = reinterpret_cast<const uint4*>(addr + head * B);
+    const uint32_t t = threadIdx.x;
+    for (uint64_t i = t; i < n_vec; i += 4u * kThreads) {
+        uint4 u[4];
+#pragma unroll
+        for (uint32_t j = 0; j < 4u; ++j) u[j] = i + j * kThreads < n_vec ? __ldg(q + i + j * kThreads) : make_uint4(0u, 0u, 0u, 0u);
+        float v[4u * V];
+#pragma unroll
+        for (uint32_t j = 0; j < 4u; ++j) Vec<TYPE>::unpack(u[j], v + j * V);
+        add_squares<TYPE, 4u * V>(v, sum, bad);
+    }
+    const uint64_t rest = head + (e1 - tail0);  // fewer than 2 V values at the two ends
+    if (t < rest) {
+        const float v = Vec<TYPE>::one(e.g, t < head ? e0 + t : tail0 + (t - head));
+        add_squares<TYPE, 1u>(&v, sum, bad);
+    }
+}
+
+template <uint32_t CAP>
+NB_DEV uint32_t entry_of(const GradTable<CAP>& t, uint32_t chunk) {
+    uint32_t lo = 0, hi = t.n;  // last entry that starts at or before the chunk and is not empty
+    while (hi - lo > 1u) {
+        const uint32_t mid = (lo + hi) / 2u;
+        if (t.e[mid].chunk0 <= chunk) lo = mid;
+        else hi = mid;
+    }
+    return lo;
+}
+
+NB_DEV double warp_sum_f64(double v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+
+template <uint32_t CAP>
+__global__ void __launch_bounds__(kThreads) k_grad_squares(const __grid_constant__ GradTable<CAP> t, GradPartial* out) {
+    const uint32_t c0 = static_cast<uint32_t>(static_cast<uint64_t>(t.chunks) * blockIdx.x / t.blocks);
+    const uint32_t c1 = static_cast<uint32_t>(static_cast<uint64_t>(t.chunks) * (blockIdx.x + 1u) / t.blocks);
+    double sum = 0.0;
+    uint32_t bad = 0u;
+    uint32_t k = c0 < c1 ? entry_of(t, c0) : 0u;
+    for (uint32_t c = c0; c < c1; ++c) {
+        while (k + 1u < t.n && t.e[k + 1u].chunk0 <= c) ++k;
+        const GradEntry& e = t.e[k];
+        const uint64_t e0 = static_cast<uint64_t>(c - e.chunk0) * kChunk, e1 = min(e.count, e0 + kChunk);
+        switch (e.type) {
+            case NERF_B200_F32: chunk_squares<NERF_B200_F32>(e, e0, e1, sum, bad); break;
+            case NERF_B200_F16: chunk_squares<NERF_B200_F16>(e, e0, e1, sum, bad); break;
+            default: chunk_squares<NERF_B200_BF16>(e, e0, e1, sum, bad); break;
+        }
+    }
+    __shared__ double ws[kThreads / 32u];
+    sum = warp_sum_f64(sum);
+    if ((threadIdx.x & 31u) == 0u) ws[threadIdx.x >> 5] = sum;
+    const int any = __syncthreads_or(static_cast<int>(bad));
+    if (threadIdx.x == 0u) {
+#pragma unroll
+        for (uint32_t w = 1; w < kThreads / 32u; ++w) sum += ws[w];
+        out[blockIdx.x] = GradPartial{sum, any ? 1u : 0u, 0u};
+    }
+}
+
+// The norm from the partial sums, the same in every block that asks.
+NB_DEV GradInfo grad_info(const GradPartial* __restrict__ p, uint32_t n, float loss_scale, float max_norm) {
+    __shared__ double ws[kThreads / 32u];
+    double sum = 0.0;
+    uint32_t bad = 0u;
+    for (uint32_t i = threadIdx.x; i < n; i += kThreads) {
+        sum += p[i].sum;
+        bad |= p[i].bad;
+    }
+    sum = warp_sum_f64(sum);
+    if ((threadIdx.x & 31u) == 0u) ws[threadIdx.x >> 5] = sum;
+    const int any = __syncthreads_or(static_cast<int>(bad));
+    sum = ws[0];
+#pragma unroll
+    for (uint32_t w = 1; w < kThreads / 32u; ++w) sum += ws[w];
+    const double norm = sqrt(sum) / static_cast<double>(loss_scale);
+    GradInfo r;
+    r.norm = static_cast<float>(norm);
+    r.nonfinite = any ? 1u : 0u;
+    r.scale = !any && norm > static_cast<double>(max_norm) ? static_cast<float>(static_cast<double>(max_norm) / norm) : 1.0f;
+    r.reserved = 0u;
+    return r;
+}
+
+__global__ void __launch_bounds__(kThreads) k_grad_finish(const GradPartial* p, uint32_t n, float loss_scale, GradInfo* info) {
+    const GradInfo r = grad_info(p, n, loss_scale, INFINITY);
+    if (threadIdx.x == 0u) *info = r;
+}
+
+template <uint32_t OUT>
+NB_DEV void store_one(void* p, uint64_t i, float v) {
+    if (OUT == NERF_B200_F32) static_cast<float*>(p)[i] = v;
+    else if (OUT == NERF_B200_F16) static_cast<__half*>(p)[i] = __float2half_rn(v);
+    else static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
+}
+template <uint32_t TYPE, uint32_t OUT>
+NB_DEV void chunk_scale(const GradEntry& e, uint64_t e0, uint64_t e1, float scale) {
+    constexpr uint32_t V = Vec<TYPE>::kN, B = Vec<TYPE>::kBytes, OB = OUT == NERF_B200_F32 ? 4u : 2u;
+    const uint64_t addr = reinterpret_cast<uint64_t>(e.g) + e0 * B;
+    const uint64_t head = min(e1 - e0, static_cast<uint64_t>(((16u - (addr & 15u)) & 15u) / B));
+    const uint64_t n_vec = (e1 - e0 - head) / V, tail0 = e0 + head + n_vec * V;
+    const uint4* q = reinterpret_cast<const uint4*>(addr + head * B);
+    unsigned char* o = static_cast<unsigned char*>(e.out) + (e0 + head) * OB;
+    const bool wide = (reinterpret_cast<uint64_t>(o) & 15u) == 0u;
+    const uint32_t t = threadIdx.x;
+    for (uint64_t i = t; i < n_vec; i += 4u * kThreads) {
+        uint4 u[4];
+#pragma unroll
+        for (uint32_t j = 0; j < 4u; ++j) u[j] = i + j * kThreads < n_vec ? q[i + j * kThreads] : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+        for (uint32_t j = 0; j < 4u; ++j) {
+            const uint64_t at = i + j * kThreads;
+            if (at >= n_vec) break;
+            float v[V];
+            Vec<TYPE>::unpack(u[j], v);
+#pragma unroll
+            for (uint32_t k = 0; k < V; ++k) v[k] *= scale;
+            if (!wide) {
+#pragma unroll
+                for (uint32_t k = 0; k < V; ++k) store_one<OUT>(o, at * V + k, v[k]);
+            } else if (OUT == NERF_B200_F32) {
+                float4* d = reinterpret_cast<float4*>(o) + at * (V / 4u);
+#pragma unroll
+                for (uint32_t k = 0; k < V / 4u; ++k) d[k] = make_float4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]);
+            } else if (V == 8u) {
+                uint32_t w[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    w[k] = OUT == NERF_B200_F16 ? pack_h2(v[(2 * k) % V], v[(2 * k + 1) % V]) : pack_bf(v[(2 * k) % V], v[(2 * k + 1) % V]);
+                reinterpret_cast<uint4*>(o)[at] = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+        }
+    }
+    const uint64_t rest = head + (e1 - tail0);
+    if (t < rest) {
+        const uint64_t i = t < head ? e0 + t : tail0 + (t - head);
+        store_one<OUT>(e.out, i, Vec<TYPE>::one(e.g, i) * scale);
+    }
+}
+
+template <uint32_t CAP>
+__global__ void __launch_bounds__(kThreads)
+    k_grad_scale(const __grid_constant__ GradTable<CAP> t, const GradPartial* p, uint32_t n_partials, float loss_scale, float max_norm,
+                 GradInfo* info) {
+    const GradInfo r = grad_info(p, n_partials, loss_scale, max_norm);
+    if (blockIdx.x == 0u && threadIdx.x == 0u) *info = r;
+    const uint32_t c0 = static_cast<uint32_t>(static_cast<uint64_t>(t.chunks) * blockIdx.x / t.blocks);
+    const uint32_t c1 = static_cast<uint32_t>(static_cast<uint64_t>(t.chunks) * (blockIdx.x + 1u) / t.blocks);
+    for (uint32_t c = c1; c-- > c0;) {
+        const GradEntry& e = t.e[entry_of(t, c)];
+        if (r.scale == 1.0f && e.out == e.g) continue;  // in place and nothing to clip
+        const uint64_t e0 = static_cast<uint64_t>(c - e.chunk0) * kChunk, e1 = min(e.count, e0 + kChunk);
+        switch (e.type * 4u + e.out_type) {
+            case NERF_B200_F32 * 4u + NERF_B200_F32: chunk_scale<NERF_B200_F32, NERF_B200_F32>(e, e0, e1, r.scale); break;
+            case NERF_B200_F16 * 4u + NERF_B200_F16: chunk_scale<NERF_B200_F16, NERF_B200_F16>(e, e0, e1, r.scale); break;
+            case NERF_B200_F16 * 4u + NERF_B200_F32: chunk_scale<NERF_B200_F16, NERF_B200_F32>(e, e0, e1, r.scale); break;
+            case NERF_B200_BF16 * 4u + NERF_B200_BF16: chunk_scale<NERF_B200_BF16, NERF_B200_BF16>(e, e0, e1, r.scale); break;
+            default: chunk_scale<NERF_B200_BF16, NERF_B200_F32>(e, e0, e1, r.scale); break;
+        }
+    }
+}
+
+// ------------------------------------------------------------------- host
+uint32_t resident_blocks() {
+    int dev = 0, sms = 148;
+    if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
+        cudaGetLastError();
+    return std::min(kMaxBlocks, 4u * static_cast<uint32_t>(sms));
+}
+uint32_t type_bytes(uint32_t t) { return t == NERF_B200_F32 ? 4u : 2u; }
+bool valid_tensor(const NerfB200GradTensor& t) {
+    if (t.dtype > NERF_B200_BF16) return false;
+    if (t.count == 0u) return true;
+    const uint64_t b = type_bytes(t.dtype), at = reinterpret_cast<uint64_t>(t.grad);
+    return t.grad && at % b == 0u && t.count <= (1ull << 40);
+}
+bool valid_output(const NerfB200GradTensor& t) {
+    if (t.out_dtype != t.dtype && t.out_dtype != NERF_B200_F32) return false;
+    return t.count == 0u || (t.out && reinterpret_cast<uint64_t>(t.out) % type_bytes(t.out_dtype) == 0u);
+}
+
+struct Range {
+    uint64_t lo, hi;
+};
+// Whether no output touches another output, or a gradient other than its own
+// (and that one only exactly in place).  1 yes, 0 no, -1 out of memory.
+int outputs_apart(const NerfB200GradTensor* ts, uint32_t n) {
+    Range* r = new (std::nothrow) Range[n ? n : 1u];
+    if (!r) return -1;
+    uint32_t m = 0;
+    bool sorted = true;
+    for (uint32_t i = 0; i < n; ++i) {
+        if (ts[i].count == 0u) continue;
+        const uint64_t lo = reinterpret_cast<uint64_t>(ts[i].out);
+        r[m] = Range{lo, lo + ts[i].count * type_bytes(ts[i].out_dtype)};
+        if (m && r[m].lo < r[m - 1u].lo) sorted = false;
+        ++m;
+    }
+    if (!sorted) std::sort(r, r + m, [](const Range& a, const Range& b) { return a.lo < b.lo; });
+    bool apart = true;
+    for (uint32_t i = 1; i < m && apart; ++i) apart = r[i - 1u].hi <= r[i].lo;
+    for (uint32_t i = 0; i < n && apart; ++i) {
+        if (ts[i].count == 0u || (ts[i].out == ts[i].grad && ts[i].dtype == ts[i].out_dtype)) continue;
+        const uint64_t lo = reinterpret_cast<uint64_t>(ts[i].grad), hi = lo + ts[i].count * type_bytes(ts[i].dtype);
+        const Range* q = std::upper_bound(r, r + m, lo, [](uint64_t v, const Range& a) { return v < a.hi; });  // first that ends after lo
+        apart = q == r + m || q->lo >= hi;
+    }
+    delete[] r;
+    return apart ? 1 : 0;
+}
+
+template <uint32_t CAP>
+void fill_table(GradTable<CAP>& t, const NerfB200GradTensor* ts, uint32_t n, uint32_t cap_blocks) {
+    t.n = 0;
+    t.pad = 0;
+    uint64_t chunks = 0;
+    for (uint32_t i = 0; i < n; ++i) {
+        if (ts[i].count == 0u) continue;
+        GradEntry& e = t.e[t.n++];
+        e.g = ts[i].grad;
+        e.out = ts[i].out;
+        e.count = ts[i].count;
+        e.chunk0 = static_cast<uint32_t>(chunks);
+        e.type = static_cast<uint16_t>(ts[i].dtype);
+        e.out_type = static_cast<uint16_t>(ts[i].out_dtype);
+        chunks += (ts[i].count + kChunk - 1u) / kChunk;
+    }
+    t.chunks = static_cast<uint32_t>(chunks);
+    t.blocks = std::max(1u, std::min(t.chunks, cap_blocks));
+}
+uint64_t group_chunks(const NerfB200GradTensor* ts, uint32_t n) {
+    uint64_t c = 0;
+    for (uint32_t i = 0; i < n; ++i) c += (ts[i].count + kChunk - 1u) / kChunk;
+    return c;
+}
+
+// Both passes over the list, `kTable` tensors a launch (16 where that is
+// enough: the table travels with every launch).
+template <uint32_t CAP>
+cudaError_t squares(const NerfB200GradTensor* ts, uint32_t n, uint32_t blocks, GradPartial* out, uint32_t* used, cudaStream_t s) {
+    GradTable<CAP> t;
+    fill_table(t, ts, n, blocks);
+    k_grad_squares<CAP><<<t.blocks, kThreads, 0, s>>>(t, out);
+    *used = t.blocks;
+    return cudaGetLastError();
+}
+template <uint32_t CAP>
+cudaError_t scales(const NerfB200GradTensor* ts, uint32_t n, uint32_t blocks, const GradPartial* p, uint32_t n_partials, float loss_scale,
+                   float max_norm, GradInfo* info, cudaStream_t s) {
+    GradTable<CAP> t;
+    fill_table(t, ts, n, blocks);
+    k_grad_scale<CAP><<<t.blocks, kThreads, 0, s>>>(t, p, n_partials, loss_scale, max_norm, info);
+    return cudaGetLastError();
+}
+
+uint32_t groups_of(uint32_t n) { return n == 0u ? 1u : (n + kTable - 1u) / kTable; }
+
+NerfStatus norm_and_clip(const NerfB200GradTensor* ts, uint32_t n, float loss_scale, bool clip, float max_norm, NerfB200GradNorm* info,
+                         void* workspace, uint64_t workspace_bytes, cudaStream_t s) {
+    if ((n && !ts) || !info || !workspace || !(loss_scale > 0.0f) || std::isinf(loss_scale)) return NERF_STATUS_INVALID_USAGE;
+    if (clip && !(max_norm >= 0.0f)) return NERF_STATUS_INVALID_USAGE;
+    if ((reinterpret_cast<uintptr_t>(info) & 3u) || (reinterpret_cast<uintptr_t>(workspace) & 15u)) return NERF_STATUS_INVALID_USAGE;
+    const uint64_t need = nerf_b200_grad_workspace_bytes(n);
+    if (need == 0u || workspace_bytes < need) return NERF_STATUS_INVALID_USAGE;
+    for (uint32_t i = 0; i < n; ++i)
+        if (!valid_tensor(ts[i]) || (clip && !valid_output(ts[i]))) return NERF_STATUS_INVALID_USAGE;
+    for (uint32_t i = 0; i < n; i += kTable)
+        if (group_chunks(ts + i, std::min(kTable, n - i)) > 0x7FFFFFFFull) return NERF_STATUS_INVALID_USAGE;
+    if (clip) {
+        const int apart = outputs_apart(ts, n);
+        if (apart != 1) return apart == 0 ? NERF_STATUS_INVALID_USAGE : NERF_STATUS_FAILURE;
+    }
+    GradPartial* parts = static_cast<GradPartial*>(workspace);
+    GradInfo* gi = reinterpret_cast<GradInfo*>(info);
+    const uint32_t blocks = resident_blocks();
+    uint32_t used = 0;
+    for (uint32_t i = 0; i < n || i == 0u; i += kTable) {
+        const uint32_t k = std::min(kTable, n - i);
+        uint32_t more = 0;
+        const cudaError_t e = k <= 16u ? squares<16u>(ts + i, k, blocks, parts + used, &more, s)
+                                       : squares<kTable>(ts + i, k, blocks, parts + used, &more, s);
+        if (e != cudaSuccess) return NERF_STATUS_CUDA_ERROR;
+        used += more;
+    }
+    if (!clip) {
+        k_grad_finish<<<1, kThreads, 0, s>>>(parts, used, loss_scale, gi);
+        return cudaGetLastError() == cudaSuccess ? NERF_STATUS_OK : NERF_STATUS_CUDA_ERROR;
+    }
+    for (uint32_t i = 0; i < n || i == 0u; i += kTable) {
+        const uint32_t k = std::min(kTable, n - i);
+        const cudaError_t e = k <= 16u ? scales<16u>(ts + i, k, blocks, parts, used, loss_scale, max_norm, gi, s)
+                                       : scales<kTable>(ts + i, k, blocks, parts, used, loss_scale, max_norm, gi, s);
+        if (e != cudaSuccess) return NERF_STATUS_CUDA_ERROR;
+    }
+    return NERF_STATUS_OK;
+}
+
+}  // namespace
+}  // namespace nb
+
+extern "C" {
+
+NERF_API uint64_t nerf_b200_grad_workspace_bytes(uint32_t n_tensors) {
+    return static_cast<uint64_t>(nb::groups_of(n_tensors)) * nb::kMaxBlocks * sizeof(nb::GradPartial);
+}
+
+NERF_API NerfStatus nerf_b200_grad_norm(const NerfB200GradTensor* tensors, uint32_t n_tensors, float loss_scale,
+                                        NerfB200GradNorm* info, void* workspace, uint64_t workspace_bytes, void* stream) {
+    return nb::norm_and_clip(tensors, n_tensors, loss_scale, false, 0.0f, info, workspace, workspace_bytes,
+                             static_cast<cudaStream_t>(stream));
+}
+
+NERF_API NerfStatus nerf_b200_grad_clip(const NerfB200GradTensor* tensors, uint32_t n_tensors, float loss_scale, float max_norm,
+                                        NerfB200GradNorm* info, void* workspace, uint64_t workspace_bytes, void* stream) {
+    return nb::norm_and_clip(tensors, n_tensors, loss_scale, true, max_norm, info, workspace, workspace_bytes,
+                             static_cast<cudaStream_t>(stream));
+}
+
+}  // extern "C"

@@ -1,0 +1,74 @@
+// linear.h -- shapes and launch interface of the dense-layer kernels
+// (internal to libnerf_b200; linear.cu holds the kernels, linear_api.cu the
+// checks and the planning behind the exported functions).
+#pragma once
+#include <cuda.h>
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+namespace nb {
+
+enum LinearAct : uint32_t { kActNone = 0, kActRelu = 1, kActSilu = 2, kActGelu = 3, kActSigmoid = 4, kActCount = 5 };
+
+// A row-major matrix of 16-bit values in global memory.
+struct MatrixView {
+    const void* ptr;
+    uint64_t ld;  // values between rows
+    uint32_t rows, cols;
+    uint32_t vec;  // values that every row start is aligned to: 8 (16 bytes), 2 or 1
+};
+
+// D[m][n] = sum over k of A(m, k) B(n, k), both 16-bit, fp32 accumulation.
+// An operand is stored [M or N][K] (K-major) or [K][M or N] (MN-major).
+struct GemmArgs {
+    MatrixView a, b;
+    uint32_t M, N, K;
+    uint32_t a_mn, b_mn;   // 1: stored [K][.]
+    uint32_t a_box_rows;   // rows of a K-major A box (fewer than 128 when M is)
+    uint32_t tiles_m, tiles_n;
+    uint32_t splits;       // parts of K, each with its own partial result
+    uint32_t k_steps;      // 64-value steps of K
+    uint32_t steps_per_split;
+    uint32_t bf16;
+    uint32_t act;
+    // epilogue of an activation output: y = act(D + bias) + res, pre = D + bias
+    const void* bias;
+    MatrixView res, y, pre;  // ptr null: none
+    // epilogue of a weight gradient: partials when splits > 1, else dw (+)= D
+    float* partials;
+    void* dw;
+    uint32_t dw_f32, dw_vec, accumulate;
+    uint32_t* error;
+};
+
+enum GemmKind : int { kGemmRows = 0, kGemmGrad = 1 };
+
+cudaError_t launch_gemm(const GemmArgs& g, int kind, uint32_t bn, const CUtensorMap* map_a, const CUtensorMap* map_b,
+                        bool plain_loads, uint32_t blocks, cudaStream_t s);
+// dz = dy act'(pre) (16-bit, rows dz_ld apart; null: not written), and the
+// column sums of dz before rounding over each of `parts` row ranges
+// ([parts][cols] fp32; null: none).
+struct DzArgs {
+    MatrixView dy, pre;
+    void* dz;
+    uint64_t dz_ld;
+    float* db_part;
+    uint32_t parts, rows_per_part;
+    uint32_t bf16, act;
+};
+cudaError_t launch_dz(const DzArgs& a, cudaStream_t s);
+// dw (+)= sum of the splits' partial tiles, db (+)= sum of the row parts.
+struct GradReduceArgs {
+    const float* partials;
+    uint32_t splits, tiles_m, tiles_n, bn, n_out, n_in;
+    const float* db_part;
+    uint32_t parts;
+    void *dw, *db;  // null: none
+    uint32_t f32, bf16, accumulate;
+};
+cudaError_t launch_grad_reduce(const GradReduceArgs& a, cudaStream_t s);
+
+constexpr uint32_t kGemmBM = 128, kGemmBK = 64;
+
+}  // namespace nb

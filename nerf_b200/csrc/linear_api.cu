@@ -1,0 +1,344 @@
+// linear_api.cu -- the exported dense-layer functions: argument checks, the
+// plan of each product (tile width, parts of K, workspace) and the launches.
+#include <mutex>
+
+#include "../../include/nerf_b200.h"
+#include "linear.h"
+
+namespace nb {
+namespace {
+
+constexpr uint32_t kMaxWidth = 1u << 20;        // n_in, n_out
+constexpr uint32_t kMaxRows = 0x7FFFFFFFu;      // tensor-copy coordinates are signed 32-bit
+constexpr uint64_t kMaxLd = 1ull << 30;         // row strides of the tensor copies stay far below their 2^40 bytes
+
+uint64_t up(uint64_t v, uint64_t a) { return (v + a - 1u) / a * a; }
+uint32_t ceil_div(uint64_t a, uint64_t b) { return static_cast<uint32_t>((a + b - 1u) / b); }
+bool aligned(const void* p, uint64_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1u)) == 0u; }
+
+// SMs of the current device; without a device the B200's.
+uint32_t current_sms() {
+    static std::mutex mu;
+    static uint32_t sms[64];
+    int dev = 0, n = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) {
+        cudaGetLastError();
+        return 148u;
+    }
+    std::lock_guard<std::mutex> lk(mu);
+    if (sms[dev] == 0u) {
+        if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n < 1) {
+            cudaGetLastError();
+            return 148u;
+        }
+        sms[dev] = static_cast<uint32_t>(n);
+    }
+    return sms[dev];
+}
+
+// Whether a kernel of the current device may read or write p: its own device
+// memory or managed memory.
+bool usable(const void* p, int dev) {
+    if (!p) return true;
+    cudaPointerAttributes at{};
+    if (cudaPointerGetAttributes(&at, p) != cudaSuccess) {
+        cudaGetLastError();
+        return false;
+    }
+    return at.type == cudaMemoryTypeManaged || (at.type == cudaMemoryTypeDevice && at.device == dev);
+}
+
+MatrixView view(const void* p, uint64_t ld, uint64_t rows, uint32_t cols) {
+    MatrixView v{};
+    v.ptr = p;
+    v.rows = static_cast<uint32_t>(rows);
+    v.cols = cols;
+    v.ld = rows > 1u ? ld : up(cols, 8u);  // of a single row the distance to the next says nothing
+    v.vec = aligned(p, 16u) && v.ld % 8u == 0u ? 8u : aligned(p, 4u) && v.ld % 2u == 0u ? 2u : 1u;
+    return v;
+}
+
+// ---------------------------------------------------------- tensor copy maps
+using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                                 const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                 CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeTiled encode_tiled() {
+    static const EncodeTiled fn = [] {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult res{};
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &res) != cudaSuccess ||
+            res != cudaDriverEntryPointSuccess) {
+            cudaGetLastError();
+            p = nullptr;
+        }
+        return reinterpret_cast<EncodeTiled>(p);
+    }();
+    return fn;
+}
+// Boxes of box_rows x 64 values of a matrix, 128-byte swizzle, zero outside it.
+bool make_map(CUtensorMap* map, const MatrixView& m, uint32_t box_rows, bool bf16) {
+    const EncodeTiled fn = encode_tiled();
+    if (!fn) return false;
+    const cuuint64_t dims[2] = {m.cols, m.rows};
+    const cuuint64_t strides[1] = {m.ld * 2u};
+    const cuuint32_t box[2] = {64u, box_rows}, elem[2] = {1u, 1u};
+    return fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2u, const_cast<void*>(m.ptr), dims, strides,
+              box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// ------------------------------------------------------------------- plans
+// Tile width of an activation product: the number of waves of 128 x bn tiles
+// times the time of one, which grows with bn and has a part (the row panel's
+// copy) that does not.
+uint32_t pick_bn(uint32_t tiles_m, uint32_t n, uint32_t sms) {
+    uint32_t best = 256u;
+    uint64_t cost = ~0ull;
+    for (uint32_t bn = 256u; bn >= 64u; bn /= 2u) {
+        if (bn > 64u && bn / 2u >= n) continue;  // half of it holds every column
+        const uint64_t tiles = static_cast<uint64_t>(tiles_m) * ceil_div(n, bn);
+        const uint64_t c = ((tiles + sms - 1u) / sms) * (bn + 64u);
+        if (c < cost) {
+            cost = c;
+            best = bn;
+        }
+    }
+    return best;
+}
+
+struct BackwardPlan {
+    uint32_t sms;
+    bool dz_needed;                     // dz is not dy itself
+    uint64_t dz_ld;
+    uint32_t parts, rows_per_part;      // row ranges of the column sums
+    uint32_t bn, tiles_m, tiles_n, splits, k_steps, steps_per_split;  // weight gradient
+    uint64_t o_dz, o_db, o_dw, bytes;   // workspace
+};
+BackwardPlan plan_backward(const NerfB200Linear& d) {
+    BackwardPlan p{};
+    p.sms = current_sms();
+    p.dz_needed = d.activation != kActNone;
+    p.dz_ld = up(d.n_out, 8u);
+    // About six 256-thread blocks an SM, each with at least 64 rows.
+    const uint32_t groups = ceil_div(d.n_out, 8u), gx = ceil_div(groups, 32u);
+    uint64_t parts = 6ull * p.sms / gx;
+    if (parts > ceil_div(d.n_rows, 64u)) parts = ceil_div(d.n_rows, 64u);
+    if (parts < 1u) parts = 1u;
+    p.rows_per_part = ceil_div(d.n_rows, parts);
+    if (p.rows_per_part == 0u) p.rows_per_part = 1u;
+    p.parts = ceil_div(d.n_rows, p.rows_per_part);
+    p.bn = d.n_in <= 64u ? 64u : d.n_in <= 128u ? 128u : 256u;
+    p.tiles_m = ceil_div(d.n_out, kGemmBM);
+    p.tiles_n = ceil_div(d.n_in, p.bn);
+    p.k_steps = ceil_div(d.n_rows, kGemmBK);
+    // One wave of (tile, row range) items, each range at least four steps.
+    const uint64_t tiles = static_cast<uint64_t>(p.tiles_m) * p.tiles_n;
+    uint64_t splits = tiles >= p.sms ? 1u : p.sms / tiles;
+    if (splits > ceil_div(p.k_steps, 4u)) splits = ceil_div(p.k_steps, 4u);
+    if (splits < 1u) splits = 1u;
+    p.steps_per_split = ceil_div(p.k_steps, splits);
+    p.splits = p.steps_per_split ? ceil_div(p.k_steps, p.steps_per_split) : 1u;
+    uint64_t at = 0;
+    p.o_dz = at;
+    if (p.dz_needed) at += up(static_cast<uint64_t>(d.n_rows) * p.dz_ld * 2u, 256u);
+    p.o_db = at;
+    at += up(static_cast<uint64_t>(p.parts) * d.n_out * 4u, 256u);
+    p.o_dw = at;
+    if (p.splits > 1u) at += static_cast<uint64_t>(p.splits) * tiles * kGemmBM * p.bn * 4u;
+    p.bytes = at ? at : 256u;
+    return p;
+}
+
+uint64_t ld_or(uint64_t ld, uint32_t tight) { return ld ? ld : tight; }
+
+bool valid_shape(const NerfB200Linear& d) {
+    if (d.dtype != NERF_B200_F16 && d.dtype != NERF_B200_BF16) return false;
+    if (d.activation >= kActCount || d.accumulate > 1u || d.reserved != 0u) return false;
+    if (d.grad_dtype != NERF_B200_F32 && d.grad_dtype != d.dtype) return false;
+    if (d.n_rows > kMaxRows || d.n_in == 0u || d.n_out == 0u || d.n_in > kMaxWidth || d.n_out > kMaxWidth) return false;
+    const uint64_t in[] = {d.ld_x, d.ld_weight, d.ld_dx}, out[] = {d.ld_y, d.ld_pre, d.ld_dy};
+    for (uint64_t l : in)
+        if (l && (l < d.n_in || l > kMaxLd)) return false;
+    for (uint64_t l : out)
+        if (l && (l < d.n_out || l > kMaxLd)) return false;
+    return d.ld_residual <= kMaxLd;  // as wide as the output it joins: checked by the calls
+}
+
+// The product with its operands' maps; plain loads where a row does not start
+// on a 16-byte boundary.
+cudaError_t run_gemm(GemmArgs& g, int kind, uint32_t bn, uint32_t sms, cudaStream_t s) {
+    CUtensorMap ma{}, mb{};
+    const bool plain = g.a.vec < 8u || g.b.vec < 8u;
+    g.a_box_rows = g.M >= kGemmBM ? kGemmBM : static_cast<uint32_t>(up(g.M, 8u));
+    if (!plain && (!make_map(&ma, g.a, g.a_mn ? kGemmBK : g.a_box_rows, g.bf16 != 0u) ||
+                   !make_map(&mb, g.b, g.b_mn ? kGemmBK : bn, g.bf16 != 0u)))
+        return cudaErrorNotSupported;
+    const uint64_t items = static_cast<uint64_t>(g.tiles_m) * g.tiles_n * g.splits;
+    return launch_gemm(g, kind, bn, &ma, &mb, plain, items < sms ? static_cast<uint32_t>(items) : sms, s);
+}
+
+}  // namespace
+}  // namespace nb
+
+extern "C" {
+
+NERF_API NerfStatus nerf_b200_linear_forward(const NerfB200Linear* desc, const void* x, const void* weight, const void* bias,
+                                             const void* residual, void* y, void* pre, uint32_t* error_word, void* stream) {
+    using namespace nb;
+    if (!desc || !valid_shape(*desc)) return NERF_STATUS_INVALID_USAGE;
+    const NerfB200Linear& d = *desc;
+    if (residual && d.ld_residual && d.ld_residual < d.n_out) return NERF_STATUS_INVALID_USAGE;
+    if (d.n_rows == 0u) return NERF_STATUS_OK;
+    if (!x || !weight || !y || !error_word) return NERF_STATUS_INVALID_USAGE;
+    const void* all[] = {x, weight, bias, residual, y, pre};
+    for (const void* p : all)
+        if (!aligned(p, 2u)) return NERF_STATUS_INVALID_USAGE;
+    if (!aligned(error_word, 4u)) return NERF_STATUS_INVALID_USAGE;
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return NERF_STATUS_CUDA_ERROR;
+    for (const void* p : all)
+        if (!usable(p, dev)) return NERF_STATUS_INVALID_USAGE;
+    if (!usable(error_word, dev)) return NERF_STATUS_INVALID_USAGE;
+
+    const uint32_t sms = current_sms();
+    GemmArgs g{};
+    g.M = d.n_rows;
+    g.N = d.n_out;
+    g.K = d.n_in;
+    g.a = view(x, ld_or(d.ld_x, d.n_in), d.n_rows, d.n_in);
+    g.b = view(weight, ld_or(d.ld_weight, d.n_in), d.n_out, d.n_in);
+    g.tiles_m = ceil_div(g.M, kGemmBM);
+    const uint32_t bn = pick_bn(g.tiles_m, g.N, sms);
+    g.tiles_n = ceil_div(g.N, bn);
+    g.splits = 1u;
+    g.k_steps = g.steps_per_split = ceil_div(g.K, kGemmBK);
+    g.bf16 = d.dtype == NERF_B200_BF16;
+    g.act = d.activation;
+    g.bias = bias;
+    g.res = view(residual, ld_or(d.ld_residual, d.n_out), d.n_rows, d.n_out);
+    g.y = view(y, ld_or(d.ld_y, d.n_out), d.n_rows, d.n_out);
+    g.pre = view(pre, ld_or(d.ld_pre, d.n_out), d.n_rows, d.n_out);
+    g.error = error_word;
+    return run_gemm(g, kGemmRows, bn, sms, static_cast<cudaStream_t>(stream)) == cudaSuccess ? NERF_STATUS_OK : NERF_STATUS_CUDA_ERROR;
+}
+
+NERF_API uint64_t nerf_b200_linear_backward_workspace_bytes(const NerfB200Linear* desc) {
+    if (!desc || !nb::valid_shape(*desc)) return 0u;
+    return nb::plan_backward(*desc).bytes;
+}
+
+NERF_API NerfStatus nerf_b200_linear_backward(const NerfB200Linear* desc, const void* x, const void* weight, const void* pre,
+                                              const void* dy, const void* dx_residual, void* dx, void* dweight, void* dbias,
+                                              void* workspace, uint64_t workspace_bytes, uint32_t* error_word, void* stream) {
+    using namespace nb;
+    if (!desc || !valid_shape(*desc)) return NERF_STATUS_INVALID_USAGE;
+    const NerfB200Linear& d = *desc;
+    if (dx_residual && d.ld_residual && d.ld_residual < d.n_in) return NERF_STATUS_INVALID_USAGE;
+    if (!dx && !dweight && !dbias) return NERF_STATUS_OK;
+    const uint64_t es = d.grad_dtype == NERF_B200_F32 ? 4u : 2u;
+    if (!aligned(dweight, es) || !aligned(dbias, es)) return NERF_STATUS_INVALID_USAGE;
+    const cudaStream_t s = static_cast<cudaStream_t>(stream);
+    int dev = 0;
+    if (d.n_rows == 0u) {  // sums over no rows
+        if (cudaGetDevice(&dev) != cudaSuccess) return NERF_STATUS_CUDA_ERROR;
+        if (!usable(dweight, dev) || !usable(dbias, dev)) return NERF_STATUS_INVALID_USAGE;
+        if (d.accumulate) return NERF_STATUS_OK;
+        if (dweight && cudaMemsetAsync(dweight, 0, es * d.n_out * d.n_in, s) != cudaSuccess) return NERF_STATUS_CUDA_ERROR;
+        if (dbias && cudaMemsetAsync(dbias, 0, es * d.n_out, s) != cudaSuccess) return NERF_STATUS_CUDA_ERROR;
+        return NERF_STATUS_OK;
+    }
+    if (!dy || !error_word || !workspace || (dx && !weight) || (dweight && !x) || (d.activation != kActNone && !pre))
+        return NERF_STATUS_INVALID_USAGE;
+    const void* all[] = {x, weight, pre, dy, dx_residual, dx, dweight, dbias};
+    for (const void* p : all)
+        if (!aligned(p, 2u)) return NERF_STATUS_INVALID_USAGE;
+    if (!aligned(workspace, 256u) || !aligned(error_word, 4u)) return NERF_STATUS_INVALID_USAGE;
+    const BackwardPlan p = plan_backward(d);
+    if (workspace_bytes < p.bytes) return NERF_STATUS_INVALID_USAGE;
+    if (cudaGetDevice(&dev) != cudaSuccess) return NERF_STATUS_CUDA_ERROR;
+    for (const void* q : all)
+        if (!usable(q, dev)) return NERF_STATUS_INVALID_USAGE;
+    if (!usable(workspace, dev) || !usable(error_word, dev)) return NERF_STATUS_INVALID_USAGE;
+
+    unsigned char* ws = static_cast<unsigned char*>(workspace);
+    const uint32_t bf16 = d.dtype == NERF_B200_BF16;
+    const MatrixView dyv = view(dy, ld_or(d.ld_dy, d.n_out), d.n_rows, d.n_out);
+    const bool dz_written = p.dz_needed && (dx || dweight);
+    const MatrixView dzv = p.dz_needed ? view(ws + p.o_dz, p.dz_ld, d.n_rows, d.n_out) : dyv;
+    if (dz_written || dbias) {
+        DzArgs a{};
+        a.dy = dyv;
+        a.pre = view(pre, ld_or(d.ld_pre, d.n_out), d.n_rows, d.n_out);
+        a.dz = dz_written ? ws + p.o_dz : nullptr;
+        a.dz_ld = p.dz_ld;
+        a.db_part = dbias ? reinterpret_cast<float*>(ws + p.o_db) : nullptr;
+        a.parts = p.parts;
+        a.rows_per_part = p.rows_per_part;
+        a.bf16 = bf16;
+        a.act = d.activation;
+        if (launch_dz(a, s) != cudaSuccess) return NERF_STATUS_CUDA_ERROR;
+    }
+    if (dx) {
+        GemmArgs g{};
+        g.M = d.n_rows;
+        g.N = d.n_in;
+        g.K = d.n_out;
+        g.a = dzv;
+        g.b = view(weight, ld_or(d.ld_weight, d.n_in), d.n_out, d.n_in);
+        g.b_mn = 1u;
+        g.tiles_m = ceil_div(g.M, kGemmBM);
+        const uint32_t bn = pick_bn(g.tiles_m, g.N, p.sms);
+        g.tiles_n = ceil_div(g.N, bn);
+        g.splits = 1u;
+        g.k_steps = g.steps_per_split = ceil_div(g.K, kGemmBK);
+        g.bf16 = bf16;
+        g.res = view(dx_residual, ld_or(d.ld_residual, d.n_in), d.n_rows, d.n_in);
+        g.y = view(dx, ld_or(d.ld_dx, d.n_in), d.n_rows, d.n_in);
+        g.error = error_word;
+        if (run_gemm(g, kGemmRows, bn, p.sms, s) != cudaSuccess) return NERF_STATUS_CUDA_ERROR;
+    }
+    GradReduceArgs r{};
+    r.n_out = d.n_out;
+    r.n_in = d.n_in;
+    r.f32 = d.grad_dtype == NERF_B200_F32;
+    r.bf16 = bf16;
+    r.accumulate = d.accumulate;
+    if (dweight) {
+        GemmArgs g{};
+        g.M = d.n_out;
+        g.N = d.n_in;
+        g.K = d.n_rows;
+        g.a = dzv;
+        g.b = view(x, ld_or(d.ld_x, d.n_in), d.n_rows, d.n_in);
+        g.a_mn = g.b_mn = 1u;
+        g.tiles_m = p.tiles_m;
+        g.tiles_n = p.tiles_n;
+        g.splits = p.splits;
+        g.k_steps = p.k_steps;
+        g.steps_per_split = p.steps_per_split;
+        g.bf16 = bf16;
+        g.partials = reinterpret_cast<float*>(ws + p.o_dw);
+        g.dw = dweight;
+        g.dw_f32 = r.f32;
+        g.dw_vec = aligned(dweight, 16u) && (es * d.n_in) % 16u == 0u;
+        g.accumulate = d.accumulate;
+        g.error = error_word;
+        if (run_gemm(g, kGemmGrad, p.bn, p.sms, s) != cudaSuccess) return NERF_STATUS_CUDA_ERROR;
+        if (p.splits > 1u) {
+            r.partials = g.partials;
+            r.splits = p.splits;
+            r.tiles_m = p.tiles_m;
+            r.tiles_n = p.tiles_n;
+            r.bn = p.bn;
+            r.dw = dweight;
+        }
+    }
+    if (dbias) {
+        r.db_part = reinterpret_cast<float*>(ws + p.o_db);
+        r.parts = p.parts;
+        r.db = dbias;
+    }
+    return launch_grad_reduce(r, s) == cudaSuccess ? NERF_STATUS_OK : NERF_STATUS_CUDA_ERROR;
+}
+
+}  // extern "C"
