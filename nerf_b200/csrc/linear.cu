@@ -13,10 +13,15 @@
 // k_gemm: persistent CTAs, one 128 x BN tile (or one part of its K range) at
 // a time.  Warp 0 copies operand boxes into a ring of shared-memory stages,
 // one thread of warp 1 issues the MMAs into one of two tensor-memory
-// accumulators, warps 4-7 drain the other one: the copies, the products and
-// the epilogue of the tile before overlap.  Matrices whose rows do not start
-// on 16-byte boundaries cannot be copied by the tensor copy unit; four more
-// warps load them instead (plain_loads).
+// accumulators, and two groups of four warps drain them in turn: the copies,
+// the products and the epilogues of the two tiles before overlap.
+//   kFeedTma    one CTA a tile.
+//   kFeedPair   two CTAs on one 256 x 256 tile: each holds its 128 rows of A
+//               and half of B, so the tensor cores read 8 KB of shared memory
+//               per 64 cycles of MMA and SM instead of 12 KB, more than it
+//               delivers (128 bytes a cycle).
+//   kFeedPlain  rows that do not start on 16-byte boundaries, which the tensor
+//               copy unit cannot address: eight more warps load them.
 #include <cuda_bf16.h>
 
 #include <atomic>
@@ -29,14 +34,9 @@ namespace {
 
 constexpr uint32_t kBM = kGemmBM, kBK = kGemmBK;
 constexpr uint32_t kStageBytesA = kBM * 128u;
-constexpr uint32_t kEpiWarps = 4;
 constexpr uint32_t kSlabBytes = 32u * 128u;  // one epilogue warp's 32 rows x 128 bytes
 constexpr uint32_t kMaxStages = 8;
 
-__host__ __device__ constexpr uint32_t gemm_stages(uint32_t bn) { return bn >= 256u ? 4u : bn >= 128u ? 6u : 8u; }
-__host__ __device__ constexpr uint32_t gemm_smem(uint32_t bn) {
-    return 1024u + gemm_stages(bn) * (kStageBytesA + bn * 128u) + kEpiWarps * kSlabBytes + bn * 4u;
-}
 __host__ __device__ constexpr uint32_t tmem_cols(uint32_t n) { return n <= 32u ? 32u : n <= 64u ? 64u : n <= 128u ? 128u : n <= 256u ? 256u : 512u; }
 
 // ------------------------------------------------------------ 16-bit values
@@ -156,34 +156,61 @@ NB_DEV void slab_put(unsigned char* slab, uint32_t row, uint32_t piece, const ui
 }
 
 // ------------------------------------------------------------- operand boxes
+constexpr uint32_t kLoadWarps = 8;
+
 // `rows` x 64 values at (row0, col0) of a matrix -> a swizzled box, zero
-// outside the matrix, by 128 threads.
+// outside the matrix, by kLoadWarps warps.
 NB_DEV void fill_box(unsigned char* box, const MatrixView& m, uint32_t row0, uint32_t rows, uint32_t col0, uint32_t tid) {
     const uint16_t* base = static_cast<const uint16_t*>(m.ptr);
-#pragma unroll 2
-    for (uint32_t c = tid; c < rows * 8u; c += 128u) {
-        const uint32_t r = c >> 3, p = c & 7u;
-        const uint64_t gr = static_cast<uint64_t>(row0) + r;
-        const uint32_t gc = col0 + 8u * p;
-        uint32_t w[4] = {0u, 0u, 0u, 0u};
-        if (gr < m.rows && gc < m.cols) {
-            const uint16_t* q = base + gr * m.ld + gc;
-            const uint32_t have = min(8u, m.cols - gc);
-            if (m.vec >= 8u && have == 8u) {
-                const uint4 u = *reinterpret_cast<const uint4*>(q);
-                w[0] = u.x; w[1] = u.y; w[2] = u.z; w[3] = u.w;
-            } else if (m.vec >= 2u && have == 8u) {
+    const uint32_t have = col0 < m.cols ? min(64u, m.cols - col0) : 0u;
+    if (m.vec >= 8u && (have & 7u) == 0u) {
+        // Whole 16-byte pieces: eight threads a row.
+#pragma unroll 4
+        for (uint32_t c = tid; c < rows * 8u; c += kLoadWarps * 32u) {
+            const uint32_t r = c >> 3, p = c & 7u;
+            const uint64_t gr = static_cast<uint64_t>(row0) + r;
+            uint4 u = make_uint4(0u, 0u, 0u, 0u);
+            if (gr < m.rows && 8u * p < have) u = *reinterpret_cast<const uint4*>(base + gr * m.ld + col0 + 8u * p);
+            *reinterpret_cast<uint4*>(box + slab_at(r, p)) = u;
+        }
+        return;
+    }
+    // A warp a row, lane i the values 2 i and 2 i + 1.  A row that starts
+    // between two 32-bit words is read as the words around it: lane i reads
+    // values 2 i - 1 and 2 i and takes 2 i + 1 from its neighbour's word.  No
+    // word reaches outside the row's values: the ends are 16-bit loads.
+    const uint32_t lane = tid & 31u, warp = tid >> 5;
+    constexpr uint32_t kBatch = 8;  // rows in flight a warp
+    for (uint32_t r0 = warp; r0 < rows; r0 += kLoadWarps * kBatch) {
+        uint32_t w[kBatch], odd[kBatch];
+        uint16_t last[kBatch];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) w[i] = reinterpret_cast<const uint32_t*>(q)[i];
+        for (uint32_t j = 0; j < kBatch; ++j) {
+            const uint32_t r = r0 + j * kLoadWarps;
+            const uint64_t gr = static_cast<uint64_t>(row0) + r;
+            const uint16_t* q = base + gr * m.ld + col0;
+            const bool live = r < rows && gr < m.rows;
+            odd[j] = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(q) >> 1) & 1u;
+            const uint32_t nv = live ? have : 0u;
+            w[j] = 0u;
+            last[j] = 0u;
+            if (odd[j]) {
+                if (lane > 0u && 2u * lane < nv) w[j] = *reinterpret_cast<const uint32_t*>(q + 2u * lane - 1u);
+                else if (lane == 0u && nv > 0u) w[j] = static_cast<uint32_t>(q[0]) << 16;
+                else if (lane > 0u && 2u * lane - 1u < nv) w[j] = q[2u * lane - 1u];
+                if (lane == 31u && nv == 64u) last[j] = q[63];
             } else {
-                uint16_t h[8];
-#pragma unroll
-                for (uint32_t i = 0; i < 8u; ++i) h[i] = i < have ? q[i] : static_cast<uint16_t>(0);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) w[i] = static_cast<uint32_t>(h[2 * i]) | (static_cast<uint32_t>(h[2 * i + 1]) << 16);
+                if (2u * lane + 1u < nv) w[j] = *reinterpret_cast<const uint32_t*>(q + 2u * lane);
+                else if (2u * lane < nv) w[j] = q[2u * lane];
             }
         }
-        *reinterpret_cast<uint4*>(box + slab_at(r, p)) = make_uint4(w[0], w[1], w[2], w[3]);
+#pragma unroll
+        for (uint32_t j = 0; j < kBatch; ++j) {
+            const uint32_t r = r0 + j * kLoadWarps;
+            const uint32_t next = __shfl_down_sync(0xffffffffu, w[j], 1);
+            if (odd[j]) w[j] = (w[j] >> 16) | ((lane == 31u ? static_cast<uint32_t>(last[j]) : next) << 16);
+            if (r < rows) *reinterpret_cast<uint32_t*>(box + slab_at(r, lane >> 2) + 4u * (lane & 3u)) = w[j];
+        }
     }
 }
 
@@ -204,53 +231,123 @@ NB_DEV void tile_of(const GemmArgs& g, uint32_t t, uint32_t& tm, uint32_t& tn) {
     tn = r / gm;
 }
 
-template <uint32_t BN, int KIND, bool PLAIN>
-__global__ void __launch_bounds__(PLAIN ? 384 : 256, 1)
-    k_gemm(const GemmArgs g, const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b) {
-    constexpr uint32_t kStages = gemm_stages(BN);
-    constexpr uint32_t kStageBytes = kStageBytesA + BN * 128u;
+// 32 accumulator columns of this thread's row plus the bias.
+NB_DEV void load_z(float (&v)[32], uint32_t taddr, const uint16_t* bias, bool bf16) {
+    umma::tmem_ld32(taddr, v);
+#pragma unroll
+    for (uint32_t i = 0; i < 4u; ++i) {
+        const uint4 u = *reinterpret_cast<const uint4*>(bias + 8u * i);
+        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float2 b = unpack_16(w[j], bf16);
+            v[8 * i + 2 * j] += b.x;
+            v[8 * i + 2 * j + 1] += b.y;
+        }
+    }
+}
+// 32 values -> pieces 4 h .. 4 h + 3 of this thread's slab row.
+NB_DEV void slab_put32(unsigned char* slab, uint32_t lane, uint32_t h, const float (&v)[32], bool bf16) {
+#pragma unroll
+    for (uint32_t p = 0; p < 4u; ++p) {
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = pack_16(v[8 * p + 2 * i], v[8 * p + 2 * i + 1], bf16);
+        slab_put(slab, lane, 4u * h + p, w);
+    }
+}
+
+// The warp's slab -> 32 rows x 64 columns at (row, col) of an output.
+NB_DEV void slab_out(unsigned char* slab, const MatrixView& m, bool by_tma, const CUtensorMap* map, uint32_t row, uint32_t col,
+                     uint32_t rows, uint32_t cols, uint32_t lane) {
+    if (by_tma) {
+        umma::fence_async_smem();
+        __syncwarp();
+        if (lane == 0u) {
+            tma::store_2d(map, smem_u32(slab), static_cast<int32_t>(col), static_cast<int32_t>(row));
+            tma::store_commit();
+        }
+    } else {
+        __syncwarp();
+        unsigned char* dst = static_cast<unsigned char*>(const_cast<void*>(m.ptr)) + 2u * (row * m.ld + col);
+        slab_copy<2, true>(slab, dst, m.ld, rows, cols, m.vec >= 8u, lane);
+        __syncwarp();
+    }
+}
+
+template <uint32_t BN, int KIND, int FEED>
+struct GemmShape {
+    static constexpr bool kPair = FEED == kFeedPair, kPlain = FEED == kFeedPlain;
+    static constexpr uint32_t kBoxN = kPair ? BN / 2u : BN;  // rows of B in this CTA's shared memory
+    static constexpr uint32_t kStageBytes = kStageBytesA + kBoxN * 128u;
+    static constexpr uint32_t kStages = kPair ? 5u : BN >= 256u ? 4u : BN >= 128u ? 4u : 5u;
+    static constexpr uint32_t kSlabs = kPair ? 2u : BN >= 256u ? 1u : 2u;  // per epilogue warp
+    static constexpr uint32_t kSmem = 1024u + kStages * kStageBytes + 8u * kSlabs * kSlabBytes + 2u * BN * 2u;
+    static constexpr uint32_t kThreads = kPlain ? 384u + 32u * kLoadWarps : 384u;
+    static_assert(kSmem <= 232448u - 512u, "shared memory of one CTA");
+};
+
+// Warps: 0 operand copies, 1 MMA, 2 tensor-memory allocation, 4-7 and 8-11 two
+// epilogue groups that take turns (item i of the CTA: group and accumulator
+// i & 1), 12.. operand loads (kFeedPlain).
+template <uint32_t BN, int KIND, int FEED>
+__global__ void __launch_bounds__(GemmShape<BN, KIND, FEED>::kThreads, 1) k_gemm(const GemmArgs g, const __grid_constant__ GemmMaps maps) {
+    using S = GemmShape<BN, KIND, FEED>;
+    constexpr uint32_t kStages = S::kStages, kStageBytes = S::kStageBytes;
+    constexpr uint32_t kCols = tmem_cols(2u * BN);
+    constexpr uint32_t kCtas = S::kPair ? 2u : 1u;
     extern __shared__ unsigned char smem_raw[];
     __shared__ Barriers bar;
     unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     unsigned char* slabs = smem + kStages * kStageBytes;
-    float* bias_s = reinterpret_cast<float*>(slabs + kEpiWarps * kSlabBytes);
+    uint16_t* bias_all = reinterpret_cast<uint16_t*>(slabs + 8u * S::kSlabs * kSlabBytes);
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
     const bool bf16 = g.bf16 != 0u;
+    const uint32_t rank = S::kPair ? tma::cluster_rank() : 0u;
+    const uint32_t first_item = blockIdx.x / kCtas, item_step = gridDim.x / kCtas;
 
     if (threadIdx.x == 0u) {
         for (uint32_t i = 0; i < kStages; ++i) {
-            umma::mbar_init(&bar.full[i], PLAIN ? 128u : 1u);
+            umma::mbar_init(&bar.full[i], S::kPlain ? 32u * kLoadWarps : 1u);
             umma::mbar_init(&bar.empty[i], 1u);
         }
         for (uint32_t i = 0; i < 2u; ++i) {
             umma::mbar_init(&bar.acc_full[i], 1u);
-            umma::mbar_init(&bar.acc_empty[i], kEpiWarps);
+            umma::mbar_init(&bar.acc_empty[i], 4u * kCtas);
         }
         umma::mbar_init(&bar.drain, 1u);
         umma::fence_mbar_init();
-        if (!PLAIN) {
-            tma::prefetch_map(&map_a);
-            tma::prefetch_map(&map_b);
+        if (!S::kPlain) {
+            tma::prefetch_map(&maps.a);
+            tma::prefetch_map(&maps.b);
         }
+        if (KIND == kGemmRows && g.y_tma) tma::prefetch_map(&maps.y);
     }
     if (warp == 2u) {
-        umma::tmem_alloc(&bar.tmem_base, tmem_cols(2u * BN));
-        umma::tmem_relinquish();
+        if (S::kPair) {
+            tma::tmem_alloc_pair(&bar.tmem_base, kCols);
+            tma::tmem_relinquish_pair();
+        } else {
+            umma::tmem_alloc(&bar.tmem_base, kCols);
+            umma::tmem_relinquish();
+        }
     }
     umma::fence_before_sync();
     __syncthreads();
+    if (S::kPair) tma::cluster_sync();  // the other CTA's barriers exist before anything signals them
     umma::fence_after_sync();
     const uint32_t tmem = bar.tmem_base;
     const uint32_t tiles = g.tiles_m * g.tiles_n, items = tiles * g.splits;
 
-    if ((!PLAIN && warp == 0u && lane == 0u) || (PLAIN && warp >= 8u)) {
-        // ---- producer: one thread issuing tensor copies, or four warps of plain loads
+    if ((!S::kPlain && warp == 0u && lane == 0u) || (S::kPlain && warp >= 12u)) {
+        // ---- producer: one thread issuing tensor copies, or warps of loads
         uint32_t stage = 0, parity = 1u, issued = 0;
         bool ok = true;
-        for (uint32_t it = blockIdx.x; it < items && ok; it += gridDim.x) {
+        for (uint32_t it = first_item; it < items && ok; it += item_step) {
             const uint32_t split = it / tiles;
             uint32_t tm, tn;
             tile_of(g, it - split * tiles, tm, tn);
+            const uint32_t m0 = (tm * kCtas + rank) * kBM, n0 = tn * BN + rank * S::kBoxN;
             const uint32_t ks1 = min(g.k_steps, (split + 1u) * g.steps_per_split);
             for (uint32_t ks = split * g.steps_per_split; ks < ks1; ++ks) {
                 if (!tma::wait(&bar.empty[stage], parity)) {
@@ -259,9 +356,9 @@ __global__ void __launch_bounds__(PLAIN ? 384 : 256, 1)
                 }
                 unsigned char* sa = smem + stage * kStageBytes;
                 unsigned char* sb = sa + kStageBytesA;
-                const uint32_t k0 = ks * kBK, m0 = tm * kBM, n0 = tn * BN;
-                if (PLAIN) {
-                    const uint32_t tid = threadIdx.x - 256u;
+                const uint32_t k0 = ks * kBK;
+                if (S::kPlain) {
+                    const uint32_t tid = threadIdx.x - 384u;
                     if (g.a_mn) {
                         for (uint32_t j = 0; j < kBM / 64u; ++j) fill_box(sa + j * 8192u, g.a, k0, kBK, m0 + 64u * j, tid);
                     } else {
@@ -275,19 +372,23 @@ __global__ void __launch_bounds__(PLAIN ? 384 : 256, 1)
                     umma::fence_async_smem();
                     tma::arrive(&bar.full[stage]);
                 } else {
-                    const uint32_t bytes_a = g.a_mn ? kStageBytesA : g.a_box_rows * 128u;
-                    tma::expect_tx(&bar.full[stage], bytes_a + BN * 128u);
+                    const uint32_t bytes = (g.a_mn ? kStageBytesA : g.a_box_rows * 128u) + S::kBoxN * 128u;
+                    // Of a pair both CTAs' copies are counted by the leading CTA's barrier.
+                    if (rank == 0u) tma::expect_tx(&bar.full[stage], kCtas * bytes);
+                    const uint32_t full = S::kPair ? tma::peer_addr(smem_u32(&bar.full[stage]), 0u) : 0u;
+                    const auto load = [&](unsigned char* dst, const CUtensorMap* map, uint32_t x, uint32_t y) {
+                        if (S::kPair) tma::load_2d_pair(smem_u32(dst), map, x, y, full);
+                        else tma::load_2d(smem_u32(dst), map, x, y, &bar.full[stage]);
+                    };
                     if (g.a_mn) {
-                        for (uint32_t j = 0; j < kBM / 64u; ++j)
-                            tma::load_2d(smem_u32(sa + j * 8192u), &map_a, m0 + 64u * j, k0, &bar.full[stage]);
+                        for (uint32_t j = 0; j < kBM / 64u; ++j) load(sa + j * 8192u, &maps.a, m0 + 64u * j, k0);
                     } else {
-                        tma::load_2d(smem_u32(sa), &map_a, k0, m0, &bar.full[stage]);
+                        load(sa, &maps.a, k0, m0);
                     }
                     if (g.b_mn) {
-                        for (uint32_t j = 0; j < BN / 64u; ++j)
-                            tma::load_2d(smem_u32(sb + j * 8192u), &map_b, n0 + 64u * j, k0, &bar.full[stage]);
+                        for (uint32_t j = 0; j < S::kBoxN / 64u; ++j) load(sb + j * 8192u, &maps.b, n0 + 64u * j, k0);
                     } else {
-                        tma::load_2d(smem_u32(sb), &map_b, k0, n0, &bar.full[stage]);
+                        load(sb, &maps.b, k0, n0);
                     }
                 }
                 ++issued;
@@ -299,16 +400,16 @@ __global__ void __launch_bounds__(PLAIN ? 384 : 256, 1)
         }
         if (!ok) {
             atomicOr(g.error, 1u);
-            if (!PLAIN)  // this CTA's copies in flight: wait for them before its shared memory goes
+            if (!S::kPlain && rank == 0u)  // copies in flight: wait for them before the shared memory goes
                 for (uint32_t i = issued > kStages ? issued - kStages : 0u; i < issued; ++i)
                     tma::wait(&bar.full[i % kStages], (i / kStages) & 1u);
         }
-    } else if (warp == 1u && lane == 0u) {
-        // ---- MMA issuer
-        const uint32_t idesc = tma::idesc_16bit(kBM, BN, g.a_mn, g.b_mn, g.bf16);
+    } else if (warp == 1u && lane == 0u && rank == 0u) {
+        // ---- MMA issuer (of a pair: the leading CTA's)
+        const uint32_t idesc = tma::idesc_16bit(kBM * kCtas, BN, g.a_mn, g.b_mn, g.bf16);
         uint32_t stage = 0, parity = 0, acc = 0, acc_parity = 1u;
         bool ok = true;
-        for (uint32_t it = blockIdx.x; it < items && ok; it += gridDim.x) {
+        for (uint32_t it = first_item; it < items && ok; it += item_step) {
             const uint32_t split = it / tiles;
             const uint32_t ks0 = split * g.steps_per_split, ks1 = min(g.k_steps, (split + 1u) * g.steps_per_split);
             if (!tma::wait(&bar.acc_empty[acc], acc_parity)) {
@@ -327,40 +428,59 @@ __global__ void __launch_bounds__(PLAIN ? 384 : 256, 1)
                 for (uint32_t k = 0; k < kBK / 16u; ++k) {
                     const uint64_t da = g.a_mn ? tma::desc_sw128(sa + 2048u * k, 8192u, 1024u) : tma::desc_sw128(sa + 32u * k, 16u, 1024u);
                     const uint64_t db = g.b_mn ? tma::desc_sw128(sb + 2048u * k, 8192u, 1024u) : tma::desc_sw128(sb + 32u * k, 16u, 1024u);
-                    umma::mma_f16(tmem + acc * BN, da, db, idesc, (ks > ks0 || k > 0u) ? 1u : 0u);
+                    const uint32_t more = (ks > ks0 || k > 0u) ? 1u : 0u;
+                    if (S::kPair) tma::mma_pair(tmem + acc * BN, da, db, idesc, more);
+                    else umma::mma_f16(tmem + acc * BN, da, db, idesc, more);
                 }
-                umma::commit(&bar.empty[stage]);
+                if (S::kPair) tma::commit_pair(&bar.empty[stage]);
+                else umma::commit(&bar.empty[stage]);
                 if (++stage == kStages) {
                     stage = 0;
                     parity ^= 1u;
                 }
             }
-            if (ok) umma::commit(&bar.acc_full[acc]);
+            if (ok) {
+                if (S::kPair) tma::commit_pair(&bar.acc_full[acc]);
+                else umma::commit(&bar.acc_full[acc]);
+            }
             acc ^= 1u;
             if (acc == 0u) acc_parity ^= 1u;
         }
         if (!ok) {  // the MMAs issued so far end before the tensor memory is freed
             atomicOr(g.error, 1u);
-            umma::commit(&bar.drain);
+            if (S::kPair) tma::commit_pair(&bar.drain);
+            else umma::commit(&bar.drain);
             tma::wait(&bar.drain, 0u);
         }
-    } else if (warp >= 4u && warp < 8u) {
-        // ---- epilogue: warp q drains rows 32 q .. 32 q + 31 of the tile
-        const uint32_t q = warp & 3u, row = 32u * q + lane;
-        unsigned char* slab = slabs + q * kSlabBytes;
-        uint32_t acc = 0, parity = 0;
+    } else if (warp >= 4u && warp < 12u) {
+        // ---- epilogue: warp q of a group drains rows 32 q .. 32 q + 31 of the tile
+        const uint32_t q = warp & 3u, acc = (warp >> 2) - 1u, row = 32u * q + lane;
+        unsigned char* my_slabs = slabs + (warp - 4u) * S::kSlabs * kSlabBytes;
+        uint16_t* bias_s = bias_all + acc * BN;
+        const uint32_t taddr = tmem + acc * BN + ((32u * q) << 16);
+        const uint32_t acc_empty = S::kPair ? tma::peer_addr(smem_u32(&bar.acc_empty[acc]), 0u) : 0u;
+        uint32_t parity = 0, slab_i = 0, bias_n = ~0u;
         bool ok = true;  // after a wait that ran out the warp only keeps the named barriers' count
-        for (uint32_t it = blockIdx.x; it < items; it += gridDim.x) {
+        // A slab that no store of this warp still reads.
+        const auto next_slab = [&]() -> unsigned char* {
+            if (lane == 0u) tma::store_wait_read<S::kSlabs - 1u>();
+            __syncwarp();
+            unsigned char* p = my_slabs + slab_i * kSlabBytes;
+            if (S::kSlabs > 1u) slab_i ^= 1u;
+            return p;
+        };
+        for (uint32_t it = first_item + acc * item_step; it < items; it += 2u * item_step) {
             const uint32_t split = it / tiles, tile = it - split * tiles;
             uint32_t tm, tn;
             tile_of(g, tile, tm, tn);
-            const uint32_t m0 = tm * kBM + 32u * q, n0 = tn * BN;
+            const uint32_t m0 = (tm * kCtas + rank) * kBM + 32u * q, n0 = tn * BN;
             const uint32_t rows = m0 < g.M ? min(32u, g.M - m0) : 0u;
-            if (KIND == kGemmRows) {  // bias of the tile's columns, once per tile, shared by the four warps
-                asm volatile("bar.sync 1, 128;\n" ::: "memory");
+            if (KIND == kGemmRows && n0 != bias_n) {  // the tile's bias, kept while the columns stay the same
+                asm volatile("bar.sync %0, 128;\n" ::"r"(1u + acc) : "memory");
                 for (uint32_t c = threadIdx.x & 127u; c < BN; c += 128u)
-                    bias_s[c] = g.bias && n0 + c < g.N ? from_16(static_cast<const uint16_t*>(g.bias)[n0 + c], bf16) : 0.0f;
-                asm volatile("bar.sync 1, 128;\n" ::: "memory");
+                    bias_s[c] = g.bias && n0 + c < g.N ? static_cast<const uint16_t*>(g.bias)[n0 + c] : static_cast<uint16_t>(0);
+                asm volatile("bar.sync %0, 128;\n" ::"r"(1u + acc) : "memory");
+                bias_n = n0;
             }
             if (ok && !tma::wait(&bar.acc_full[acc], parity)) {
                 atomicOr(g.error, 1u);
@@ -369,67 +489,51 @@ __global__ void __launch_bounds__(PLAIN ? 384 : 256, 1)
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) continue;
             umma::fence_after_sync();
-            const uint32_t taddr = tmem + acc * BN + ((32u * q) << 16);
             if (KIND == kGemmRows) {
                 for (uint32_t c0 = 0; c0 < BN && n0 + c0 < g.N; c0 += 64u) {
                     const uint32_t cols = min(64u, g.N - n0 - c0);
-                    float v[64];
-                    umma::tmem_ld32(taddr + c0, v);
-                    umma::tmem_ld32(taddr + c0 + 32u, v + 32);
-#pragma unroll
-                    for (uint32_t i = 0; i < 16u; ++i) {
-                        const float4 b = *reinterpret_cast<const float4*>(bias_s + c0 + 4u * i);
-                        v[4 * i] += b.x;
-                        v[4 * i + 1] += b.y;
-                        v[4 * i + 2] += b.z;
-                        v[4 * i + 3] += b.w;
-                    }
                     if (g.pre.ptr) {
+                        unsigned char* slab = next_slab();
 #pragma unroll
-                        for (uint32_t p = 0; p < 8u; ++p) {
-                            uint32_t w[4];
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) w[i] = pack_16(v[8 * p + 2 * i], v[8 * p + 2 * i + 1], bf16);
-                            slab_put(slab, lane, p, w);
+                        for (uint32_t h = 0; h < 2u; ++h) {
+                            float v[32];
+                            load_z(v, taddr + c0 + 32u * h, bias_s + c0 + 32u * h, bf16);
+                            slab_put32(slab, lane, h, v, bf16);
                         }
-                        __syncwarp();
-                        unsigned char* dst = static_cast<unsigned char*>(const_cast<void*>(g.pre.ptr)) + 2u * (m0 * g.pre.ld + n0 + c0);
-                        slab_copy<2, true>(slab, dst, g.pre.ld, rows, cols, g.pre.vec >= 8u, lane);
-                        __syncwarp();
+                        slab_out(slab, g.pre, g.pre_tma != 0u, &maps.pre, m0, n0 + c0, rows, cols, lane);
                     }
-                    act_row(v, g.act);
+                    unsigned char* slab = next_slab();
                     if (g.res.ptr) {
                         unsigned char* src = static_cast<unsigned char*>(const_cast<void*>(g.res.ptr)) + 2u * (m0 * g.res.ld + n0 + c0);
                         slab_copy<2, false>(slab, src, g.res.ld, rows, cols, g.res.vec >= 8u, lane);
                         __syncwarp();
+                    }
 #pragma unroll
-                        for (uint32_t p = 0; p < 8u; ++p) {
-                            const uint4 u = *reinterpret_cast<const uint4*>(slab + slab_at(lane, p));
-                            const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+                    for (uint32_t h = 0; h < 2u; ++h) {
+                        float v[32];
+                        load_z(v, taddr + c0 + 32u * h, bias_s + c0 + 32u * h, bf16);
+                        act_row(v, g.act);
+                        if (g.res.ptr) {
 #pragma unroll
-                            for (int i = 0; i < 4; ++i) {
-                                const float2 f = unpack_16(w[i], bf16);
-                                v[8 * p + 2 * i] += f.x;
-                                v[8 * p + 2 * i + 1] += f.y;
+                            for (uint32_t p = 0; p < 4u; ++p) {
+                                const uint4 u = *reinterpret_cast<const uint4*>(slab + slab_at(lane, 4u * h + p));
+                                const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) {
+                                    const float2 f = unpack_16(w[i], bf16);
+                                    v[8 * p + 2 * i] += f.x;
+                                    v[8 * p + 2 * i + 1] += f.y;
+                                }
                             }
                         }
-                        __syncwarp();
+                        slab_put32(slab, lane, h, v, bf16);
                     }
-#pragma unroll
-                    for (uint32_t p = 0; p < 8u; ++p) {
-                        uint32_t w[4];
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) w[i] = pack_16(v[8 * p + 2 * i], v[8 * p + 2 * i + 1], bf16);
-                        slab_put(slab, lane, p, w);
-                    }
-                    __syncwarp();
-                    unsigned char* dst = static_cast<unsigned char*>(const_cast<void*>(g.y.ptr)) + 2u * (m0 * g.y.ld + n0 + c0);
-                    slab_copy<2, true>(slab, dst, g.y.ld, rows, cols, g.y.vec >= 8u, lane);
-                    __syncwarp();
+                    slab_out(slab, g.y, g.y_tma != 0u, &maps.y, m0, n0 + c0, rows, cols, lane);
                 }
             } else if (g.splits > 1u) {
                 // Partial tile, four columns of 128 rows at a time: 512 contiguous bytes a warp store.
-                float4* dst = reinterpret_cast<float4*>(g.partials) + static_cast<uint64_t>(it) * (BN / 4u) * kBM + row;
+                float4* dst = reinterpret_cast<float4*>(g.partials) +
+                              static_cast<uint64_t>(it * kCtas + rank) * (BN / 4u) * kBM + row;
                 for (uint32_t c0 = 0; c0 < BN && n0 + c0 < g.N; c0 += 32u) {
                     float v[32];
                     umma::tmem_ld32(taddr + c0, v);
@@ -439,6 +543,7 @@ __global__ void __launch_bounds__(PLAIN ? 384 : 256, 1)
                 }
             } else {
                 // The gradient itself: 32 fp32 or 64 16-bit columns (128 bytes) a slab.
+                unsigned char* slab = my_slabs;
                 const uint32_t es = g.dw_f32 ? 4u : 2u, wide = 128u / es;
                 for (uint32_t c0 = 0; c0 < BN && n0 + c0 < g.N; c0 += wide) {
                     const uint32_t cols = min(wide, g.N - n0 - c0);
@@ -460,20 +565,20 @@ __global__ void __launch_bounds__(PLAIN ? 384 : 256, 1)
                                 *l = make_float4(o.x + v[4 * p], o.y + v[4 * p + 1], o.z + v[4 * p + 2], o.w + v[4 * p + 3]);
                             }
                         } else {
+                            if (g.accumulate) {
 #pragma unroll
-                            for (uint32_t p = 0; p < 4u; ++p) {
-                                uint4* l = reinterpret_cast<uint4*>(slab + slab_at(lane, p + h / 8u));
-                                uint4 o = make_uint4(0u, 0u, 0u, 0u);
-                                if (g.accumulate) o = *l;
-                                const uint32_t ow[4] = {o.x, o.y, o.z, o.w};
-                                uint32_t w[4];
+                                for (uint32_t p = 0; p < 4u; ++p) {
+                                    const uint4 u = *reinterpret_cast<const uint4*>(slab + slab_at(lane, p + h / 8u));
+                                    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-                                for (int i = 0; i < 4; ++i) {
-                                    const float2 f = unpack_16(ow[i], bf16);
-                                    w[i] = pack_16(f.x + v[8 * p + 2 * i], f.y + v[8 * p + 2 * i + 1], bf16);
+                                    for (int i = 0; i < 4; ++i) {
+                                        const float2 f = unpack_16(w[i], bf16);
+                                        v[8 * p + 2 * i] += f.x;
+                                        v[8 * p + 2 * i + 1] += f.y;
+                                    }
                                 }
-                                *l = make_uint4(w[0], w[1], w[2], w[3]);
                             }
+                            slab_put32(slab, lane, h / 32u, v, bf16);
                         }
                     }
                     __syncwarp();
@@ -484,15 +589,22 @@ __global__ void __launch_bounds__(PLAIN ? 384 : 256, 1)
             }
             umma::fence_before_sync();
             __syncwarp();
-            if (lane == 0u) tma::arrive(&bar.acc_empty[acc]);
-            acc ^= 1u;
-            if (acc == 0u) parity ^= 1u;
+            if (lane == 0u) {
+                if (S::kPair) tma::arrive_at(acc_empty);
+                else tma::arrive(&bar.acc_empty[acc]);
+            }
+            parity ^= 1u;
         }
+        if (lane == 0u) tma::store_wait_all();
     }
     __syncwarp();
     umma::fence_before_sync();
     __syncthreads();
-    if (warp == 2u) umma::tmem_dealloc(tmem, tmem_cols(2u * BN));
+    if (S::kPair) tma::cluster_sync();  // neither CTA's shared or tensor memory goes while the other's MMAs use it
+    if (warp == 2u) {
+        if (S::kPair) tma::tmem_dealloc_pair(tmem, kCols);
+        else umma::tmem_dealloc(tmem, kCols);
+    }
 }
 
 // ------------------------------------------------- dz and its column sums
@@ -574,16 +686,17 @@ NB_DEV void grad_out(void* p, uint64_t i, float v, const GradReduceArgs& a) {
 // order; the others: 32 columns of db, eight warps each a range of the parts.
 __global__ void __launch_bounds__(256) k_grad_reduce(const GradReduceArgs a, uint32_t n_dw) {
     if (blockIdx.x < n_dw) {
+        // half: 128 rows of a tile (a pair of CTAs leaves two)
         const uint32_t per_tile = a.bn / 4u, idx = 2u * blockIdx.x + (threadIdx.x >> 7);
-        const uint32_t tile = idx / per_tile, c4 = idx - tile * per_tile, row = threadIdx.x & 127u;
-        const uint32_t tiles = a.tiles_m * a.tiles_n;
+        const uint32_t half = idx / per_tile, c4 = idx - half * per_tile, row = threadIdx.x & 127u;
+        const uint32_t tiles = a.tiles_m * a.tiles_n, tile = half / a.ctas;
         if (tile >= tiles) return;
         const uint32_t per = 16u * a.tiles_n, group = tile / per, first = 16u * group;
         const uint32_t gm = min(16u, a.tiles_m - first), r = tile - group * per;
-        const uint32_t m = (first + r % gm) * kBM + row, n = (r / gm) * a.bn + 4u * c4;
+        const uint32_t m = ((first + r % gm) * a.ctas + half % a.ctas) * kBM + row, n = (r / gm) * a.bn + 4u * c4;
         if (m >= a.n_out || n >= a.n_in) return;
-        const float4* src = reinterpret_cast<const float4*>(a.partials) + (static_cast<uint64_t>(tile) * per_tile + c4) * kBM + row;
-        const uint64_t step = static_cast<uint64_t>(tiles) * per_tile * kBM;
+        const float4* src = reinterpret_cast<const float4*>(a.partials) + (static_cast<uint64_t>(half) * per_tile + c4) * kBM + row;
+        const uint64_t step = static_cast<uint64_t>(tiles) * a.ctas * per_tile * kBM;
         float4 t = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 8
         for (uint32_t k = 0; k < a.splits; ++k) {
@@ -617,8 +730,9 @@ __global__ void __launch_bounds__(256) k_grad_reduce(const GradReduceArgs a, uin
     }
 }
 
-template <uint32_t BN, int KIND, bool PLAIN>
-cudaError_t launch_gemm_t(const GemmArgs& g, const CUtensorMap& ma, const CUtensorMap& mb, uint32_t blocks, cudaStream_t s) {
+template <uint32_t BN, int KIND, int FEED>
+cudaError_t launch_gemm_t(const GemmArgs& g, const GemmMaps& maps, uint32_t blocks, cudaStream_t s) {
+    using S = GemmShape<BN, KIND, FEED>;
     // The attribute belongs to the device: set once for each.
     static std::atomic<bool> done[64];
     int dev = 0;
@@ -626,32 +740,48 @@ cudaError_t launch_gemm_t(const GemmArgs& g, const CUtensorMap& ma, const CUtens
     if (e != cudaSuccess) return e;
     if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
     if (!done[dev]) {
-        e = cudaFuncSetAttribute(k_gemm<BN, KIND, PLAIN>, cudaFuncAttributeMaxDynamicSharedMemorySize, gemm_smem(BN));
+        e = cudaFuncSetAttribute(k_gemm<BN, KIND, FEED>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
         if (e != cudaSuccess) return e;
         done[dev] = true;
     }
-    k_gemm<BN, KIND, PLAIN><<<blocks, PLAIN ? 384u : 256u, gemm_smem(BN), s>>>(g, ma, mb);
-    return cudaGetLastError();
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(blocks);
+    cfg.blockDim = dim3(S::kThreads);
+    cfg.dynamicSmemBytes = S::kSmem;
+    cfg.stream = s;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = S::kPair ? 2u : 1u;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1u;
+    cfg.attrs = at;
+    cfg.numAttrs = S::kPair ? 1u : 0u;
+    return cudaLaunchKernelEx(&cfg, k_gemm<BN, KIND, FEED>, g, maps);
 }
-template <int KIND, bool PLAIN>
-cudaError_t launch_gemm_bn(const GemmArgs& g, uint32_t bn, const CUtensorMap& ma, const CUtensorMap& mb, uint32_t blocks, cudaStream_t s) {
+template <int KIND, int FEED>
+cudaError_t launch_gemm_bn(const GemmArgs& g, uint32_t bn, const GemmMaps& maps, uint32_t blocks, cudaStream_t s) {
     switch (bn) {
-        case 64u: return launch_gemm_t<64u, KIND, PLAIN>(g, ma, mb, blocks, s);
-        case 128u: return launch_gemm_t<128u, KIND, PLAIN>(g, ma, mb, blocks, s);
-        case 256u: return launch_gemm_t<256u, KIND, PLAIN>(g, ma, mb, blocks, s);
+        case 64u: return launch_gemm_t<64u, KIND, FEED>(g, maps, blocks, s);
+        case 128u: return launch_gemm_t<128u, KIND, FEED>(g, maps, blocks, s);
+        case 256u: return launch_gemm_t<256u, KIND, FEED>(g, maps, blocks, s);
         default: return cudaErrorInvalidValue;
+    }
+}
+template <int KIND>
+cudaError_t launch_gemm_kind(const GemmArgs& g, uint32_t bn, int feed, const GemmMaps& maps, uint32_t blocks, cudaStream_t s) {
+    switch (feed) {
+        case kFeedTma: return launch_gemm_bn<KIND, kFeedTma>(g, bn, maps, blocks, s);
+        case kFeedPlain: return launch_gemm_bn<KIND, kFeedPlain>(g, bn, maps, blocks, s);
+        default:
+            if (bn != kGemmPairBN || (blocks & 1u)) return cudaErrorInvalidValue;
+            return launch_gemm_t<kGemmPairBN, KIND, kFeedPair>(g, maps, blocks, s);
     }
 }
 
 }  // namespace
 
-cudaError_t launch_gemm(const GemmArgs& g, int kind, uint32_t bn, const CUtensorMap* map_a, const CUtensorMap* map_b,
-                        bool plain_loads, uint32_t blocks, cudaStream_t s) {
-    if (kind == kGemmRows)
-        return plain_loads ? launch_gemm_bn<kGemmRows, true>(g, bn, *map_a, *map_b, blocks, s)
-                           : launch_gemm_bn<kGemmRows, false>(g, bn, *map_a, *map_b, blocks, s);
-    return plain_loads ? launch_gemm_bn<kGemmGrad, true>(g, bn, *map_a, *map_b, blocks, s)
-                       : launch_gemm_bn<kGemmGrad, false>(g, bn, *map_a, *map_b, blocks, s);
+cudaError_t launch_gemm(const GemmArgs& g, int kind, uint32_t bn, int feed, const GemmMaps& maps, uint32_t blocks, cudaStream_t s) {
+    return kind == kGemmRows ? launch_gemm_kind<kGemmRows>(g, bn, feed, maps, blocks, s)
+                             : launch_gemm_kind<kGemmGrad>(g, bn, feed, maps, blocks, s);
 }
 
 cudaError_t launch_dz(const DzArgs& a, cudaStream_t s) {
@@ -664,7 +794,7 @@ cudaError_t launch_dz(const DzArgs& a, cudaStream_t s) {
 }
 
 cudaError_t launch_grad_reduce(const GradReduceArgs& a, cudaStream_t s) {
-    const uint32_t n_dw = a.dw ? (a.tiles_m * a.tiles_n * (a.bn / 4u) + 1u) / 2u : 0u;
+    const uint32_t n_dw = a.dw ? (a.tiles_m * a.tiles_n * a.ctas * (a.bn / 4u) + 1u) / 2u : 0u;
     const uint32_t n_db = a.db ? (a.n_out + 31u) / 32u : 0u;
     if (n_dw + n_db == 0u) return cudaSuccess;
     k_grad_reduce<<<n_dw + n_db, 256, 0, s>>>(a, n_dw);

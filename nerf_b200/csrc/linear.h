@@ -35,6 +35,7 @@ struct GemmArgs {
     // epilogue of an activation output: y = act(D + bias) + res, pre = D + bias
     const void* bias;
     MatrixView res, y, pre;  // ptr null: none
+    uint32_t y_tma, pre_tma; // stored by the tensor copy unit (rows on 16-byte boundaries)
     // epilogue of a weight gradient: partials when splits > 1, else dw (+)= D
     float* partials;
     void* dw;
@@ -44,8 +45,15 @@ struct GemmArgs {
 
 enum GemmKind : int { kGemmRows = 0, kGemmGrad = 1 };
 
-cudaError_t launch_gemm(const GemmArgs& g, int kind, uint32_t bn, const CUtensorMap* map_a, const CUtensorMap* map_b,
-                        bool plain_loads, uint32_t blocks, cudaStream_t s);
+struct GemmMaps {
+    CUtensorMap a, b, y, pre;
+};
+// How a product's operands reach shared memory: copied for one CTA a tile,
+// copied for a pair of CTAs on one 256 x 256 tile, or loaded by warps.
+enum GemmFeed : int { kFeedTma = 0, kFeedPair = 1, kFeedPlain = 2 };
+constexpr uint32_t kGemmPairBN = 256;
+
+cudaError_t launch_gemm(const GemmArgs& g, int kind, uint32_t bn, int feed, const GemmMaps& maps, uint32_t blocks, cudaStream_t s);
 // dz = dy act'(pre) (16-bit, rows dz_ld apart; null: not written), and the
 // column sums of dz before rounding over each of `parts` row ranges
 // ([parts][cols] fp32; null: none).
@@ -61,7 +69,7 @@ cudaError_t launch_dz(const DzArgs& a, cudaStream_t s);
 // dw (+)= sum of the splits' partial tiles, db (+)= sum of the row parts.
 struct GradReduceArgs {
     const float* partials;
-    uint32_t splits, tiles_m, tiles_n, bn, n_out, n_in;
+    uint32_t splits, tiles_m, tiles_n, bn, ctas, n_out, n_in;  // ctas: 128-row halves of a tile
     const float* db_part;
     uint32_t parts;
     void *dw, *db;  // null: none

@@ -106,11 +106,18 @@ uint32_t pick_bn(uint32_t tiles_m, uint32_t n, uint32_t sms) {
     return best;
 }
 
+// Whether a product is worth a pair of CTAs on 256 x 256 tiles: enough tiles
+// for every pair, and a K long enough for the MMAs to be what takes the time.
+bool pair_pays(uint64_t m, uint64_t n, uint64_t k, uint32_t sms) {
+    return k >= 512u && static_cast<uint64_t>(ceil_div(m, 256u)) * ceil_div(n, 256u) >= sms / 2u;
+}
+
 struct BackwardPlan {
     uint32_t sms;
     bool dz_needed;                     // dz is not dy itself
     uint64_t dz_ld;
     uint32_t parts, rows_per_part;      // row ranges of the column sums
+    bool pair;                          // weight gradient: the tiles are those of a pair of CTAs, where it can be fed
     uint32_t bn, tiles_m, tiles_n, splits, k_steps, steps_per_split;  // weight gradient
     uint64_t o_dz, o_db, o_dw, bytes;   // workspace
 };
@@ -128,12 +135,14 @@ BackwardPlan plan_backward(const NerfB200Linear& d) {
     if (p.rows_per_part == 0u) p.rows_per_part = 1u;
     p.parts = ceil_div(d.n_rows, p.rows_per_part);
     p.bn = d.n_in <= 64u ? 64u : d.n_in <= 128u ? 128u : 256u;
-    p.tiles_m = ceil_div(d.n_out, kGemmBM);
+    p.pair = pair_pays(d.n_out, d.n_in, d.n_rows, p.sms);
+    p.tiles_m = ceil_div(d.n_out, p.pair ? 2u * kGemmBM : kGemmBM);
     p.tiles_n = ceil_div(d.n_in, p.bn);
     p.k_steps = ceil_div(d.n_rows, kGemmBK);
     // One wave of (tile, row range) items, each range at least four steps.
     const uint64_t tiles = static_cast<uint64_t>(p.tiles_m) * p.tiles_n;
-    uint64_t splits = tiles >= p.sms ? 1u : p.sms / tiles;
+    const uint32_t slots = p.pair ? p.sms / 2u : p.sms;
+    uint64_t splits = tiles >= slots ? 1u : slots / tiles;
     if (splits > ceil_div(p.k_steps, 4u)) splits = ceil_div(p.k_steps, 4u);
     if (splits < 1u) splits = 1u;
     p.steps_per_split = ceil_div(p.k_steps, splits);
@@ -144,7 +153,7 @@ BackwardPlan plan_backward(const NerfB200Linear& d) {
     p.o_db = at;
     at += up(static_cast<uint64_t>(p.parts) * d.n_out * 4u, 256u);
     p.o_dw = at;
-    if (p.splits > 1u) at += static_cast<uint64_t>(p.splits) * tiles * kGemmBM * p.bn * 4u;
+    if (p.splits > 1u) at += static_cast<uint64_t>(p.splits) * tiles * (p.pair ? 2u : 1u) * kGemmBM * p.bn * 4u;
     p.bytes = at ? at : 256u;
     return p;
 }
@@ -164,17 +173,35 @@ bool valid_shape(const NerfB200Linear& d) {
     return d.ld_residual <= kMaxLd;  // as wide as the output it joins: checked by the calls
 }
 
-// The product with its operands' maps; plain loads where a row does not start
-// on a 16-byte boundary.
-cudaError_t run_gemm(GemmArgs& g, int kind, uint32_t bn, uint32_t sms, cudaStream_t s) {
-    CUtensorMap ma{}, mb{};
-    const bool plain = g.a.vec < 8u || g.b.vec < 8u;
+// The product with its operands' and outputs' maps; loads by warps where an
+// operand's rows do not start on 16-byte boundaries.  pair: the tiles are
+// those of a pair of CTAs.
+cudaError_t run_gemm(GemmArgs& g, int kind, uint32_t bn, bool pair, uint32_t sms, cudaStream_t s) {
+    GemmMaps maps{};
+    const bool plain = g.a.vec < 8u || g.b.vec < 8u, bf16 = g.bf16 != 0u;
+    if (plain && pair) return cudaErrorInvalidValue;
     g.a_box_rows = g.M >= kGemmBM ? kGemmBM : static_cast<uint32_t>(up(g.M, 8u));
-    if (!plain && (!make_map(&ma, g.a, g.a_mn ? kGemmBK : g.a_box_rows, g.bf16 != 0u) ||
-                   !make_map(&mb, g.b, g.b_mn ? kGemmBK : bn, g.bf16 != 0u)))
+    if (!plain && (!make_map(&maps.a, g.a, g.a_mn ? kGemmBK : g.a_box_rows, bf16) ||
+                   !make_map(&maps.b, g.b, g.b_mn ? kGemmBK : pair ? bn / 2u : bn, bf16)))
         return cudaErrorNotSupported;
-    const uint64_t items = static_cast<uint64_t>(g.tiles_m) * g.tiles_n * g.splits;
-    return launch_gemm(g, kind, bn, &ma, &mb, plain, items < sms ? static_cast<uint32_t>(items) : sms, s);
+    // The copy unit writes whole 16-byte pieces: a row must end with one.
+    g.y_tma = g.y.ptr && g.y.vec >= 8u && g.y.cols % 8u == 0u;
+    g.pre_tma = g.pre.ptr && g.pre.vec >= 8u && g.pre.cols % 8u == 0u;
+    if ((g.y_tma && !make_map(&maps.y, g.y, 32u, bf16)) || (g.pre_tma && !make_map(&maps.pre, g.pre, 32u, bf16)))
+        return cudaErrorNotSupported;
+    const uint64_t items = static_cast<uint64_t>(g.tiles_m) * g.tiles_n * g.splits, slots = pair ? sms / 2u : sms;
+    const uint32_t blocks = static_cast<uint32_t>(items < slots ? items : slots) * (pair ? 2u : 1u);
+    return launch_gemm(g, kind, bn, plain ? kFeedPlain : pair ? kFeedPair : kFeedTma, maps, blocks, s);
+}
+// y = act(a b^T + bias) + res: fills in the tiles and runs the product.
+cudaError_t run_rows(GemmArgs& g, uint32_t sms, cudaStream_t s) {
+    const bool pair = g.a.vec >= 8u && g.b.vec >= 8u && pair_pays(g.M, g.N, g.K, sms);
+    g.tiles_m = ceil_div(g.M, pair ? 2u * kGemmBM : kGemmBM);
+    const uint32_t bn = pair ? kGemmPairBN : pick_bn(g.tiles_m, g.N, sms);
+    g.tiles_n = ceil_div(g.N, bn);
+    g.splits = 1u;
+    g.k_steps = g.steps_per_split = ceil_div(g.K, kGemmBK);
+    return run_gemm(g, kGemmRows, bn, pair, sms, s);
 }
 
 }  // namespace
@@ -207,11 +234,6 @@ NERF_API NerfStatus nerf_b200_linear_forward(const NerfB200Linear* desc, const v
     g.K = d.n_in;
     g.a = view(x, ld_or(d.ld_x, d.n_in), d.n_rows, d.n_in);
     g.b = view(weight, ld_or(d.ld_weight, d.n_in), d.n_out, d.n_in);
-    g.tiles_m = ceil_div(g.M, kGemmBM);
-    const uint32_t bn = pick_bn(g.tiles_m, g.N, sms);
-    g.tiles_n = ceil_div(g.N, bn);
-    g.splits = 1u;
-    g.k_steps = g.steps_per_split = ceil_div(g.K, kGemmBK);
     g.bf16 = d.dtype == NERF_B200_BF16;
     g.act = d.activation;
     g.bias = bias;
@@ -219,7 +241,7 @@ NERF_API NerfStatus nerf_b200_linear_forward(const NerfB200Linear* desc, const v
     g.y = view(y, ld_or(d.ld_y, d.n_out), d.n_rows, d.n_out);
     g.pre = view(pre, ld_or(d.ld_pre, d.n_out), d.n_rows, d.n_out);
     g.error = error_word;
-    return run_gemm(g, kGemmRows, bn, sms, static_cast<cudaStream_t>(stream)) == cudaSuccess ? NERF_STATUS_OK : NERF_STATUS_CUDA_ERROR;
+    return run_rows(g, sms, static_cast<cudaStream_t>(stream)) == cudaSuccess ? NERF_STATUS_OK : NERF_STATUS_CUDA_ERROR;
 }
 
 NERF_API uint64_t nerf_b200_linear_backward_workspace_bytes(const NerfB200Linear* desc) {
@@ -286,16 +308,11 @@ NERF_API NerfStatus nerf_b200_linear_backward(const NerfB200Linear* desc, const 
         g.a = dzv;
         g.b = view(weight, ld_or(d.ld_weight, d.n_in), d.n_out, d.n_in);
         g.b_mn = 1u;
-        g.tiles_m = ceil_div(g.M, kGemmBM);
-        const uint32_t bn = pick_bn(g.tiles_m, g.N, p.sms);
-        g.tiles_n = ceil_div(g.N, bn);
-        g.splits = 1u;
-        g.k_steps = g.steps_per_split = ceil_div(g.K, kGemmBK);
         g.bf16 = bf16;
         g.res = view(dx_residual, ld_or(d.ld_residual, d.n_in), d.n_rows, d.n_in);
         g.y = view(dx, ld_or(d.ld_dx, d.n_in), d.n_rows, d.n_in);
         g.error = error_word;
-        if (run_gemm(g, kGemmRows, bn, p.sms, s) != cudaSuccess) return NERF_STATUS_CUDA_ERROR;
+        if (run_rows(g, p.sms, s) != cudaSuccess) return NERF_STATUS_CUDA_ERROR;
     }
     GradReduceArgs r{};
     r.n_out = d.n_out;
@@ -311,7 +328,9 @@ NERF_API NerfStatus nerf_b200_linear_backward(const NerfB200Linear* desc, const 
         g.a = dzv;
         g.b = view(x, ld_or(d.ld_x, d.n_in), d.n_rows, d.n_in);
         g.a_mn = g.b_mn = 1u;
-        g.tiles_m = p.tiles_m;
+        // A pair's plan on rows that only warps can load: the same tiles' 128-row halves.
+        const bool pair = p.pair && g.a.vec >= 8u && g.b.vec >= 8u;
+        g.tiles_m = p.pair && !pair ? ceil_div(d.n_out, kGemmBM) : p.tiles_m;
         g.tiles_n = p.tiles_n;
         g.splits = p.splits;
         g.k_steps = p.k_steps;
@@ -323,11 +342,12 @@ NERF_API NerfStatus nerf_b200_linear_backward(const NerfB200Linear* desc, const 
         g.dw_vec = aligned(dweight, 16u) && (es * d.n_in) % 16u == 0u;
         g.accumulate = d.accumulate;
         g.error = error_word;
-        if (run_gemm(g, kGemmGrad, p.bn, p.sms, s) != cudaSuccess) return NERF_STATUS_CUDA_ERROR;
+        if (run_gemm(g, kGemmGrad, p.bn, pair, p.sms, s) != cudaSuccess) return NERF_STATUS_CUDA_ERROR;
         if (p.splits > 1u) {
             r.partials = g.partials;
             r.splits = p.splits;
-            r.tiles_m = p.tiles_m;
+            r.ctas = pair ? 2u : 1u;
+            r.tiles_m = g.tiles_m;
             r.tiles_n = p.tiles_n;
             r.bn = p.bn;
             r.dw = dweight;

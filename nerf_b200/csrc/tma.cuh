@@ -38,6 +38,27 @@ NB_DEV void load_2d(uint32_t dst, const CUtensorMap* map, int32_t x, int32_t y, 
         "l"(map), "r"(x), "r"(y), "r"(smem_u32(mbar))
         : "memory");
 }
+// The same with the completion signalled at a barrier of the cluster's leading
+// CTA (mbar: its shared::cluster address), for a pair of CTAs on one MMA.
+NB_DEV void load_2d_pair(uint32_t dst, const CUtensorMap* map, int32_t x, int32_t y, uint32_t mbar) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];\n" ::"r"(
+            dst),
+        "l"(map), "r"(x), "r"(y), "r"(mbar)
+        : "memory");
+}
+// Shared memory -> global; out-of-range rows and columns of the box are not written.
+NB_DEV void store_2d(const CUtensorMap* map, uint32_t src, int32_t x, int32_t y) {
+    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];\n" ::"l"(map), "r"(x), "r"(y), "r"(src)
+                 : "memory");
+}
+NB_DEV void store_commit() { asm volatile("cp.async.bulk.commit_group;\n" ::: "memory"); }
+// At most N of this thread's store groups still read shared memory.
+template <int N>
+NB_DEV void store_wait_read() {
+    asm volatile("cp.async.bulk.wait_group.read %0;\n" ::"n"(N) : "memory");
+}
+NB_DEV void store_wait_all() { asm volatile("cp.async.bulk.wait_group 0;\n" ::: "memory"); }
 NB_DEV void prefetch_map(const CUtensorMap* map) { asm volatile("prefetch.tensormap [%0];\n" ::"l"(map) : "memory"); }
 
 NB_DEV void expect_tx(uint64_t* mbar, uint32_t bytes) {
@@ -73,7 +94,42 @@ NB_DEV bool wait(uint64_t* mbar, uint32_t parity) {
     }
 }
 
+// ---- a pair of CTAs on one MMA (cta_group::2) ----
+NB_DEV void tmem_alloc_pair(uint32_t* slot, uint32_t ncols) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_u32(slot)), "r"(ncols) : "memory");
+}
+NB_DEV void tmem_relinquish_pair() { asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;\n" ::: "memory"); }
+NB_DEV void tmem_dealloc_pair(uint32_t taddr, uint32_t ncols) {
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;\n" ::"r"(taddr), "r"(ncols) : "memory");
+}
+NB_DEV void mma_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n"
+        ".reg .pred p;\n"
+        "setp.ne.b32 p, %4, 0;\n"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n"
+        "}\n" ::"r"(d_tmem),
+        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+// Arrival at the same barrier of both CTAs when the MMAs issued so far are done.
+NB_DEV void commit_pair(uint64_t* mbar) {
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n" ::"r"(smem_u32(mbar)),
+        "h"(static_cast<uint16_t>(3u))
+        : "memory");
+}
+
 // ---- clusters ----
+// shared::cluster address of another CTA's variable (addr: this CTA's address of it).
+NB_DEV uint32_t peer_addr(uint32_t addr, uint32_t rank) {
+    uint32_t remote;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(remote) : "r"(addr), "r"(rank));
+    return remote;
+}
+NB_DEV void arrive_at(uint32_t mbar_cluster_addr) {
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];\n" ::"r"(mbar_cluster_addr) : "memory");
+}
 NB_DEV uint32_t cluster_rank() {
     uint32_t r;
     asm volatile("mov.u32 %0, %%cluster_ctarank;\n" : "=r"(r));
@@ -84,10 +140,8 @@ NB_DEV void cluster_sync() {
 }
 // A float of another CTA's shared memory (addr: this CTA's address of the same variable).
 NB_DEV float peer_f32(uint32_t addr, uint32_t rank) {
-    uint32_t remote;
     float v;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(remote) : "r"(addr), "r"(rank));
-    asm volatile("ld.shared::cluster.f32 %0, [%1];\n" : "=f"(v) : "r"(remote) : "memory");
+    asm volatile("ld.shared::cluster.f32 %0, [%1];\n" : "=f"(v) : "r"(peer_addr(addr, rank)) : "memory");
     return v;
 }
 

@@ -14,9 +14,10 @@ from linear_util import (ACTS, SENTINEL, act64, backward, dact64, dtype_of, forw
 
 pytestmark = pytest.mark.gpu
 
-# rows, in, out: one value, tile edges of 64 / 128 / 256, odd widths, several tiles each way, a long K
+# rows, in, out: one value, tile edges of 64 / 128 / 256, odd widths, several tiles each way, a long K; the last three
+# have enough 256 x 256 tiles for pairs of CTAs in the forward, the input gradient and the weight gradient
 SHAPES = [(1, 1, 1), (1, 64, 64), (2, 17, 9), (5, 64, 48), (63, 63, 65), (64, 128, 128), (127, 200, 256), (128, 64, 257), (129, 65, 64),
-          (300, 320, 511), (1000, 63, 255), (257, 1024, 96), (19, 2048, 520), (4097, 32, 64), (20000, 64, 64)]
+          (300, 320, 511), (1000, 63, 255), (257, 1024, 96), (19, 2048, 520), (4097, 32, 64), (20000, 64, 64), (2500, 520, 2056), (2500, 2049, 520), (700, 2328, 2312)]
 
 
 def _floor(torch, t):
