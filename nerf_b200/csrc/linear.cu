@@ -36,6 +36,10 @@ constexpr uint32_t kBM = kGemmBM, kBK = kGemmBK;
 constexpr uint32_t kStageBytesA = kBM * 128u;
 constexpr uint32_t kSlabBytes = 32u * 128u;  // one epilogue warp's 32 rows x 128 bytes
 constexpr uint32_t kMaxStages = 8;
+// 64-row steps that a weight gradient's MMAs sum in tensor memory before the
+// sum moves to registers.  The tensor core's additions cut off instead of
+// rounding: 32 of them in a row are off by 6e-7 of the result, 512 by 1e-5.
+constexpr uint32_t kChunkSteps = 8;
 
 __host__ __device__ constexpr uint32_t tmem_cols(uint32_t n) { return n <= 32u ? 32u : n <= 64u ? 64u : n <= 128u ? 128u : n <= 256u ? 256u : 512u; }
 
@@ -59,11 +63,29 @@ NB_DEV uint16_t to_16(float v, bool bf16) { return static_cast<uint16_t>(pack_16
 
 // ------------------------------------------------------------- activations
 NB_DEV float sigmoid_f(float z) { return __fdividef(1.0f, 1.0f + __expf(-z)); }
+// Phi(z) and exp(-z^2 / 2).  erfc(x) = (a1 t + ... + a5 t^5) exp(-x^2) with
+// t = 1 / (1 + p x) (Abramowitz and Stegun, Handbook of Mathematical
+// Functions, 7.1.26: off by at most 1.5e-7, a thousandth of a step of the
+// 16-bit result).
+NB_DEV float phi_f(float z, float& e) {
+    const float x = fabsf(z) * 0.70710678118654752f;
+    const float t = __fdividef(1.0f, fmaf(0.3275911f, x, 1.0f));
+    float p = fmaf(1.061405429f, t, -1.453152027f);
+    p = fmaf(p, t, 1.421413741f);
+    p = fmaf(p, t, -0.284496736f);
+    p = fmaf(p, t, 0.254829592f);
+    e = __expf(-0.5f * z * z);
+    const float tail = 0.5f * p * t * e;
+    return z > 0.0f ? 1.0f - tail : tail;
+}
 NB_DEV float act_f(float z, uint32_t act) {
     switch (act) {
         case kActRelu: return z > 0.0f ? z : 0.0f;
         case kActSilu: return z * sigmoid_f(z);
-        case kActGelu: return 0.5f * z * (1.0f + erff(z * 0.70710678118654752f));
+        case kActGelu: {
+            float e;
+            return z * phi_f(z, e);
+        }
         case kActSigmoid: return sigmoid_f(z);
         default: return z;
     }
@@ -92,8 +114,11 @@ NB_DEV float dact_f(float dy, float z, uint32_t act) {
             const float s = sigmoid_f(z);
             return dy * (s * (1.0f + z * (1.0f - s)));
         }
-        case kActGelu:
-            return dy * (0.5f * (1.0f + erff(z * 0.70710678118654752f)) + z * 0.39894228040143268f * __expf(-0.5f * z * z));
+        case kActGelu: {
+            float e;
+            const float p = phi_f(z, e);
+            return dy * fmaf(z * 0.39894228040143268f, e, p);
+        }
         case kActSigmoid: {
             const float s = sigmoid_f(z);
             return dy * (s * (1.0f - s));
@@ -137,18 +162,45 @@ NB_DEV void slab_copy(unsigned char* slab, unsigned char* g, uint64_t ld, uint32
         }
         return;
     }
-    for (uint32_t r = 0; r < rows; ++r) {
-        for (uint32_t c = lane; c < cols; c += 32u) {
-            unsigned char* q = g + (r * ld + c) * ES;
-            unsigned char* l = slab + slab_at(r, c / kPer) + (c % kPer) * ES;
-            if (ES == 2) {
-                if (kStore) *reinterpret_cast<uint16_t*>(q) = *reinterpret_cast<const uint16_t*>(l);
-                else *reinterpret_cast<uint16_t*>(l) = *reinterpret_cast<const uint16_t*>(q);
+    // A row is 32 words of the slab: lane i moves word i, as one or two values.
+    const bool words = ES == 4 || ((reinterpret_cast<uintptr_t>(g) & 3u) == 0u && (ld & 1u) == 0u);
+    const bool lo = ES == 4 ? lane < cols : 2u * lane < cols, hi = ES == 4 ? lane < cols : 2u * lane + 1u < cols;
+    unsigned char* q = g + 4u * lane;
+    constexpr uint32_t kBatch = 8;
+    for (uint32_t r0 = 0; r0 < rows; r0 += kBatch) {
+        uint32_t w[kBatch];
+#pragma unroll
+        for (uint32_t j = 0; j < kBatch; ++j) {
+            unsigned char* l = slab + slab_at(r0 + j, lane >> 2) + 4u * (lane & 3u);
+            if (kStore) {
+                w[j] = *reinterpret_cast<const uint32_t*>(l);
             } else {
-                if (kStore) *reinterpret_cast<uint32_t*>(q) = *reinterpret_cast<const uint32_t*>(l);
-                else *reinterpret_cast<uint32_t*>(l) = *reinterpret_cast<const uint32_t*>(q);
+                const unsigned char* p = q + j * ld * ES;
+                const bool live = r0 + j < rows;
+                if (words) {
+                    w[j] = live && hi ? *reinterpret_cast<const uint32_t*>(p) : live && lo ? *reinterpret_cast<const uint16_t*>(p) : 0u;
+                } else {
+                    w[j] = live && lo ? *reinterpret_cast<const uint16_t*>(p) : 0u;
+                    if (live && hi) w[j] |= static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(p)[1]) << 16;
+                }
             }
         }
+#pragma unroll
+        for (uint32_t j = 0; j < kBatch; ++j) {
+            if (kStore) {
+                unsigned char* p = q + j * ld * ES;
+                if (r0 + j >= rows) break;
+                if (words && hi) {
+                    *reinterpret_cast<uint32_t*>(p) = w[j];
+                } else {
+                    if (lo) *reinterpret_cast<uint16_t*>(p) = static_cast<uint16_t>(w[j]);
+                    if (hi) reinterpret_cast<uint16_t*>(p)[1] = static_cast<uint16_t>(w[j] >> 16);
+                }
+            } else {
+                *reinterpret_cast<uint32_t*>(slab + slab_at(r0 + j, lane >> 2) + 4u * (lane & 3u)) = w[j];
+            }
+        }
+        q += kBatch * ld * ES;
     }
 }
 NB_DEV void slab_put(unsigned char* slab, uint32_t row, uint32_t piece, const uint32_t w[4]) {
@@ -175,40 +227,41 @@ NB_DEV void fill_box(unsigned char* box, const MatrixView& m, uint32_t row0, uin
         }
         return;
     }
-    // A warp a row, lane i the values 2 i and 2 i + 1.  A row that starts
-    // between two 32-bit words is read as the words around it: lane i reads
-    // values 2 i - 1 and 2 i and takes 2 i + 1 from its neighbour's word.  No
-    // word reaches outside the row's values: the ends are 16-bit loads.
+    // A warp a row, lane i the values 2 i and 2 i + 1: one 32-bit load where
+    // every row starts on a word, else two of 16 bits.  kBatch rows' loads are
+    // in flight before the first is stored.
     const uint32_t lane = tid & 31u, warp = tid >> 5;
-    constexpr uint32_t kBatch = 8;  // rows in flight a warp
+    constexpr uint32_t kBatch = 16;
+    const bool lo = 2u * lane < have, hi = 2u * lane + 1u < have, words = m.vec >= 2u;
     for (uint32_t r0 = warp; r0 < rows; r0 += kLoadWarps * kBatch) {
-        uint32_t w[kBatch], odd[kBatch];
-        uint16_t last[kBatch];
+        const uint32_t in = row0 + r0 < m.rows ? m.rows - row0 - r0 : 0u;  // matrix rows from r0 on
+        const uint16_t* q = base + (static_cast<uint64_t>(row0) + r0) * m.ld + col0 + 2u * lane;
+        const uint64_t step = kLoadWarps * m.ld;
+        uint32_t w[kBatch];
+        if (words) {
 #pragma unroll
-        for (uint32_t j = 0; j < kBatch; ++j) {
-            const uint32_t r = r0 + j * kLoadWarps;
-            const uint64_t gr = static_cast<uint64_t>(row0) + r;
-            const uint16_t* q = base + gr * m.ld + col0;
-            const bool live = r < rows && gr < m.rows;
-            odd[j] = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(q) >> 1) & 1u;
-            const uint32_t nv = live ? have : 0u;
-            w[j] = 0u;
-            last[j] = 0u;
-            if (odd[j]) {
-                if (lane > 0u && 2u * lane < nv) w[j] = *reinterpret_cast<const uint32_t*>(q + 2u * lane - 1u);
-                else if (lane == 0u && nv > 0u) w[j] = static_cast<uint32_t>(q[0]) << 16;
-                else if (lane > 0u && 2u * lane - 1u < nv) w[j] = q[2u * lane - 1u];
-                if (lane == 31u && nv == 64u) last[j] = q[63];
-            } else {
-                if (2u * lane + 1u < nv) w[j] = *reinterpret_cast<const uint32_t*>(q + 2u * lane);
-                else if (2u * lane < nv) w[j] = q[2u * lane];
+            for (uint32_t j = 0; j < kBatch; ++j) {
+                const uint32_t r = j * kLoadWarps;
+                const bool live = r0 + r < rows && r < in;
+                w[j] = live && hi ? *reinterpret_cast<const uint32_t*>(q) : live && lo ? *q : 0u;
+                q += step;
             }
+        } else {
+            uint16_t v[kBatch];
+#pragma unroll
+            for (uint32_t j = 0; j < kBatch; ++j) {
+                const uint32_t r = j * kLoadWarps;
+                const bool live = r0 + r < rows && r < in;
+                w[j] = live && lo ? q[0] : 0u;
+                v[j] = live && hi ? q[1] : static_cast<uint16_t>(0);
+                q += step;
+            }
+#pragma unroll
+            for (uint32_t j = 0; j < kBatch; ++j) w[j] |= static_cast<uint32_t>(v[j]) << 16;
         }
 #pragma unroll
         for (uint32_t j = 0; j < kBatch; ++j) {
             const uint32_t r = r0 + j * kLoadWarps;
-            const uint32_t next = __shfl_down_sync(0xffffffffu, w[j], 1);
-            if (odd[j]) w[j] = (w[j] >> 16) | ((lane == 31u ? static_cast<uint32_t>(last[j]) : next) << 16);
             if (r < rows) *reinterpret_cast<uint32_t*>(box + slab_at(r, lane >> 2) + 4u * (lane & 3u)) = w[j];
         }
     }
@@ -284,6 +337,11 @@ struct GemmShape {
     static constexpr uint32_t kSlabs = kPair ? 2u : BN >= 256u ? 1u : 2u;  // per epilogue warp
     static constexpr uint32_t kSmem = 1024u + kStages * kStageBytes + 8u * kSlabs * kSlabBytes + 2u * BN * 2u;
     static constexpr uint32_t kThreads = kPlain ? 384u + 32u * kLoadWarps : 384u;
+    // Weight gradients of 256 columns keep 128 sums a thread: registers move
+    // from the copying and issuing warps to the two groups that sum.
+    static constexpr bool kRegs = KIND == kGemmGrad && BN == 256u && !kPlain;
+    static constexpr int kRegsDown = 40, kRegsUp = 208;
+    static constexpr uint32_t kRegsNeeded = 128u * kRegsDown + 256u * kRegsUp;  // of the block's at launch
     static_assert(kSmem <= 232448u - 512u, "shared memory of one CTA");
 };
 
@@ -313,7 +371,7 @@ __global__ void __launch_bounds__(GemmShape<BN, KIND, FEED>::kThreads, 1) k_gemm
         }
         for (uint32_t i = 0; i < 2u; ++i) {
             umma::mbar_init(&bar.acc_full[i], 1u);
-            umma::mbar_init(&bar.acc_empty[i], 4u * kCtas);
+            umma::mbar_init(&bar.acc_empty[i], (KIND == kGemmGrad ? 8u : 4u) * kCtas);
         }
         umma::mbar_init(&bar.drain, 1u);
         umma::fence_mbar_init();
@@ -338,6 +396,7 @@ __global__ void __launch_bounds__(GemmShape<BN, KIND, FEED>::kThreads, 1) k_gemm
     umma::fence_after_sync();
     const uint32_t tmem = bar.tmem_base;
     const uint32_t tiles = g.tiles_m * g.tiles_n, items = tiles * g.splits;
+    if (S::kRegs && warp < 4u) tma::registers_down<S::kRegsDown>();
 
     if ((!S::kPlain && warp == 0u && lane == 0u) || (S::kPlain && warp >= 12u)) {
         // ---- producer: one thread issuing tensor copies, or warps of loads
@@ -411,7 +470,9 @@ __global__ void __launch_bounds__(GemmShape<BN, KIND, FEED>::kThreads, 1) k_gemm
         bool ok = true;
         for (uint32_t it = first_item; it < items && ok; it += item_step) {
             const uint32_t split = it / tiles;
-            const uint32_t ks0 = split * g.steps_per_split, ks1 = min(g.k_steps, (split + 1u) * g.steps_per_split);
+            const uint32_t end = min(g.k_steps, (split + 1u) * g.steps_per_split);
+            for (uint32_t ks0 = split * g.steps_per_split, ks1; ks0 < end && ok; ks0 = ks1) {  // one accumulator's steps
+            ks1 = KIND == kGemmGrad ? min(end, ks0 + kChunkSteps) : end;
             if (!tma::wait(&bar.acc_empty[acc], acc_parity)) {
                 ok = false;
                 break;
@@ -445,6 +506,7 @@ __global__ void __launch_bounds__(GemmShape<BN, KIND, FEED>::kThreads, 1) k_gemm
             }
             acc ^= 1u;
             if (acc == 0u) acc_parity ^= 1u;
+            }
         }
         if (!ok) {  // the MMAs issued so far end before the tensor memory is freed
             atomicOr(g.error, 1u);
@@ -452,9 +514,105 @@ __global__ void __launch_bounds__(GemmShape<BN, KIND, FEED>::kThreads, 1) k_gemm
             else umma::commit(&bar.drain);
             tma::wait(&bar.drain, 0u);
         }
-    } else if (warp >= 4u && warp < 12u) {
+    } else if (KIND == kGemmGrad && warp >= 4u && warp < 12u) {
+        // ---- epilogue of a weight gradient: group h sums the chunks' columns
+        // h BN / 2 .. in registers, rows 32 q .. 32 q + 31 of the tile a warp
+        constexpr uint32_t kHalf = BN / 2u;
+        const uint32_t q = warp & 3u, h = (warp >> 2) - 1u, row = 32u * q + lane;
+        unsigned char* slab = slabs + (warp - 4u) * S::kSlabs * kSlabBytes;
+        if (S::kRegs) tma::registers_up<S::kRegsUp>();
+        uint32_t acc = 0, parity = 0;
+        bool ok = true;
+        for (uint32_t it = first_item; it < items && ok; it += item_step) {
+            const uint32_t split = it / tiles, tile = it - split * tiles;
+            uint32_t tm, tn;
+            tile_of(g, tile, tm, tn);
+            const uint32_t m0 = (tm * kCtas + rank) * kBM + 32u * q, n0 = tn * BN + h * kHalf;
+            const uint32_t rows = m0 < g.M ? min(32u, g.M - m0) : 0u;
+            const uint32_t ks0 = split * g.steps_per_split, ks1 = min(g.k_steps, (split + 1u) * g.steps_per_split);
+            float s[kHalf];
+#pragma unroll
+            for (uint32_t i = 0; i < kHalf; ++i) s[i] = 0.0f;
+            for (uint32_t ks = ks0; ks < ks1 && ok; ks += kChunkSteps) {
+                if (!tma::wait(&bar.acc_full[acc], parity)) {
+                    atomicOr(g.error, 1u);
+                    ok = false;
+                }
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                umma::fence_after_sync();
+#pragma unroll
+                for (uint32_t c = 0; c < kHalf; c += 16u) {
+                    float v[16];
+                    umma::tmem_ld16(tmem + acc * BN + h * kHalf + c + ((32u * q) << 16), v);
+#pragma unroll
+                    for (uint32_t i = 0; i < 16u; ++i) s[c + i] += v[i];
+                }
+                umma::fence_before_sync();
+                __syncwarp();
+                if (lane == 0u) {
+                    if (S::kPair) tma::arrive_at(tma::peer_addr(smem_u32(&bar.acc_empty[acc]), 0u));
+                    else tma::arrive(&bar.acc_empty[acc]);
+                }
+                acc ^= 1u;
+                if (acc == 0u) parity ^= 1u;
+            }
+            if (!ok) break;
+            if (g.splits > 1u) {
+                // Partial tile, four columns of 128 rows at a time: 512 contiguous bytes a warp store.
+                float4* dst = reinterpret_cast<float4*>(g.partials) +
+                              (static_cast<uint64_t>(it * kCtas + rank) * (BN / 4u) + h * (kHalf / 4u)) * kBM + row;
+#pragma unroll
+                for (uint32_t i = 0; i < kHalf / 4u; ++i)
+                    if (n0 + 4u * i < g.N) dst[i * kBM] = make_float4(s[4 * i], s[4 * i + 1], s[4 * i + 2], s[4 * i + 3]);
+                continue;
+            }
+            // The gradient itself, 32 columns at a time: 128 or 64 bytes a row of the slab.
+            const uint32_t es = g.dw_f32 ? 4u : 2u;
+#pragma unroll
+            for (uint32_t c0 = 0; c0 < kHalf; c0 += 32u) {
+                if (n0 + c0 >= g.N) break;
+                const uint32_t cols = min(32u, g.N - n0 - c0);
+                unsigned char* at = static_cast<unsigned char*>(g.dw) + (static_cast<uint64_t>(m0) * g.N + n0 + c0) * es;
+                if (g.accumulate) {
+                    if (g.dw_f32) slab_copy<4, false>(slab, at, g.N, rows, cols, g.dw_vec != 0u, lane);
+                    else slab_copy<2, false>(slab, at, g.N, rows, cols, g.dw_vec != 0u, lane);
+                    __syncwarp();
+                }
+                if (g.dw_f32) {
+#pragma unroll
+                    for (uint32_t p = 0; p < 8u; ++p) {
+                        float4* l = reinterpret_cast<float4*>(slab + slab_at(lane, p));
+                        float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                        if (g.accumulate) o = *l;
+                        const uint32_t i = c0 + 4u * p;
+                        *l = make_float4(o.x + s[i], o.y + s[i + 1], o.z + s[i + 2], o.w + s[i + 3]);
+                    }
+                } else {
+#pragma unroll
+                    for (uint32_t p = 0; p < 4u; ++p) {
+                        uint4* l = reinterpret_cast<uint4*>(slab + slab_at(lane, p));
+                        uint4 o = make_uint4(0u, 0u, 0u, 0u);
+                        if (g.accumulate) o = *l;
+                        const uint32_t ow[4] = {o.x, o.y, o.z, o.w};
+                        uint32_t w[4];
+#pragma unroll
+                        for (uint32_t i = 0; i < 4u; ++i) {
+                            const float2 f = unpack_16(ow[i], bf16);
+                            w[i] = pack_16(f.x + s[c0 + 8u * p + 2u * i], f.y + s[c0 + 8u * p + 2u * i + 1u], bf16);
+                        }
+                        *l = make_uint4(w[0], w[1], w[2], w[3]);
+                    }
+                }
+                __syncwarp();
+                if (g.dw_f32) slab_copy<4, true>(slab, at, g.N, rows, cols, g.dw_vec != 0u, lane);
+                else slab_copy<2, true>(slab, at, g.N, rows, cols, g.dw_vec != 0u, lane);
+                __syncwarp();
+            }
+        }
+    } else if (KIND == kGemmRows && warp >= 4u && warp < 12u) {
         // ---- epilogue: warp q of a group drains rows 32 q .. 32 q + 31 of the tile
-        const uint32_t q = warp & 3u, acc = (warp >> 2) - 1u, row = 32u * q + lane;
+        const uint32_t q = warp & 3u, acc = (warp >> 2) - 1u;
         unsigned char* my_slabs = slabs + (warp - 4u) * S::kSlabs * kSlabBytes;
         uint16_t* bias_s = bias_all + acc * BN;
         const uint32_t taddr = tmem + acc * BN + ((32u * q) << 16);
@@ -475,12 +633,24 @@ __global__ void __launch_bounds__(GemmShape<BN, KIND, FEED>::kThreads, 1) k_gemm
             tile_of(g, tile, tm, tn);
             const uint32_t m0 = (tm * kCtas + rank) * kBM + 32u * q, n0 = tn * BN;
             const uint32_t rows = m0 < g.M ? min(32u, g.M - m0) : 0u;
-            if (KIND == kGemmRows && n0 != bias_n) {  // the tile's bias, kept while the columns stay the same
+            if (n0 != bias_n) {  // the tile's bias, kept while the columns stay the same
                 asm volatile("bar.sync %0, 128;\n" ::"r"(1u + acc) : "memory");
                 for (uint32_t c = threadIdx.x & 127u; c < BN; c += 128u)
                     bias_s[c] = g.bias && n0 + c < g.N ? static_cast<const uint16_t*>(g.bias)[n0 + c] : static_cast<uint16_t>(0);
                 asm volatile("bar.sync %0, 128;\n" ::"r"(1u + acc) : "memory");
                 bias_n = n0;
+            }
+            if (g.res_tma && lane == 0u) {
+                // The residual of this group's next tile (and of its first) on its way to the L2 cache.
+                for (uint32_t w = it == first_item + acc * item_step ? 0u : 1u; w < 2u; ++w) {
+                    const uint32_t jt = it + 2u * w * item_step;
+                    if (jt >= items) break;
+                    uint32_t jm, jn;
+                    tile_of(g, jt, jm, jn);
+                    const uint32_t jr = (jm * kCtas + rank) * kBM + 32u * q;
+                    for (uint32_t c = jn * BN; jr < g.M && c < min(jn * BN + BN, g.N); c += 64u)
+                        tma::prefetch_2d(&maps.res, static_cast<int32_t>(c), static_cast<int32_t>(jr));
+                }
             }
             if (ok && !tma::wait(&bar.acc_full[acc], parity)) {
                 atomicOr(g.error, 1u);
@@ -489,7 +659,7 @@ __global__ void __launch_bounds__(GemmShape<BN, KIND, FEED>::kThreads, 1) k_gemm
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) continue;
             umma::fence_after_sync();
-            if (KIND == kGemmRows) {
+            {
                 for (uint32_t c0 = 0; c0 < BN && n0 + c0 < g.N; c0 += 64u) {
                     const uint32_t cols = min(64u, g.N - n0 - c0);
                     if (g.pre.ptr) {
@@ -530,62 +700,6 @@ __global__ void __launch_bounds__(GemmShape<BN, KIND, FEED>::kThreads, 1) k_gemm
                     }
                     slab_out(slab, g.y, g.y_tma != 0u, &maps.y, m0, n0 + c0, rows, cols, lane);
                 }
-            } else if (g.splits > 1u) {
-                // Partial tile, four columns of 128 rows at a time: 512 contiguous bytes a warp store.
-                float4* dst = reinterpret_cast<float4*>(g.partials) +
-                              static_cast<uint64_t>(it * kCtas + rank) * (BN / 4u) * kBM + row;
-                for (uint32_t c0 = 0; c0 < BN && n0 + c0 < g.N; c0 += 32u) {
-                    float v[32];
-                    umma::tmem_ld32(taddr + c0, v);
-#pragma unroll
-                    for (uint32_t i = 0; i < 8u; ++i)
-                        dst[(c0 / 4u + i) * kBM] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
-                }
-            } else {
-                // The gradient itself: 32 fp32 or 64 16-bit columns (128 bytes) a slab.
-                unsigned char* slab = my_slabs;
-                const uint32_t es = g.dw_f32 ? 4u : 2u, wide = 128u / es;
-                for (uint32_t c0 = 0; c0 < BN && n0 + c0 < g.N; c0 += wide) {
-                    const uint32_t cols = min(wide, g.N - n0 - c0);
-                    unsigned char* at = static_cast<unsigned char*>(g.dw) + (static_cast<uint64_t>(m0) * g.N + n0 + c0) * es;
-                    if (g.accumulate) {
-                        if (g.dw_f32) slab_copy<4, false>(slab, at, g.N, rows, cols, g.dw_vec != 0u, lane);
-                        else slab_copy<2, false>(slab, at, g.N, rows, cols, g.dw_vec != 0u, lane);
-                        __syncwarp();
-                    }
-                    for (uint32_t h = 0; h < wide; h += 32u) {
-                        float v[32];
-                        umma::tmem_ld32(taddr + c0 + h, v);
-                        if (g.dw_f32) {
-#pragma unroll
-                            for (uint32_t p = 0; p < 8u; ++p) {
-                                float4* l = reinterpret_cast<float4*>(slab + slab_at(lane, p));
-                                float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                                if (g.accumulate) o = *l;
-                                *l = make_float4(o.x + v[4 * p], o.y + v[4 * p + 1], o.z + v[4 * p + 2], o.w + v[4 * p + 3]);
-                            }
-                        } else {
-                            if (g.accumulate) {
-#pragma unroll
-                                for (uint32_t p = 0; p < 4u; ++p) {
-                                    const uint4 u = *reinterpret_cast<const uint4*>(slab + slab_at(lane, p + h / 8u));
-                                    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-                                    for (int i = 0; i < 4; ++i) {
-                                        const float2 f = unpack_16(w[i], bf16);
-                                        v[8 * p + 2 * i] += f.x;
-                                        v[8 * p + 2 * i + 1] += f.y;
-                                    }
-                                }
-                            }
-                            slab_put32(slab, lane, h / 32u, v, bf16);
-                        }
-                    }
-                    __syncwarp();
-                    if (g.dw_f32) slab_copy<4, true>(slab, at, g.N, rows, cols, g.dw_vec != 0u, lane);
-                    else slab_copy<2, true>(slab, at, g.N, rows, cols, g.dw_vec != 0u, lane);
-                    __syncwarp();
-                }
             }
             umma::fence_before_sync();
             __syncwarp();
@@ -610,7 +724,21 @@ __global__ void __launch_bounds__(GemmShape<BN, KIND, FEED>::kThreads, 1) k_gemm
 // ------------------------------------------------- dz and its column sums
 // 256 threads: 8 columns a thread, `cg` column groups side by side (a power of
 // two up to 32), 256 / cg rows at a time.
-__global__ void __launch_bounds__(256) k_dz(const DzArgs a, uint32_t cg_log2) {
+NB_DEV void dz_row(uint32_t (&w)[4], const uint16_t* q, uint32_t have, bool vec) {
+    w[0] = w[1] = w[2] = w[3] = 0u;
+    if (have == 8u && vec) {
+        const uint4 u = *reinterpret_cast<const uint4*>(q);
+        w[0] = u.x; w[1] = u.y; w[2] = u.z; w[3] = u.w;
+    } else {
+        uint16_t h[8];
+#pragma unroll
+        for (uint32_t i = 0; i < 8u; ++i) h[i] = i < have ? q[i] : static_cast<uint16_t>(0);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = static_cast<uint32_t>(h[2 * i]) | (static_cast<uint32_t>(h[2 * i + 1]) << 16);
+    }
+}
+template <uint32_t ACT, bool VEC>
+__global__ void __launch_bounds__(256, 4) k_dz(const DzArgs a, uint32_t cg_log2) {
     __shared__ float sums[256][8];
     const bool bf16 = a.bf16 != 0u;
     const uint32_t cg = 1u << cg_log2, gx = threadIdx.x & (cg - 1u), gy = threadIdx.x >> cg_log2, ny = 256u >> cg_log2;
@@ -620,43 +748,34 @@ __global__ void __launch_bounds__(256) k_dz(const DzArgs a, uint32_t cg_log2) {
     if (have) {
         const uint64_t r0 = static_cast<uint64_t>(blockIdx.y) * a.rows_per_part;
         const uint64_t r1 = min(static_cast<uint64_t>(a.dy.rows), r0 + a.rows_per_part);
-        for (uint64_t r = r0 + gy; r < r1; r += ny) {
-            const uint16_t* qd = static_cast<const uint16_t*>(a.dy.ptr) + r * a.dy.ld + c0;
-            uint32_t d[4] = {0u, 0u, 0u, 0u}, z[4] = {0u, 0u, 0u, 0u};
-            if (have == 8u && a.dy.vec >= 8u) {
-                const uint4 u = *reinterpret_cast<const uint4*>(qd);
-                d[0] = u.x; d[1] = u.y; d[2] = u.z; d[3] = u.w;
-            } else {
+        const uint16_t* qd = static_cast<const uint16_t*>(a.dy.ptr) + c0;
+        const uint16_t* qz = static_cast<const uint16_t*>(a.pre.ptr) + c0;
+        constexpr uint32_t kRows = VEC ? 4u : 2u;  // in flight a thread
+        for (uint64_t r = r0 + gy; r < r1; r += kRows * ny) {
+            uint32_t d[kRows][4], z[kRows][4];
 #pragma unroll
-                for (uint32_t i = 0; i < 8u; ++i)
-                    if (i < have) d[i / 2u] |= static_cast<uint32_t>(qd[i]) << (16u * (i & 1u));
+            for (uint32_t k = 0; k < kRows; ++k) {
+                const uint64_t at = r + k * ny;
+                dz_row(d[k], qd + at * a.dy.ld, at < r1 ? have : 0u, VEC);
+                dz_row(z[k], qz + at * a.pre.ld, at < r1 && ACT != kActNone ? have : 0u, VEC);
             }
-            if (a.act != kActNone) {
-                const uint16_t* qz = static_cast<const uint16_t*>(a.pre.ptr) + r * a.pre.ld + c0;
-                if (have == 8u && a.pre.vec >= 8u) {
-                    const uint4 u = *reinterpret_cast<const uint4*>(qz);
-                    z[0] = u.x; z[1] = u.y; z[2] = u.z; z[3] = u.w;
-                } else {
 #pragma unroll
-                    for (uint32_t i = 0; i < 8u; ++i)
-                        if (i < have) z[i / 2u] |= static_cast<uint32_t>(qz[i]) << (16u * (i & 1u));
+            for (uint32_t k = 0; k < kRows; ++k) {
+                const uint64_t at = r + k * ny;
+                float f[8];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float2 dd = unpack_16(d[k][i], bf16), zz = unpack_16(z[k][i], bf16);
+                    f[2 * i] = dact_f(dd.x, zz.x, ACT);
+                    f[2 * i + 1] = dact_f(dd.y, zz.y, ACT);
                 }
-            }
-            uint32_t o[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                float2 f = unpack_16(d[i], bf16);
-                if (a.act != kActNone) {
-                    const float2 zz = unpack_16(z[i], bf16);
-                    f.x = dact_f(f.x, zz.x, a.act);
-                    f.y = dact_f(f.y, zz.y, a.act);
-                }
-                s[2 * i] += f.x;
-                s[2 * i + 1] += f.y;
-                o[i] = pack_16(f.x, f.y, bf16);  // the tensor cores take 16-bit operands
+                for (int i = 0; i < 8; ++i) s[i] += f[i];
+                // The tensor cores take 16-bit operands.  Rows of dz are padded to a multiple of 8 values.
+                if (a.dz && at < r1)
+                    *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.dz) + at * a.dz_ld + c0) =
+                        make_uint4(pack_16(f[0], f[1], bf16), pack_16(f[2], f[3], bf16), pack_16(f[4], f[5], bf16), pack_16(f[6], f[7], bf16));
             }
-            // dz rows are padded to a multiple of 8 values
-            if (a.dz) *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.dz) + r * a.dz_ld + c0) = make_uint4(o[0], o[1], o[2], o[3]);
         }
     }
     if (!a.db_part) return;
@@ -717,7 +836,7 @@ __global__ void __launch_bounds__(256) k_grad_reduce(const GradReduceArgs a, uin
     const uint32_t per = (a.parts + 7u) / 8u, p0 = min(a.parts, warp * per), p1 = min(a.parts, p0 + per);
     float t = 0.0f;
     if (c < a.n_out) {
-#pragma unroll 8
+#pragma unroll 16
         for (uint32_t p = p0; p < p1; ++p) t += a.db_part[static_cast<uint64_t>(p) * a.n_out + c];
     }
     ws[warp][lane] = t;
@@ -742,6 +861,10 @@ cudaError_t launch_gemm_t(const GemmArgs& g, const GemmMaps& maps, uint32_t bloc
     if (!done[dev]) {
         e = cudaFuncSetAttribute(k_gemm<BN, KIND, FEED>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
         if (e != cudaSuccess) return e;
+        cudaFuncAttributes fa{};
+        if ((e = cudaFuncGetAttributes(&fa, k_gemm<BN, KIND, FEED>)) != cudaSuccess) return e;
+        // Registers that move between warpgroups have to be there at launch.
+        if (S::kRegs && static_cast<uint32_t>(fa.numRegs) * S::kThreads < S::kRegsNeeded) return cudaErrorInvalidConfiguration;
         done[dev] = true;
     }
     cudaLaunchConfig_t cfg{};
@@ -762,7 +885,9 @@ cudaError_t launch_gemm_bn(const GemmArgs& g, uint32_t bn, const GemmMaps& maps,
     switch (bn) {
         case 64u: return launch_gemm_t<64u, KIND, FEED>(g, maps, blocks, s);
         case 128u: return launch_gemm_t<128u, KIND, FEED>(g, maps, blocks, s);
-        case 256u: return launch_gemm_t<256u, KIND, FEED>(g, maps, blocks, s);
+        case 256u:
+            if constexpr (KIND == kGemmRows || FEED != kFeedPlain) return launch_gemm_t<256u, KIND, FEED>(g, maps, blocks, s);
+            return cudaErrorInvalidValue;
         default: return cudaErrorInvalidValue;
     }
 }
@@ -789,7 +914,16 @@ cudaError_t launch_dz(const DzArgs& a, cudaStream_t s) {
     uint32_t log2 = 0;
     while (log2 < 5u && (1u << log2) < groups) ++log2;
     const dim3 grid((groups + (1u << log2) - 1u) >> log2, a.parts);
-    k_dz<<<grid, 256, 0, s>>>(a, log2);
+    const bool vec = a.dy.vec >= 8u && (a.act == kActNone || a.pre.vec >= 8u);
+    switch (a.act) {
+        case kActRelu: vec ? k_dz<kActRelu, true><<<grid, 256, 0, s>>>(a, log2) : k_dz<kActRelu, false><<<grid, 256, 0, s>>>(a, log2); break;
+        case kActSilu: vec ? k_dz<kActSilu, true><<<grid, 256, 0, s>>>(a, log2) : k_dz<kActSilu, false><<<grid, 256, 0, s>>>(a, log2); break;
+        case kActGelu: vec ? k_dz<kActGelu, true><<<grid, 256, 0, s>>>(a, log2) : k_dz<kActGelu, false><<<grid, 256, 0, s>>>(a, log2); break;
+        case kActSigmoid:
+            vec ? k_dz<kActSigmoid, true><<<grid, 256, 0, s>>>(a, log2) : k_dz<kActSigmoid, false><<<grid, 256, 0, s>>>(a, log2);
+            break;
+        default: vec ? k_dz<kActNone, true><<<grid, 256, 0, s>>>(a, log2) : k_dz<kActNone, false><<<grid, 256, 0, s>>>(a, log2); break;
+    }
     return cudaGetLastError();
 }
 

@@ -35,7 +35,8 @@ struct GemmArgs {
     // epilogue of an activation output: y = act(D + bias) + res, pre = D + bias
     const void* bias;
     MatrixView res, y, pre;  // ptr null: none
-    uint32_t y_tma, pre_tma; // stored by the tensor copy unit (rows on 16-byte boundaries)
+    uint32_t y_tma, pre_tma; // stored by the tensor copy unit (rows of whole 16-byte pieces)
+    uint32_t res_tma;        // prefetched by it
     // epilogue of a weight gradient: partials when splits > 1, else dw (+)= D
     float* partials;
     void* dw;
@@ -46,7 +47,7 @@ struct GemmArgs {
 enum GemmKind : int { kGemmRows = 0, kGemmGrad = 1 };
 
 struct GemmMaps {
-    CUtensorMap a, b, y, pre;
+    CUtensorMap a, b, y, pre, res;
 };
 // How a product's operands reach shared memory: copied for one CTA a tile,
 // copied for a pair of CTAs on one 256 x 256 tile, or loaded by warps.

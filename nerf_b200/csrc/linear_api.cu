@@ -112,48 +112,61 @@ bool pair_pays(uint64_t m, uint64_t n, uint64_t k, uint32_t sms) {
     return k >= 512u && static_cast<uint64_t>(ceil_div(m, 256u)) * ceil_div(n, 256u) >= sms / 2u;
 }
 
+// The weight gradient's tiles, and the row ranges that each is split into.
+struct GradPlan {
+    bool pair;
+    uint32_t bn, tiles_m, tiles_n, splits, k_steps, steps_per_split;
+    uint64_t bytes;  // partial tiles
+};
+GradPlan plan_grad(const NerfB200Linear& d, bool plain, uint32_t sms) {
+    GradPlan p{};
+    p.pair = !plain && pair_pays(d.n_out, d.n_in, d.n_rows, sms);
+    // 256 columns need registers that the loading warps hold in a plain product.
+    p.bn = d.n_in <= 64u ? 64u : d.n_in <= 128u || plain ? 128u : 256u;
+    p.tiles_m = ceil_div(d.n_out, p.pair ? 2u * kGemmBM : kGemmBM);
+    p.tiles_n = ceil_div(d.n_in, p.bn);
+    p.k_steps = ceil_div(d.n_rows, kGemmBK);
+    // One wave of (tile, row range) items, each range at least four steps.
+    const uint64_t tiles = static_cast<uint64_t>(p.tiles_m) * p.tiles_n;
+    const uint32_t slots = p.pair ? sms / 2u : sms;
+    uint64_t splits = tiles >= slots ? 1u : slots / tiles;
+    if (splits > ceil_div(p.k_steps, 4u)) splits = ceil_div(p.k_steps, 4u);
+    if (splits < 1u) splits = 1u;
+    p.steps_per_split = ceil_div(p.k_steps, splits);
+    p.splits = p.steps_per_split ? ceil_div(p.k_steps, p.steps_per_split) : 1u;
+    if (p.splits > 1u) p.bytes = p.splits * tiles * (p.pair ? 2u : 1u) * kGemmBM * p.bn * 4u;
+    return p;
+}
+
 struct BackwardPlan {
     uint32_t sms;
-    bool dz_needed;                     // dz is not dy itself
+    bool dz_needed;                 // dz is not dy itself
     uint64_t dz_ld;
-    uint32_t parts, rows_per_part;      // row ranges of the column sums
-    bool pair;                          // weight gradient: the tiles are those of a pair of CTAs, where it can be fed
-    uint32_t bn, tiles_m, tiles_n, splits, k_steps, steps_per_split;  // weight gradient
-    uint64_t o_dz, o_db, o_dw, bytes;   // workspace
+    uint32_t parts, rows_per_part;  // row ranges of the column sums
+    uint64_t o_dz, o_db, o_dw, bytes;  // workspace
 };
 BackwardPlan plan_backward(const NerfB200Linear& d) {
     BackwardPlan p{};
     p.sms = current_sms();
     p.dz_needed = d.activation != kActNone;
     p.dz_ld = up(d.n_out, 8u);
-    // About six 256-thread blocks an SM, each with at least 64 rows.
+    // One wave of four 256-thread blocks an SM, each with at least 128 rows.
     const uint32_t groups = ceil_div(d.n_out, 8u), gx = ceil_div(groups, 32u);
-    uint64_t parts = 6ull * p.sms / gx;
-    if (parts > ceil_div(d.n_rows, 64u)) parts = ceil_div(d.n_rows, 64u);
+    uint64_t parts = 4ull * p.sms / gx;
+    if (parts > ceil_div(d.n_rows, 128u)) parts = ceil_div(d.n_rows, 128u);
     if (parts < 1u) parts = 1u;
     p.rows_per_part = ceil_div(d.n_rows, parts);
     if (p.rows_per_part == 0u) p.rows_per_part = 1u;
     p.parts = ceil_div(d.n_rows, p.rows_per_part);
-    p.bn = d.n_in <= 64u ? 64u : d.n_in <= 128u ? 128u : 256u;
-    p.pair = pair_pays(d.n_out, d.n_in, d.n_rows, p.sms);
-    p.tiles_m = ceil_div(d.n_out, p.pair ? 2u * kGemmBM : kGemmBM);
-    p.tiles_n = ceil_div(d.n_in, p.bn);
-    p.k_steps = ceil_div(d.n_rows, kGemmBK);
-    // One wave of (tile, row range) items, each range at least four steps.
-    const uint64_t tiles = static_cast<uint64_t>(p.tiles_m) * p.tiles_n;
-    const uint32_t slots = p.pair ? p.sms / 2u : p.sms;
-    uint64_t splits = tiles >= slots ? 1u : slots / tiles;
-    if (splits > ceil_div(p.k_steps, 4u)) splits = ceil_div(p.k_steps, 4u);
-    if (splits < 1u) splits = 1u;
-    p.steps_per_split = ceil_div(p.k_steps, splits);
-    p.splits = p.steps_per_split ? ceil_div(p.k_steps, p.steps_per_split) : 1u;
     uint64_t at = 0;
     p.o_dz = at;
     if (p.dz_needed) at += up(static_cast<uint64_t>(d.n_rows) * p.dz_ld * 2u, 256u);
     p.o_db = at;
     at += up(static_cast<uint64_t>(p.parts) * d.n_out * 4u, 256u);
     p.o_dw = at;
-    if (p.splits > 1u) at += static_cast<uint64_t>(p.splits) * tiles * (p.pair ? 2u : 1u) * kGemmBM * p.bn * 4u;
+    // How the operands can be fed depends on the pointers: room for either way.
+    const uint64_t tma = plan_grad(d, false, p.sms).bytes, plain = plan_grad(d, true, p.sms).bytes;
+    at += tma > plain ? tma : plain;
     p.bytes = at ? at : 256u;
     return p;
 }
@@ -187,7 +200,8 @@ cudaError_t run_gemm(GemmArgs& g, int kind, uint32_t bn, bool pair, uint32_t sms
     // The copy unit writes whole 16-byte pieces: a row must end with one.
     g.y_tma = g.y.ptr && g.y.vec >= 8u && g.y.cols % 8u == 0u;
     g.pre_tma = g.pre.ptr && g.pre.vec >= 8u && g.pre.cols % 8u == 0u;
-    if ((g.y_tma && !make_map(&maps.y, g.y, 32u, bf16)) || (g.pre_tma && !make_map(&maps.pre, g.pre, 32u, bf16)))
+    g.res_tma = g.res.ptr && g.res.vec >= 8u;
+    if ((g.res_tma && !make_map(&maps.res, g.res, 32u, bf16)) || (g.y_tma && !make_map(&maps.y, g.y, 32u, bf16)) || (g.pre_tma && !make_map(&maps.pre, g.pre, 32u, bf16)))
         return cudaErrorNotSupported;
     const uint64_t items = static_cast<uint64_t>(g.tiles_m) * g.tiles_n * g.splits, slots = pair ? sms / 2u : sms;
     const uint32_t blocks = static_cast<uint32_t>(items < slots ? items : slots) * (pair ? 2u : 1u);
@@ -328,13 +342,12 @@ NERF_API NerfStatus nerf_b200_linear_backward(const NerfB200Linear* desc, const 
         g.a = dzv;
         g.b = view(x, ld_or(d.ld_x, d.n_in), d.n_rows, d.n_in);
         g.a_mn = g.b_mn = 1u;
-        // A pair's plan on rows that only warps can load: the same tiles' 128-row halves.
-        const bool pair = p.pair && g.a.vec >= 8u && g.b.vec >= 8u;
-        g.tiles_m = p.pair && !pair ? ceil_div(d.n_out, kGemmBM) : p.tiles_m;
-        g.tiles_n = p.tiles_n;
-        g.splits = p.splits;
-        g.k_steps = p.k_steps;
-        g.steps_per_split = p.steps_per_split;
+        const GradPlan w = plan_grad(d, g.a.vec < 8u || g.b.vec < 8u, p.sms);
+        g.tiles_m = w.tiles_m;
+        g.tiles_n = w.tiles_n;
+        g.splits = w.splits;
+        g.k_steps = w.k_steps;
+        g.steps_per_split = w.steps_per_split;
         g.bf16 = bf16;
         g.partials = reinterpret_cast<float*>(ws + p.o_dw);
         g.dw = dweight;
@@ -342,14 +355,14 @@ NERF_API NerfStatus nerf_b200_linear_backward(const NerfB200Linear* desc, const 
         g.dw_vec = aligned(dweight, 16u) && (es * d.n_in) % 16u == 0u;
         g.accumulate = d.accumulate;
         g.error = error_word;
-        if (run_gemm(g, kGemmGrad, p.bn, pair, p.sms, s) != cudaSuccess) return NERF_STATUS_CUDA_ERROR;
-        if (p.splits > 1u) {
+        if (run_gemm(g, kGemmGrad, w.bn, w.pair, p.sms, s) != cudaSuccess) return NERF_STATUS_CUDA_ERROR;
+        if (w.splits > 1u) {
             r.partials = g.partials;
-            r.splits = p.splits;
-            r.ctas = pair ? 2u : 1u;
-            r.tiles_m = g.tiles_m;
-            r.tiles_n = p.tiles_n;
-            r.bn = p.bn;
+            r.splits = w.splits;
+            r.ctas = w.pair ? 2u : 1u;
+            r.tiles_m = w.tiles_m;
+            r.tiles_n = w.tiles_n;
+            r.bn = w.bn;
             r.dw = dweight;
         }
     }

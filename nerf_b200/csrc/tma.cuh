@@ -52,6 +52,10 @@ NB_DEV void store_2d(const CUtensorMap* map, uint32_t src, int32_t x, int32_t y)
     asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];\n" ::"l"(map), "r"(x), "r"(y), "r"(src)
                  : "memory");
 }
+// A box into the L2 cache, ahead of its loads.
+NB_DEV void prefetch_2d(const CUtensorMap* map, int32_t x, int32_t y) {
+    asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global [%0, {%1, %2}];\n" ::"l"(map), "r"(x), "r"(y) : "memory");
+}
 NB_DEV void store_commit() { asm volatile("cp.async.bulk.commit_group;\n" ::: "memory"); }
 // At most N of this thread's store groups still read shared memory.
 template <int N>
@@ -92,6 +96,16 @@ NB_DEV bool wait(uint64_t* mbar, uint32_t parity) {
             else if (t - t0 > kWaitLimitNs) return false;
         }
     }
+}
+
+// Registers of the executing warpgroup's threads from here on.
+template <int N>
+NB_DEV void registers_down() {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(N));
+}
+template <int N>
+NB_DEV void registers_up() {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(N));
 }
 
 // ---- a pair of CTAs on one MMA (cta_group::2) ----
