@@ -127,6 +127,25 @@ NB_DEV float dact_f(float dy, float z, uint32_t act) {
     }
 }
 
+// Loads that read nothing and give zero where `on` is false: predicated, so
+// that a batch of them is in flight together (as branches each would wait for
+// the one before).
+NB_DEV uint32_t load_16(const uint16_t* q, bool on) {
+    uint32_t v;
+    asm volatile(
+        "{\n.reg .pred p;\n.reg .u16 h;\nsetp.ne.u32 p, %2, 0;\nmov.u16 h, 0;\n@p ld.global.u16 h, [%1];\ncvt.u32.u16 %0, h;\n}\n"
+        : "=r"(v)
+        : "l"(q), "r"(static_cast<uint32_t>(on)));
+    return v;
+}
+NB_DEV uint32_t load_32(const void* q, bool on) {
+    uint32_t v;
+    asm volatile("{\n.reg .pred p;\nsetp.ne.u32 p, %2, 0;\nmov.u32 %0, 0;\n@p ld.global.u32 %0, [%1];\n}\n"
+                 : "=r"(v)
+                 : "l"(q), "r"(static_cast<uint32_t>(on)));
+    return v;
+}
+
 // ------------------------------------------------- slabs: 32 rows x 128 bytes
 // A warp's shared-memory slab, 16-byte pieces swizzled by the row so that both
 // "one row a thread" and "eight threads a row" accesses are conflict-free.
@@ -165,42 +184,42 @@ NB_DEV void slab_copy(unsigned char* slab, unsigned char* g, uint64_t ld, uint32
     // A row is 32 words of the slab: lane i moves word i, as one or two values.
     const bool words = ES == 4 || ((reinterpret_cast<uintptr_t>(g) & 3u) == 0u && (ld & 1u) == 0u);
     const bool lo = ES == 4 ? lane < cols : 2u * lane < cols, hi = ES == 4 ? lane < cols : 2u * lane + 1u < cols;
+    const uint64_t step = ld * ES;
     unsigned char* q = g + 4u * lane;
     constexpr uint32_t kBatch = 8;
+#pragma unroll 1
     for (uint32_t r0 = 0; r0 < rows; r0 += kBatch) {
+        const uint32_t in = rows - r0;
         uint32_t w[kBatch];
+        unsigned char* l[kBatch];
 #pragma unroll
-        for (uint32_t j = 0; j < kBatch; ++j) {
-            unsigned char* l = slab + slab_at(r0 + j, lane >> 2) + 4u * (lane & 3u);
-            if (kStore) {
-                w[j] = *reinterpret_cast<const uint32_t*>(l);
-            } else {
-                const unsigned char* p = q + j * ld * ES;
-                const bool live = r0 + j < rows;
-                if (words) {
-                    w[j] = live && hi ? *reinterpret_cast<const uint32_t*>(p) : live && lo ? *reinterpret_cast<const uint16_t*>(p) : 0u;
+        for (uint32_t j = 0; j < kBatch; ++j) l[j] = slab + slab_at(r0 + j, lane >> 2) + 4u * (lane & 3u);
+        if (kStore) {
+#pragma unroll
+            for (uint32_t j = 0; j < kBatch; ++j) w[j] = *reinterpret_cast<const uint32_t*>(l[j]);
+#pragma unroll
+            for (uint32_t j = 0; j < kBatch; ++j) {
+                unsigned char* p = q + j * step;
+                if (words && !(cols & 1u)) {
+                    if (hi && j < in) *reinterpret_cast<uint32_t*>(p) = w[j];
+                } else if (ES == 4) {
+                    if (lo && j < in) *reinterpret_cast<uint32_t*>(p) = w[j];
                 } else {
-                    w[j] = live && lo ? *reinterpret_cast<const uint16_t*>(p) : 0u;
-                    if (live && hi) w[j] |= static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(p)[1]) << 16;
+                    if (lo && j < in) *reinterpret_cast<uint16_t*>(p) = static_cast<uint16_t>(w[j]);
+                    if (hi && j < in) reinterpret_cast<uint16_t*>(p)[1] = static_cast<uint16_t>(w[j] >> 16);
                 }
             }
-        }
+        } else {
 #pragma unroll
-        for (uint32_t j = 0; j < kBatch; ++j) {
-            if (kStore) {
-                unsigned char* p = q + j * ld * ES;
-                if (r0 + j >= rows) break;
-                if (words && hi) {
-                    *reinterpret_cast<uint32_t*>(p) = w[j];
-                } else {
-                    if (lo) *reinterpret_cast<uint16_t*>(p) = static_cast<uint16_t>(w[j]);
-                    if (hi) reinterpret_cast<uint16_t*>(p)[1] = static_cast<uint16_t>(w[j] >> 16);
-                }
-            } else {
-                *reinterpret_cast<uint32_t*>(slab + slab_at(r0 + j, lane >> 2) + 4u * (lane & 3u)) = w[j];
+            for (uint32_t j = 0; j < kBatch; ++j) {
+                const uint16_t* p = reinterpret_cast<const uint16_t*>(q + j * step);
+                if (ES == 4 || (words && !(cols & 1u))) w[j] = load_32(p, hi && j < in);
+                else w[j] = load_16(p, lo && j < in) | (load_16(p + 1, hi && j < in) << 16);
             }
+#pragma unroll
+            for (uint32_t j = 0; j < kBatch; ++j) *reinterpret_cast<uint32_t*>(l[j]) = w[j];
         }
-        q += kBatch * ld * ES;
+        q += kBatch * step;
     }
 }
 NB_DEV void slab_put(unsigned char* slab, uint32_t row, uint32_t piece, const uint32_t w[4]) {
@@ -210,15 +229,16 @@ NB_DEV void slab_put(unsigned char* slab, uint32_t row, uint32_t piece, const ui
 // ------------------------------------------------------------- operand boxes
 constexpr uint32_t kLoadWarps = 8;
 
-// `rows` x 64 values at (row0, col0) of a matrix -> a swizzled box, zero
-// outside the matrix, by kLoadWarps warps.
-NB_DEV void fill_box(unsigned char* box, const MatrixView& m, uint32_t row0, uint32_t rows, uint32_t col0, uint32_t tid) {
+// ROWS x 64 values at (row0, col0) of a matrix -> a swizzled box, zero outside
+// the matrix, by kLoadWarps warps.
+template <uint32_t ROWS>
+NB_DEV void fill_box(unsigned char* box, const MatrixView& m, uint32_t row0, uint32_t col0, uint32_t tid) {
     const uint16_t* base = static_cast<const uint16_t*>(m.ptr);
     const uint32_t have = col0 < m.cols ? min(64u, m.cols - col0) : 0u;
     if (m.vec >= 8u && (have & 7u) == 0u) {
         // Whole 16-byte pieces: eight threads a row.
 #pragma unroll 4
-        for (uint32_t c = tid; c < rows * 8u; c += kLoadWarps * 32u) {
+        for (uint32_t c = tid; c < ROWS * 8u; c += kLoadWarps * 32u) {
             const uint32_t r = c >> 3, p = c & 7u;
             const uint64_t gr = static_cast<uint64_t>(row0) + r;
             uint4 u = make_uint4(0u, 0u, 0u, 0u);
@@ -227,43 +247,48 @@ NB_DEV void fill_box(unsigned char* box, const MatrixView& m, uint32_t row0, uin
         }
         return;
     }
-    // A warp a row, lane i the values 2 i and 2 i + 1: one 32-bit load where
-    // every row starts on a word, else two of 16 bits.  kBatch rows' loads are
-    // in flight before the first is stored.
+    // A warp every eighth row, lane i the values 2 i and 2 i + 1: one 32-bit
+    // load where every row starts on a word, else two of 16 bits.  A batch of
+    // rows is in flight before the first is stored, and only a box over the
+    // matrix's last rows looks at each row: the instructions a row are what
+    // bounds this path.
+    static_assert(kLoadWarps == 8u, "the swizzle of a warp's rows is the same");
+    constexpr uint32_t kBatch = ROWS / kLoadWarps < 16u ? ROWS / kLoadWarps : 16u;
     const uint32_t lane = tid & 31u, warp = tid >> 5;
-    constexpr uint32_t kBatch = 16;
-    const bool lo = 2u * lane < have, hi = 2u * lane + 1u < have, words = m.vec >= 2u;
-    for (uint32_t r0 = warp; r0 < rows; r0 += kLoadWarps * kBatch) {
+    const bool lo = 2u * lane < have, hi = 2u * lane + 1u < have, words = m.vec >= 2u && !(have & 1u);
+    const uint64_t step = kLoadWarps * m.ld;
+    unsigned char* dst = box + slab_at(warp, lane >> 2) + 4u * (lane & 3u);
+    const uint16_t* q = base + (static_cast<uint64_t>(row0) + warp) * m.ld + col0 + 2u * lane;
+#pragma unroll 1
+    for (uint32_t r0 = warp; r0 < ROWS; r0 += kLoadWarps * kBatch) {
         const uint32_t in = row0 + r0 < m.rows ? m.rows - row0 - r0 : 0u;  // matrix rows from r0 on
-        const uint16_t* q = base + (static_cast<uint64_t>(row0) + r0) * m.ld + col0 + 2u * lane;
-        const uint64_t step = kLoadWarps * m.ld;
-        uint32_t w[kBatch];
-        if (words) {
+        uint32_t w[kBatch], v[kBatch];
+        if (in > (kBatch - 1u) * kLoadWarps) {
+            if (words) {
 #pragma unroll
-            for (uint32_t j = 0; j < kBatch; ++j) {
-                const uint32_t r = j * kLoadWarps;
-                const bool live = r0 + r < rows && r < in;
-                w[j] = live && hi ? *reinterpret_cast<const uint32_t*>(q) : live && lo ? *q : 0u;
-                q += step;
+                for (uint32_t j = 0; j < kBatch; ++j) w[j] = load_32(q + j * step, hi);
+            } else {
+#pragma unroll
+                for (uint32_t j = 0; j < kBatch; ++j) {
+                    w[j] = load_16(q + j * step, lo);
+                    v[j] = load_16(q + j * step + 1, hi);
+                }
             }
         } else {
-            uint16_t v[kBatch];
 #pragma unroll
             for (uint32_t j = 0; j < kBatch; ++j) {
-                const uint32_t r = j * kLoadWarps;
-                const bool live = r0 + r < rows && r < in;
-                w[j] = live && lo ? q[0] : 0u;
-                v[j] = live && hi ? q[1] : static_cast<uint16_t>(0);
-                q += step;
+                w[j] = load_16(q + j * step, lo && j * kLoadWarps < in);
+                v[j] = load_16(q + j * step + 1, hi && j * kLoadWarps < in);
             }
+        }
+        if (!words || in <= (kBatch - 1u) * kLoadWarps) {
 #pragma unroll
-            for (uint32_t j = 0; j < kBatch; ++j) w[j] |= static_cast<uint32_t>(v[j]) << 16;
+            for (uint32_t j = 0; j < kBatch; ++j) w[j] |= v[j] << 16;
         }
 #pragma unroll
-        for (uint32_t j = 0; j < kBatch; ++j) {
-            const uint32_t r = r0 + j * kLoadWarps;
-            if (r < rows) *reinterpret_cast<uint32_t*>(box + slab_at(r, lane >> 2) + 4u * (lane & 3u)) = w[j];
-        }
+        for (uint32_t j = 0; j < kBatch; ++j) *reinterpret_cast<uint32_t*>(dst + j * kLoadWarps * 128u) = w[j];
+        q += kBatch * step;
+        dst += kBatch * kLoadWarps * 128u;
     }
 }
 
@@ -333,8 +358,8 @@ struct GemmShape {
     static constexpr bool kPair = FEED == kFeedPair, kPlain = FEED == kFeedPlain;
     static constexpr uint32_t kBoxN = kPair ? BN / 2u : BN;  // rows of B in this CTA's shared memory
     static constexpr uint32_t kStageBytes = kStageBytesA + kBoxN * 128u;
-    static constexpr uint32_t kStages = kPair ? 5u : BN >= 256u ? 4u : BN >= 128u ? 4u : 5u;
-    static constexpr uint32_t kSlabs = kPair ? 2u : BN >= 256u ? 1u : 2u;  // per epilogue warp
+    static constexpr uint32_t kStages = kPlain ? 2u : kPair ? 5u : BN >= 256u ? 4u : BN >= 128u ? 4u : 5u;
+    static constexpr uint32_t kSlabs = kPlain ? 1u : kPair ? 2u : BN >= 256u ? 1u : 2u;  // per epilogue warp
     static constexpr uint32_t kSmem = 1024u + kStages * kStageBytes + 8u * kSlabs * kSlabBytes + 2u * BN * 2u;
     static constexpr uint32_t kThreads = kPlain ? 384u + 32u * kLoadWarps : 384u;
     // Weight gradients of 256 columns keep 128 sums a thread: registers move
@@ -419,14 +444,14 @@ __global__ void __launch_bounds__(GemmShape<BN, KIND, FEED>::kThreads, 1) k_gemm
                 if (S::kPlain) {
                     const uint32_t tid = threadIdx.x - 384u;
                     if (g.a_mn) {
-                        for (uint32_t j = 0; j < kBM / 64u; ++j) fill_box(sa + j * 8192u, g.a, k0, kBK, m0 + 64u * j, tid);
+                        for (uint32_t j = 0; j < kBM / 64u; ++j) fill_box<kBK>(sa + j * 8192u, g.a, k0, m0 + 64u * j, tid);
                     } else {
-                        fill_box(sa, g.a, m0, kBM, k0, tid);
+                        fill_box<kBM>(sa, g.a, m0, k0, tid);
                     }
                     if (g.b_mn) {
-                        for (uint32_t j = 0; j < BN / 64u; ++j) fill_box(sb + j * 8192u, g.b, k0, kBK, n0 + 64u * j, tid);
+                        for (uint32_t j = 0; j < BN / 64u; ++j) fill_box<kBK>(sb + j * 8192u, g.b, k0, n0 + 64u * j, tid);
                     } else {
-                        fill_box(sb, g.b, n0, BN, k0, tid);
+                        fill_box<BN>(sb, g.b, n0, k0, tid);
                     }
                     umma::fence_async_smem();
                     tma::arrive(&bar.full[stage]);
