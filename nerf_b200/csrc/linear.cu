@@ -746,6 +746,205 @@ __global__ void __launch_bounds__(GemmShape<BN, KIND, FEED>::kThreads, 1) k_gemm
     }
 }
 
+// --------------------------------------------------------------- few rows
+// With few activation rows the weight's read is what takes the time: as many
+// CTAs as there are SMs have to read it, which the 128-row tiles of k_gemm
+// leave too few of.  Here the weight's rows fill the tensor core's 128 rows
+// and BN (16 to 128) activation rows its columns, and a cluster of `splits`
+// CTAs takes one tile, each a part of K.  Every CTA leaves its partial tile in
+// its own shared memory, and the cluster adds them in rank order over
+// distributed shared memory: no workspace, and the same bits every time.
+template <uint32_t BN, bool PLAIN>
+struct ColsShape {
+    static constexpr uint32_t kStageBytes = kStageBytesA + BN * 128u;
+    static constexpr uint32_t kStages = 4u;
+    static constexpr uint32_t kSmem = 1024u + kStages * kStageBytes;
+    static constexpr uint32_t kThreads = PLAIN ? 256u + 32u * kLoadWarps : 256u;
+    static_assert(BN * kBM * 4u <= kStages * kStageBytes, "the partial tile takes the stages' place");
+};
+
+template <uint32_t BN, bool PLAIN>
+__global__ void __launch_bounds__(ColsShape<BN, PLAIN>::kThreads) k_gemm_cols(const GemmArgs g, const __grid_constant__ GemmMaps maps) {
+    using S = ColsShape<BN, PLAIN>;
+    constexpr uint32_t kStages = S::kStages, kStageBytes = S::kStageBytes, kCols = tmem_cols(BN);
+    extern __shared__ unsigned char smem_raw[];
+    __shared__ uint64_t full[kStages], empty[kStages], acc_full, drain;
+    __shared__ uint32_t tmem_base, failed;
+    unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
+    const bool bf16 = g.bf16 != 0u;
+    const uint32_t rank = g.splits > 1u ? tma::cluster_rank() : 0u;
+    const uint32_t tile = blockIdx.x / g.splits, tm = tile % g.tiles_m, tn = tile / g.tiles_m;
+    const uint32_t m0 = tm * kBM, n0 = tn * BN;
+    const uint32_t ks0 = rank * g.steps_per_split, ks1 = min(g.k_steps, ks0 + g.steps_per_split);
+
+    if (threadIdx.x == 0u) {
+        for (uint32_t i = 0; i < kStages; ++i) {
+            umma::mbar_init(&full[i], PLAIN ? 32u * kLoadWarps : 1u);
+            umma::mbar_init(&empty[i], 1u);
+        }
+        umma::mbar_init(&acc_full, 1u);
+        umma::mbar_init(&drain, 1u);
+        umma::fence_mbar_init();
+        failed = 0u;
+    }
+    if (warp == 2u) {
+        umma::tmem_alloc(&tmem_base, kCols);
+        umma::tmem_relinquish();
+    }
+    umma::fence_before_sync();
+    __syncthreads();
+    umma::fence_after_sync();
+    const uint32_t tmem = tmem_base;
+
+    if ((!PLAIN && warp == 0u && lane == 0u) || (PLAIN && warp >= 8u)) {
+        uint32_t issued = 0;
+        bool ok = true;
+        for (uint32_t ks = ks0; ks < ks1; ++ks, ++issued) {
+            const uint32_t stage = issued % kStages;
+            if (!tma::wait(&empty[stage], (issued / kStages + 1u) & 1u)) {
+                ok = false;
+                break;
+            }
+            unsigned char* sa = smem + stage * kStageBytes;
+            unsigned char* sb = sa + kStageBytesA;
+            const uint32_t k0 = ks * kBK;
+            if (PLAIN) {
+                const uint32_t tid = threadIdx.x - 256u;
+                if (g.a_mn) {
+                    for (uint32_t j = 0; j < kBM / 64u; ++j) fill_box<kBK>(sa + j * 8192u, g.a, k0, m0 + 64u * j, tid);
+                } else {
+                    fill_box<kBM>(sa, g.a, m0, k0, tid);
+                }
+                fill_box<BN>(sb, g.b, n0, k0, tid);
+                umma::fence_async_smem();
+                tma::arrive(&full[stage]);
+            } else {
+                tma::expect_tx(&full[stage], kStageBytes);
+                if (g.a_mn) {
+                    for (uint32_t j = 0; j < kBM / 64u; ++j) tma::load_2d(smem_u32(sa + j * 8192u), &maps.a, m0 + 64u * j, k0, &full[stage]);
+                } else {
+                    tma::load_2d(smem_u32(sa), &maps.a, k0, m0, &full[stage]);
+                }
+                tma::load_2d(smem_u32(sb), &maps.b, k0, n0, &full[stage]);
+            }
+        }
+        if (!ok) {
+            atomicOr(g.error, 1u);
+            if (!PLAIN)
+                for (uint32_t i = issued > kStages ? issued - kStages : 0u; i < issued; ++i) tma::wait(&full[i % kStages], (i / kStages) & 1u);
+        }
+    } else if (warp == 1u && lane == 0u) {
+        const uint32_t idesc = tma::idesc_16bit(kBM, BN, g.a_mn, 0u, g.bf16);
+        bool ok = true;
+        for (uint32_t ks = ks0; ks < ks1; ++ks) {
+            const uint32_t i = ks - ks0, stage = i % kStages;
+            if (!tma::wait(&full[stage], (i / kStages) & 1u)) {
+                ok = false;
+                break;
+            }
+            umma::fence_after_sync();
+            const uint32_t sa = smem_u32(smem + stage * kStageBytes), sb = sa + kStageBytesA;
+#pragma unroll
+            for (uint32_t k = 0; k < kBK / 16u; ++k) {
+                const uint64_t da = g.a_mn ? tma::desc_sw128(sa + 2048u * k, 8192u, 1024u) : tma::desc_sw128(sa + 32u * k, 16u, 1024u);
+                umma::mma_f16(tmem, da, tma::desc_sw128(sb + 32u * k, 16u, 1024u), idesc, (i > 0u || k > 0u) ? 1u : 0u);
+            }
+            umma::commit(&empty[stage]);
+        }
+        if (ok) {
+            umma::commit(&acc_full);
+        } else {
+            atomicOr(g.error, 1u);
+            umma::commit(&drain);
+            tma::wait(&drain, 0u);
+        }
+    }
+    __syncwarp();
+    // What the output needs beside the sums, on its way while they are made:
+    // thread t of rank r takes values r 256 + t, + splits 256, ... of the tile
+    // ([BN][128]), so always the same weight row.
+    const uint32_t t = threadIdx.x & 255u, m = m0 + (t & 127u);
+    const bool mine = threadIdx.x < 256u && m < g.M;
+    const float bias = mine && g.bias ? from_16(static_cast<const uint16_t*>(g.bias)[m], bf16) : 0.0f;
+    const uint32_t rows = min(BN, g.N - n0);
+    float* part = reinterpret_cast<float*>(smem);
+    if (warp >= 4u && warp < 8u) {
+        bool ok = tma::wait(&acc_full, 0u);
+        if (!ok) {
+            atomicOr(g.error, 1u);
+            failed = 1u;
+        }
+        ok = __all_sync(0xffffffffu, ok);
+        umma::fence_after_sync();
+        if (ok) {
+            const uint32_t q = warp & 3u;
+            for (uint32_t c0 = 0; c0 < rows; c0 += 16u) {
+                float v[16];
+                umma::tmem_ld16(tmem + c0 + ((32u * q) << 16), v);
+#pragma unroll
+                for (uint32_t i = 0; i < 16u; ++i) part[(c0 + i) * kBM + 32u * q + lane] = v[i];
+            }
+        }
+        umma::fence_before_sync();
+    }
+    __syncthreads();
+    if (g.splits > 1u) tma::cluster_sync();
+    if (mine && failed == 0u) {
+        const uint32_t part_at = smem_u32(part);
+        for (uint32_t i = rank * 256u + t; i < rows * kBM; i += g.splits * 256u) {
+            const uint64_t j = n0 + (i >> 7);
+            float z = 0.0f, r = 0.0f;
+            if (g.res.ptr) r = from_16(static_cast<const uint16_t*>(g.res.ptr)[j * g.res.ld + m], bf16);
+            if (g.splits == 1u) {
+                z = part[i];
+            } else {
+                float p[kColsMaxCluster];
+#pragma unroll
+                for (uint32_t c = 0; c < kColsMaxCluster; ++c) p[c] = c < g.splits ? tma::peer_f32(part_at + 4u * i, c) : 0.0f;
+#pragma unroll
+                for (uint32_t c = 0; c < kColsMaxCluster; ++c) z += p[c];
+            }
+            z += bias;
+            if (g.pre.ptr) static_cast<uint16_t*>(const_cast<void*>(g.pre.ptr))[j * g.pre.ld + m] = to_16(z, bf16);
+            float v[1] = {z};
+            act_row(v, g.act);
+            static_cast<uint16_t*>(const_cast<void*>(g.y.ptr))[j * g.y.ld + m] = to_16(v[0] + r, bf16);
+        }
+    }
+    umma::fence_before_sync();
+    __syncthreads();
+    if (g.splits > 1u) tma::cluster_sync();  // no CTA leaves while another reads its sums
+    if (warp == 2u) umma::tmem_dealloc(tmem, kCols);
+}
+
+template <uint32_t BN, bool PLAIN>
+cudaError_t launch_cols_t(const GemmArgs& g, const GemmMaps& maps, cudaStream_t s) {
+    using S = ColsShape<BN, PLAIN>;
+    static std::atomic<bool> done[64];
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+    if (!done[dev]) {
+        e = cudaFuncSetAttribute(k_gemm_cols<BN, PLAIN>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
+        if (e != cudaSuccess) return e;
+        done[dev] = true;
+    }
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(g.tiles_m * g.tiles_n * g.splits);
+    cfg.blockDim = dim3(S::kThreads);
+    cfg.dynamicSmemBytes = S::kSmem;
+    cfg.stream = s;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = g.splits;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1u;
+    cfg.attrs = at;
+    cfg.numAttrs = g.splits > 1u ? 1u : 0u;
+    return cudaLaunchKernelEx(&cfg, k_gemm_cols<BN, PLAIN>, g, maps);
+}
+
 // ------------------------------------------------- dz and its column sums
 // 256 threads: 8 columns a thread, `cg` column groups side by side (a power of
 // two up to 32), 256 / cg rows at a time.
@@ -932,6 +1131,17 @@ cudaError_t launch_gemm_kind(const GemmArgs& g, uint32_t bn, int feed, const Gem
 cudaError_t launch_gemm(const GemmArgs& g, int kind, uint32_t bn, int feed, const GemmMaps& maps, uint32_t blocks, cudaStream_t s) {
     return kind == kGemmRows ? launch_gemm_kind<kGemmRows>(g, bn, feed, maps, blocks, s)
                              : launch_gemm_kind<kGemmGrad>(g, bn, feed, maps, blocks, s);
+}
+
+cudaError_t launch_gemm_cols(const GemmArgs& g, uint32_t bn, bool plain_loads, const GemmMaps& maps, cudaStream_t s) {
+    if (g.splits == 0u || g.splits > kColsMaxCluster || g.b_mn) return cudaErrorInvalidValue;
+    switch (bn) {
+        case 16u: return plain_loads ? launch_cols_t<16u, true>(g, maps, s) : launch_cols_t<16u, false>(g, maps, s);
+        case 32u: return plain_loads ? launch_cols_t<32u, true>(g, maps, s) : launch_cols_t<32u, false>(g, maps, s);
+        case 64u: return plain_loads ? launch_cols_t<64u, true>(g, maps, s) : launch_cols_t<64u, false>(g, maps, s);
+        case 128u: return plain_loads ? launch_cols_t<128u, true>(g, maps, s) : launch_cols_t<128u, false>(g, maps, s);
+        default: return cudaErrorInvalidValue;
+    }
 }
 
 cudaError_t launch_dz(const DzArgs& a, cudaStream_t s) {

@@ -55,6 +55,11 @@ enum GemmFeed : int { kFeedTma = 0, kFeedPair = 1, kFeedPlain = 2 };
 constexpr uint32_t kGemmPairBN = 256;
 
 cudaError_t launch_gemm(const GemmArgs& g, int kind, uint32_t bn, int feed, const GemmMaps& maps, uint32_t blocks, cudaStream_t s);
+// Few rows: D^T[n][m], the weight's rows along the tensor core's 128, the
+// activations' rows along its columns, K split over a cluster of CTAs.  In the
+// arguments A is the weight and M its rows; y, res and pre are [N][M].
+constexpr uint32_t kColsMaxCluster = 8;
+cudaError_t launch_gemm_cols(const GemmArgs& g, uint32_t bn, bool plain_loads, const GemmMaps& maps, cudaStream_t s);
 // dz = dy act'(pre) (16-bit, rows dz_ld apart; null: not written), and the
 // column sums of dz before rounding over each of `parts` row ranges
 // ([parts][cols] fp32; null: none).

@@ -207,9 +207,41 @@ cudaError_t run_gemm(GemmArgs& g, int kind, uint32_t bn, bool pair, uint32_t sms
     const uint32_t blocks = static_cast<uint32_t>(items < slots ? items : slots) * (pair ? 2u : 1u);
     return launch_gemm(g, kind, bn, plain ? kFeedPlain : pair ? kFeedPair : kFeedTma, maps, blocks, s);
 }
-// y = act(a b^T + bias) + res: fills in the tiles and runs the product.
+// Few rows (run_cols) or tiles of 128 (run_rows)?  The first where every row
+// fits one column tile, or where the 128-row tiles would leave half of the SMs
+// without work and K is long enough to be split.
+bool cols_pay(uint64_t m, uint64_t n, uint64_t k, uint32_t sms) {
+    return m <= 128u || (k >= 512u && static_cast<uint64_t>(ceil_div(m, 128u)) * ceil_div(n, 64u) <= sms / 2u);
+}
+cudaError_t run_cols(const GemmArgs& rows, cudaStream_t s, uint32_t sms) {
+    GemmArgs g = rows;  // the weight as A, the activations as B
+    g.a = rows.b;
+    g.b = rows.a;
+    g.a_mn = rows.b_mn;
+    g.b_mn = 0u;
+    g.M = rows.N;
+    g.N = rows.M;
+    const uint32_t bn = g.N <= 16u ? 16u : g.N <= 32u ? 32u : g.N <= 64u ? 64u : 128u;
+    g.tiles_m = ceil_div(g.M, kGemmBM);
+    g.tiles_n = ceil_div(g.N, bn);
+    g.k_steps = ceil_div(g.K, kGemmBK);
+    // As many parts of K as fill the SMs once, each at least two steps.
+    const uint64_t tiles = static_cast<uint64_t>(g.tiles_m) * g.tiles_n;
+    uint64_t splits = tiles >= sms ? 1u : sms / tiles;
+    if (splits > kColsMaxCluster) splits = kColsMaxCluster;
+    if (splits > ceil_div(g.k_steps, 2u)) splits = ceil_div(g.k_steps, 2u);
+    g.steps_per_split = ceil_div(g.k_steps, splits);
+    g.splits = ceil_div(g.k_steps, g.steps_per_split);
+    GemmMaps maps{};
+    const bool plain = g.a.vec < 8u || g.b.vec < 8u, bf16 = g.bf16 != 0u;
+    if (!plain && (!make_map(&maps.a, g.a, g.a_mn ? kGemmBK : kGemmBM, bf16) || !make_map(&maps.b, g.b, bn, bf16)))
+        return cudaErrorNotSupported;
+    return launch_gemm_cols(g, bn, plain, maps, s);
+}
+// y = act(a b^T + bias) + res: picks the kernel, fills in the tiles and runs it.
 cudaError_t run_rows(GemmArgs& g, uint32_t sms, cudaStream_t s) {
     const bool pair = g.a.vec >= 8u && g.b.vec >= 8u && pair_pays(g.M, g.N, g.K, sms);
+    if (!pair && cols_pay(g.M, g.N, g.K, sms)) return run_cols(g, s, sms);
     g.tiles_m = ceil_div(g.M, pair ? 2u * kGemmBM : kGemmBM);
     const uint32_t bn = pair ? kGemmPairBN : pick_bn(g.tiles_m, g.N, sms);
     g.tiles_n = ceil_div(g.N, bn);
