@@ -157,24 +157,40 @@ template <int ES, bool kStore>
 NB_DEV void slab_copy(unsigned char* slab, unsigned char* g, uint64_t ld, uint32_t rows, uint32_t cols, bool vec, uint32_t lane) {
     constexpr uint32_t kPer = 16u / ES;
     if (vec) {
-        const uint32_t p = lane & 7u;
+        const uint32_t p = lane & 7u, r0 = lane >> 3;
+        if (rows == 32u && cols * ES == 128u) {  // whole: eight pieces a lane in flight
+            unsigned char* q = g + (r0 * ld + p * kPer) * ES;
+            const uint64_t step = 4u * ld * ES;
+            uint4 u[8];
+            if (kStore) {
 #pragma unroll
-        for (uint32_t i = 0; i < 8u; ++i) {
-            const uint32_t r = (lane >> 3) + 4u * i;
-            if (r >= rows || p * kPer >= cols) continue;
+                for (uint32_t i = 0; i < 8u; ++i) u[i] = *reinterpret_cast<const uint4*>(slab + slab_at(r0 + 4u * i, p));
+#pragma unroll
+                for (uint32_t i = 0; i < 8u; ++i) *reinterpret_cast<uint4*>(q + i * step) = u[i];
+            } else {
+#pragma unroll
+                for (uint32_t i = 0; i < 8u; ++i) u[i] = *reinterpret_cast<const uint4*>(q + i * step);
+#pragma unroll
+                for (uint32_t i = 0; i < 8u; ++i) *reinterpret_cast<uint4*>(slab + slab_at(r0 + 4u * i, p)) = u[i];
+            }
+            return;
+        }
+#pragma unroll 1
+        for (uint32_t r = r0; r < rows; r += 4u) {
             unsigned char* q = g + (r * ld + p * kPer) * ES;
             unsigned char* l = slab + slab_at(r, p);
             if ((p + 1u) * kPer <= cols) {
                 if (kStore) *reinterpret_cast<uint4*>(q) = *reinterpret_cast<const uint4*>(l);
                 else *reinterpret_cast<uint4*>(l) = *reinterpret_cast<const uint4*>(q);
             } else {
-                for (uint32_t e = 0; e < cols - p * kPer; ++e) {
+                for (uint32_t e = p * kPer; e < cols; ++e) {
+                    const uint32_t o = (e - p * kPer) * ES;
                     if (ES == 2) {
-                        if (kStore) reinterpret_cast<uint16_t*>(q)[e] = reinterpret_cast<const uint16_t*>(l)[e];
-                        else reinterpret_cast<uint16_t*>(l)[e] = reinterpret_cast<const uint16_t*>(q)[e];
+                        if (kStore) *reinterpret_cast<uint16_t*>(q + o) = *reinterpret_cast<const uint16_t*>(l + o);
+                        else *reinterpret_cast<uint16_t*>(l + o) = *reinterpret_cast<const uint16_t*>(q + o);
                     } else {
-                        if (kStore) reinterpret_cast<uint32_t*>(q)[e] = reinterpret_cast<const uint32_t*>(l)[e];
-                        else reinterpret_cast<uint32_t*>(l)[e] = reinterpret_cast<const uint32_t*>(q)[e];
+                        if (kStore) *reinterpret_cast<uint32_t*>(q + o) = *reinterpret_cast<const uint32_t*>(l + o);
+                        else *reinterpret_cast<uint32_t*>(l + o) = *reinterpret_cast<const uint32_t*>(q + o);
                     }
                 }
             }
@@ -296,6 +312,7 @@ NB_DEV void fill_box(unsigned char* box, const MatrixView& m, uint32_t row0, uin
 struct Barriers {
     uint64_t full[kMaxStages], empty[kMaxStages];
     uint64_t acc_full[2], acc_empty[2];
+    uint64_t res[8];  // an epilogue warp's residual rows have arrived
     uint64_t drain;
     uint32_t tmem_base;
 };
@@ -358,8 +375,8 @@ struct GemmShape {
     static constexpr bool kPair = FEED == kFeedPair, kPlain = FEED == kFeedPlain;
     static constexpr uint32_t kBoxN = kPair ? BN / 2u : BN;  // rows of B in this CTA's shared memory
     static constexpr uint32_t kStageBytes = kStageBytesA + kBoxN * 128u;
-    static constexpr uint32_t kStages = kPlain ? 2u : kPair ? 5u : BN >= 256u ? 4u : BN >= 128u ? 4u : 5u;
-    static constexpr uint32_t kSlabs = kPlain ? 1u : kPair ? 2u : BN >= 256u ? 1u : 2u;  // per epilogue warp
+    static constexpr uint32_t kStages = kPlain ? 2u : kPair ? 5u : BN >= 256u ? 3u : BN >= 128u ? 4u : 5u;
+    static constexpr uint32_t kSlabs = kPlain ? 1u : 2u;  // per epilogue warp
     static constexpr uint32_t kSmem = 1024u + kStages * kStageBytes + 8u * kSlabs * kSlabBytes + 2u * BN * 2u;
     static constexpr uint32_t kThreads = kPlain ? 384u + 32u * kLoadWarps : 384u;
     // Weight gradients of 256 columns keep 128 sums a thread: registers move
@@ -398,6 +415,7 @@ __global__ void __launch_bounds__(GemmShape<BN, KIND, FEED>::kThreads, 1) k_gemm
             umma::mbar_init(&bar.acc_full[i], 1u);
             umma::mbar_init(&bar.acc_empty[i], (KIND == kGemmGrad ? 8u : 4u) * kCtas);
         }
+        for (uint32_t i = 0; i < 8u; ++i) umma::mbar_init(&bar.res[i], 1u);
         umma::mbar_init(&bar.drain, 1u);
         umma::fence_mbar_init();
         if (!S::kPlain) {
@@ -642,7 +660,7 @@ __global__ void __launch_bounds__(GemmShape<BN, KIND, FEED>::kThreads, 1) k_gemm
         uint16_t* bias_s = bias_all + acc * BN;
         const uint32_t taddr = tmem + acc * BN + ((32u * q) << 16);
         const uint32_t acc_empty = S::kPair ? tma::peer_addr(smem_u32(&bar.acc_empty[acc]), 0u) : 0u;
-        uint32_t parity = 0, slab_i = 0, bias_n = ~0u;
+        uint32_t parity = 0, res_parity = 0, slab_i = 0, bias_n = ~0u;
         bool ok = true;  // after a wait that ran out the warp only keeps the named barriers' count
         // A slab that no store of this warp still reads.
         const auto next_slab = [&]() -> unsigned char* {
@@ -687,18 +705,34 @@ __global__ void __launch_bounds__(GemmShape<BN, KIND, FEED>::kThreads, 1) k_gemm
             {
                 for (uint32_t c0 = 0; c0 < BN && n0 + c0 < g.N; c0 += 64u) {
                     const uint32_t cols = min(64u, g.N - n0 - c0);
+                    // The residual's rows come straight into the slab of the output, where this thread's
+                    // row replaces them; the copy runs while z is made.
+                    unsigned char* slab = nullptr;
+                    if (S::kSlabs > 1u || !g.pre.ptr) {
+                        slab = next_slab();
+                        if (g.res_tma && rows && lane == 0u) {
+                            tma::expect_tx(&bar.res[warp - 4u], kSlabBytes);
+                            tma::load_2d(smem_u32(slab), &maps.res, static_cast<int32_t>(n0 + c0), static_cast<int32_t>(m0), &bar.res[warp - 4u]);
+                        }
+                    }
                     if (g.pre.ptr) {
-                        unsigned char* slab = next_slab();
+                        unsigned char* slab_z = next_slab();
 #pragma unroll
                         for (uint32_t h = 0; h < 2u; ++h) {
                             float v[32];
                             load_z(v, taddr + c0 + 32u * h, bias_s + c0 + 32u * h, bf16);
-                            slab_put32(slab, lane, h, v, bf16);
+                            slab_put32(slab_z, lane, h, v, bf16);
                         }
-                        slab_out(slab, g.pre, g.pre_tma != 0u, &maps.pre, m0, n0 + c0, rows, cols, lane);
+                        slab_out(slab_z, g.pre, g.pre_tma != 0u, &maps.pre, m0, n0 + c0, rows, cols, lane);
+                        if (S::kSlabs == 1u) {
+                            slab = next_slab();
+                            if (g.res_tma && rows && lane == 0u) {
+                                tma::expect_tx(&bar.res[warp - 4u], kSlabBytes);
+                                tma::load_2d(smem_u32(slab), &maps.res, static_cast<int32_t>(n0 + c0), static_cast<int32_t>(m0), &bar.res[warp - 4u]);
+                            }
+                        }
                     }
-                    unsigned char* slab = next_slab();
-                    if (g.res.ptr) {
+                    if (g.res.ptr && !g.res_tma) {
                         unsigned char* src = static_cast<unsigned char*>(const_cast<void*>(g.res.ptr)) + 2u * (m0 * g.res.ld + n0 + c0);
                         slab_copy<2, false>(slab, src, g.res.ld, rows, cols, g.res.vec >= 8u, lane);
                         __syncwarp();
@@ -708,6 +742,11 @@ __global__ void __launch_bounds__(GemmShape<BN, KIND, FEED>::kThreads, 1) k_gemm
                         float v[32];
                         load_z(v, taddr + c0 + 32u * h, bias_s + c0 + 32u * h, bf16);
                         act_row(v, g.act);
+                        if (h == 0u && g.res_tma && rows) {
+                            if (!tma::wait(&bar.res[warp - 4u], res_parity)) atomicOr(g.error, 1u);
+                            res_parity ^= 1u;
+                            __syncwarp();
+                        }
                         if (g.res.ptr) {
 #pragma unroll
                             for (uint32_t p = 0; p < 4u; ++p) {
