@@ -139,6 +139,33 @@ NB_DEV void red_add_f16x2(void* gptr, uint32_t v) {
 }
 
 // ---------------------------------------------------------------------------
+// Programmatic dependent launch: a kernel launched with launch_after() may
+// start while the one before it in the stream still runs.  after_previous()
+// waits until that one has ended and its writes are visible (every thread
+// calls it before it touches global memory); let_next_start() lets the next
+// kernel's blocks take their places as soon as every block of this one runs.
+// ---------------------------------------------------------------------------
+NB_DEV void after_previous() { asm volatile("griddepcontrol.wait;\n" ::: "memory"); }
+NB_DEV void let_next_start() { asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory"); }
+template <typename Kernel, typename... Args>
+cudaError_t launch_after(Kernel kernel, dim3 grid, uint32_t threads, uint32_t smem, uint32_t cluster, cudaStream_t s, const Args&... args) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute at[2];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim.x = cluster;
+    at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1u;
+    cfg.attrs = at;
+    cfg.numAttrs = cluster > 1u ? 2u : 1u;
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
+// ---------------------------------------------------------------------------
 // Reductions
 // ---------------------------------------------------------------------------
 NB_DEV float warp_sum(float v) {

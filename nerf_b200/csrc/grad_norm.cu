@@ -17,15 +17,17 @@
 #include <new>
 
 #include "../../include/nerf_b200.h"
-#include "common.cuh"
+#include "tma.cuh"
 
 namespace nb {
 namespace {
 
 constexpr uint32_t kChunk = 8192;
 constexpr uint32_t kThreads = 256;
+constexpr uint32_t kFlight = 4;        // 16-byte loads in flight a thread
 constexpr uint32_t kMaxBlocks = 1024;  // partial sums of one launch
 constexpr uint32_t kTable = 512;       // tensors of one launch
+constexpr uint32_t kSmallBlocks = 8, kSmallChunks = 32;
 
 struct GradEntry {
     const void* g;
@@ -80,48 +82,49 @@ struct Vec {
     }
 };
 
-// Squares of fp32 and bf16 values leave the range of fp32 sums at both ends: a
-// batch whose sum does not lie well inside it is added again in fp64 (fp16
-// squares never leave it).
+// Adds the squares of N values.  Most batches are finite and well inside the
+// range of fp32 sums, which the sum itself shows; the others are looked at
+// value by value: infinities and NaN are left out and reported, and fp32 and
+// bf16 squares that fp32 cannot hold are added in fp64 (fp16 squares always
+// fit).
 template <uint32_t TYPE, uint32_t N>
 NB_DEV void add_squares(const float* v, double& sum, uint32_t& bad) {
     float s = 0.0f;
 #pragma unroll
-    for (uint32_t i = 0; i < N; ++i) {
-        const bool fine = isfinite(v[i]);
-        bad |= fine ? 0u : 1u;
-        const float x = fine ? v[i] : 0.0f;
-        s = fmaf(x, x, s);
-    }
-    if (TYPE != NERF_B200_F16 && !(s >= 1e-25f && s <= 1e37f)) {
-#pragma unroll
-        for (uint32_t i = 0; i < N; ++i)
-            if (isfinite(v[i]) && v[i] != 0.0f) sum += static_cast<double>(v[i]) * v[i];
+    for (uint32_t i = 0; i < N; ++i) s = fmaf(v[i], v[i], s);
+    if (TYPE == NERF_B200_F16 ? s < INFINITY : s >= 1e-25f && s <= 1e37f) {
+        sum += s;
         return;
     }
-    sum += s;
+#pragma unroll
+    for (uint32_t i = 0; i < N; ++i) {
+        if (!isfinite(v[i])) bad = 1u;
+        else if (v[i] != 0.0f) sum += static_cast<double>(v[i]) * v[i];
+    }
 }
 
 template <uint32_t TYPE>
 NB_DEV void chunk_squares(const GradEntry& e, uint64_t e0, uint64_t e1, double& sum, uint32_t& bad) {
     constexpr uint32_t V = Vec<TYPE>::kN, B = Vec<TYPE>::kBytes;
     const uint64_t addr = reinterpret_cast<uint64_t>(e.g) + e0 * B;
-    const uint64_t head = min(e1 - e0, static_cast<uint64_t>(((16u - (addr & 15u)) & 15u) / B));
-    const uint64_t n_vec = (e1 - e0 - head) / V, tail0 = e0 + head + n_vec * V;
+    const uint32_t n = static_cast<uint32_t>(e1 - e0), head = min(n, ((16u - (static_cast<uint32_t>(addr) & 15u)) & 15u) / B);
+    const uint32_t n_vec = (n - head) / V, tail0 = head + n_vec * V, t = threadIdx.x;
     const uint4* q = reinterpret_cast<const uint4*>(addr + head * B);
-    const uint32_t t = threadIdx.x;
-    for (uint64_t i = t; i < n_vec; i += 4u * kThreads) {
-        uint4 u[4];
+    for (uint32_t i = t; i < n_vec; i += kFlight * kThreads) {
+        uint4 u[kFlight];
 #pragma unroll
-        for (uint32_t j = 0; j < 4u; ++j) u[j] = i + j * kThreads < n_vec ? __ldg(q + i + j * kThreads) : make_uint4(0u, 0u, 0u, 0u);
-        float v[4u * V];
+        for (uint32_t j = 0; j < kFlight; ++j) u[j] = i + j * kThreads < n_vec ? q[i + j * kThreads] : make_uint4(0u, 0u, 0u, 0u);
 #pragma unroll
-        for (uint32_t j = 0; j < 4u; ++j) Vec<TYPE>::unpack(u[j], v + j * V);
-        add_squares<TYPE, 4u * V>(v, sum, bad);
+        for (uint32_t j = 0; j < kFlight; j += 2u) {
+            float v[2u * V];
+            Vec<TYPE>::unpack(u[j], v);
+            Vec<TYPE>::unpack(u[j + 1u], v + V);
+            add_squares<TYPE, 2u * V>(v, sum, bad);
+        }
     }
-    const uint64_t rest = head + (e1 - tail0);  // fewer than 2 V values at the two ends
+    const uint32_t rest = head + (n - tail0);  // fewer than 2 V values at the two ends
     if (t < rest) {
-        const float v = Vec<TYPE>::one(e.g, t < head ? e0 + t : tail0 + (t - head));
+        const float v = Vec<TYPE>::one(e.g, e0 + (t < head ? t : tail0 + (t - head)));
         add_squares<TYPE, 1u>(&v, sum, bad);
     }
 }
@@ -143,6 +146,26 @@ NB_DEV double warp_sum_f64(double v) {
     return v;
 }
 
+// A chunk's squares into the thread's sum.
+NB_DEV void squares_of(const GradEntry& e, uint32_t chunk, double& sum, uint32_t& bad) {
+    const uint64_t e0 = static_cast<uint64_t>(chunk - e.chunk0) * kChunk, e1 = min(e.count, e0 + kChunk);
+    switch (e.type) {
+        case NERF_B200_F32: chunk_squares<NERF_B200_F32>(e, e0, e1, sum, bad); break;
+        case NERF_B200_F16: chunk_squares<NERF_B200_F16>(e, e0, e1, sum, bad); break;
+        default: chunk_squares<NERF_B200_BF16>(e, e0, e1, sum, bad); break;
+    }
+}
+// The threads' sums, in thread 0, and (in every thread) whether any is bad.
+NB_DEV bool block_sum(double& sum, uint32_t bad) {
+    __shared__ double ws[kThreads / 32u];
+    sum = warp_sum_f64(sum);
+    if ((threadIdx.x & 31u) == 0u) ws[threadIdx.x >> 5] = sum;
+    const int any = __syncthreads_or(static_cast<int>(bad));
+#pragma unroll
+    for (uint32_t w = 1; w < kThreads / 32u; ++w) sum += ws[w];
+    return any != 0;
+}
+
 template <uint32_t CAP>
 __global__ void __launch_bounds__(kThreads) k_grad_squares(const __grid_constant__ GradTable<CAP> t, GradPartial* out) {
     const uint32_t c0 = static_cast<uint32_t>(static_cast<uint64_t>(t.chunks) * blockIdx.x / t.blocks);
@@ -150,27 +173,25 @@ __global__ void __launch_bounds__(kThreads) k_grad_squares(const __grid_constant
     double sum = 0.0;
     uint32_t bad = 0u;
     uint32_t k = c0 < c1 ? entry_of(t, c0) : 0u;
+    after_previous();
+    let_next_start();
     for (uint32_t c = c0; c < c1; ++c) {
         while (k + 1u < t.n && t.e[k + 1u].chunk0 <= c) ++k;
-        const GradEntry& e = t.e[k];
-        const uint64_t e0 = static_cast<uint64_t>(c - e.chunk0) * kChunk, e1 = min(e.count, e0 + kChunk);
-        switch (e.type) {
-            case NERF_B200_F32: chunk_squares<NERF_B200_F32>(e, e0, e1, sum, bad); break;
-            case NERF_B200_F16: chunk_squares<NERF_B200_F16>(e, e0, e1, sum, bad); break;
-            default: chunk_squares<NERF_B200_BF16>(e, e0, e1, sum, bad); break;
-        }
+        squares_of(t.e[k], c, sum, bad);
     }
-    __shared__ double ws[kThreads / 32u];
-    sum = warp_sum_f64(sum);
-    if ((threadIdx.x & 31u) == 0u) ws[threadIdx.x >> 5] = sum;
-    const int any = __syncthreads_or(static_cast<int>(bad));
-    if (threadIdx.x == 0u) {
-#pragma unroll
-        for (uint32_t w = 1; w < kThreads / 32u; ++w) sum += ws[w];
-        out[blockIdx.x] = GradPartial{sum, any ? 1u : 0u, 0u};
-    }
+    const bool any = block_sum(sum, bad);
+    if (threadIdx.x == 0u) out[blockIdx.x] = GradPartial{sum, any ? 1u : 0u, 0u};
 }
 
+NB_DEV GradInfo make_info(double sum, bool bad, float loss_scale, float max_norm) {
+    const double norm = sqrt(sum) / static_cast<double>(loss_scale);
+    GradInfo r;
+    r.norm = static_cast<float>(norm);
+    r.nonfinite = bad ? 1u : 0u;
+    r.scale = !bad && norm > static_cast<double>(max_norm) ? static_cast<float>(static_cast<double>(max_norm) / norm) : 1.0f;
+    r.reserved = 0u;
+    return r;
+}
 // The norm from the partial sums, the same in every block that asks.
 NB_DEV GradInfo grad_info(const GradPartial* __restrict__ p, uint32_t n, float loss_scale, float max_norm) {
     __shared__ double ws[kThreads / 32u];
@@ -186,16 +207,12 @@ NB_DEV GradInfo grad_info(const GradPartial* __restrict__ p, uint32_t n, float l
     sum = ws[0];
 #pragma unroll
     for (uint32_t w = 1; w < kThreads / 32u; ++w) sum += ws[w];
-    const double norm = sqrt(sum) / static_cast<double>(loss_scale);
-    GradInfo r;
-    r.norm = static_cast<float>(norm);
-    r.nonfinite = any ? 1u : 0u;
-    r.scale = !any && norm > static_cast<double>(max_norm) ? static_cast<float>(static_cast<double>(max_norm) / norm) : 1.0f;
-    r.reserved = 0u;
-    return r;
+    return make_info(sum, any != 0, loss_scale, max_norm);
 }
 
 __global__ void __launch_bounds__(kThreads) k_grad_finish(const GradPartial* p, uint32_t n, float loss_scale, GradInfo* info) {
+    after_previous();
+    let_next_start();
     const GradInfo r = grad_info(p, n, loss_scale, INFINITY);
     if (threadIdx.x == 0u) *info = r;
 }
@@ -210,19 +227,19 @@ template <uint32_t TYPE, uint32_t OUT>
 NB_DEV void chunk_scale(const GradEntry& e, uint64_t e0, uint64_t e1, float scale) {
     constexpr uint32_t V = Vec<TYPE>::kN, B = Vec<TYPE>::kBytes, OB = OUT == NERF_B200_F32 ? 4u : 2u;
     const uint64_t addr = reinterpret_cast<uint64_t>(e.g) + e0 * B;
-    const uint64_t head = min(e1 - e0, static_cast<uint64_t>(((16u - (addr & 15u)) & 15u) / B));
-    const uint64_t n_vec = (e1 - e0 - head) / V, tail0 = e0 + head + n_vec * V;
+    const uint32_t n = static_cast<uint32_t>(e1 - e0), head = min(n, ((16u - (static_cast<uint32_t>(addr) & 15u)) & 15u) / B);
+    const uint32_t n_vec = (n - head) / V, tail0 = head + n_vec * V;
     const uint4* q = reinterpret_cast<const uint4*>(addr + head * B);
     unsigned char* o = static_cast<unsigned char*>(e.out) + (e0 + head) * OB;
     const bool wide = (reinterpret_cast<uint64_t>(o) & 15u) == 0u;
     const uint32_t t = threadIdx.x;
-    for (uint64_t i = t; i < n_vec; i += 4u * kThreads) {
-        uint4 u[4];
+    for (uint32_t i = t; i < n_vec; i += kFlight * kThreads) {
+        uint4 u[kFlight];
 #pragma unroll
-        for (uint32_t j = 0; j < 4u; ++j) u[j] = i + j * kThreads < n_vec ? q[i + j * kThreads] : make_uint4(0u, 0u, 0u, 0u);
+        for (uint32_t j = 0; j < kFlight; ++j) u[j] = i + j * kThreads < n_vec ? __ldcs(q + i + j * kThreads) : make_uint4(0u, 0u, 0u, 0u);
 #pragma unroll
-        for (uint32_t j = 0; j < 4u; ++j) {
-            const uint64_t at = i + j * kThreads;
+        for (uint32_t j = 0; j < kFlight; ++j) {
+            const uint32_t at = i + j * kThreads;
             if (at >= n_vec) break;
             float v[V];
             Vec<TYPE>::unpack(u[j], v);
@@ -234,43 +251,80 @@ NB_DEV void chunk_scale(const GradEntry& e, uint64_t e0, uint64_t e1, float scal
             } else if (OUT == NERF_B200_F32) {
                 float4* d = reinterpret_cast<float4*>(o) + at * (V / 4u);
 #pragma unroll
-                for (uint32_t k = 0; k < V / 4u; ++k) d[k] = make_float4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]);
+                for (uint32_t k = 0; k < V / 4u; ++k) __stcs(d + k, make_float4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]));
             } else if (V == 8u) {
                 uint32_t w[4];
 #pragma unroll
                 for (int k = 0; k < 4; ++k)
                     w[k] = OUT == NERF_B200_F16 ? pack_h2(v[(2 * k) % V], v[(2 * k + 1) % V]) : pack_bf(v[(2 * k) % V], v[(2 * k + 1) % V]);
-                reinterpret_cast<uint4*>(o)[at] = make_uint4(w[0], w[1], w[2], w[3]);
+                __stcs(reinterpret_cast<uint4*>(o) + at, make_uint4(w[0], w[1], w[2], w[3]));
             }
         }
     }
-    const uint64_t rest = head + (e1 - tail0);
+    const uint32_t rest = head + (n - tail0);
     if (t < rest) {
-        const uint64_t i = t < head ? e0 + t : tail0 + (t - head);
+        const uint64_t i = e0 + (t < head ? t : tail0 + (t - head));
         store_one<OUT>(e.out, i, Vec<TYPE>::one(e.g, i) * scale);
     }
 }
 
+NB_DEV void scale_of(const GradEntry& e, uint32_t chunk, float scale) {
+    if (scale == 1.0f && e.out == e.g) return;  // in place and nothing to clip
+    const uint64_t e0 = static_cast<uint64_t>(chunk - e.chunk0) * kChunk, e1 = min(e.count, e0 + kChunk);
+    switch (e.type * 4u + e.out_type) {
+        case NERF_B200_F32 * 4u + NERF_B200_F32: chunk_scale<NERF_B200_F32, NERF_B200_F32>(e, e0, e1, scale); break;
+        case NERF_B200_F16 * 4u + NERF_B200_F16: chunk_scale<NERF_B200_F16, NERF_B200_F16>(e, e0, e1, scale); break;
+        case NERF_B200_F16 * 4u + NERF_B200_F32: chunk_scale<NERF_B200_F16, NERF_B200_F32>(e, e0, e1, scale); break;
+        case NERF_B200_BF16 * 4u + NERF_B200_BF16: chunk_scale<NERF_B200_BF16, NERF_B200_BF16>(e, e0, e1, scale); break;
+        default: chunk_scale<NERF_B200_BF16, NERF_B200_F32>(e, e0, e1, scale); break;
+    }
+}
 template <uint32_t CAP>
 __global__ void __launch_bounds__(kThreads)
     k_grad_scale(const __grid_constant__ GradTable<CAP> t, const GradPartial* p, uint32_t n_partials, float loss_scale, float max_norm,
                  GradInfo* info) {
+    after_previous();
+    let_next_start();
     const GradInfo r = grad_info(p, n_partials, loss_scale, max_norm);
     if (blockIdx.x == 0u && threadIdx.x == 0u) *info = r;
     const uint32_t c0 = static_cast<uint32_t>(static_cast<uint64_t>(t.chunks) * blockIdx.x / t.blocks);
     const uint32_t c1 = static_cast<uint32_t>(static_cast<uint64_t>(t.chunks) * (blockIdx.x + 1u) / t.blocks);
-    for (uint32_t c = c1; c-- > c0;) {
-        const GradEntry& e = t.e[entry_of(t, c)];
-        if (r.scale == 1.0f && e.out == e.g) continue;  // in place and nothing to clip
-        const uint64_t e0 = static_cast<uint64_t>(c - e.chunk0) * kChunk, e1 = min(e.count, e0 + kChunk);
-        switch (e.type * 4u + e.out_type) {
-            case NERF_B200_F32 * 4u + NERF_B200_F32: chunk_scale<NERF_B200_F32, NERF_B200_F32>(e, e0, e1, r.scale); break;
-            case NERF_B200_F16 * 4u + NERF_B200_F16: chunk_scale<NERF_B200_F16, NERF_B200_F16>(e, e0, e1, r.scale); break;
-            case NERF_B200_F16 * 4u + NERF_B200_F32: chunk_scale<NERF_B200_F16, NERF_B200_F32>(e, e0, e1, r.scale); break;
-            case NERF_B200_BF16 * 4u + NERF_B200_BF16: chunk_scale<NERF_B200_BF16, NERF_B200_BF16>(e, e0, e1, r.scale); break;
-            default: chunk_scale<NERF_B200_BF16, NERF_B200_F32>(e, e0, e1, r.scale); break;
-        }
+    for (uint32_t c = c1; c-- > c0;) scale_of(t.e[entry_of(t, c)], c, r.scale);
+}
+
+// A list of at most kSmallChunks chunks: one cluster of eight blocks makes the
+// norm and clips in one launch, the partial sums over distributed shared memory.
+template <uint32_t CAP>
+__global__ void __launch_bounds__(kThreads)
+    k_grad_small(const __grid_constant__ GradTable<CAP> t, float loss_scale, float max_norm, uint32_t clip, GradInfo* info) {
+    __shared__ double part;
+    __shared__ uint32_t part_bad;
+    const uint32_t rank = tma::cluster_rank();
+    double sum = 0.0;
+    uint32_t bad = 0u;
+    after_previous();
+    let_next_start();
+    for (uint32_t c = rank; c < t.chunks; c += kSmallBlocks) squares_of(t.e[entry_of(t, c)], c, sum, bad);
+    const bool any = block_sum(sum, bad);
+    if (threadIdx.x == 0u) {
+        part = sum;
+        part_bad = any ? 1u : 0u;
     }
+    __syncthreads();
+    tma::cluster_sync();
+    sum = 0.0;
+    bad = 0u;
+#pragma unroll
+    for (uint32_t r = 0; r < kSmallBlocks; ++r) {
+        sum += tma::peer_f64(smem_u32(&part), r);
+        bad |= tma::peer_u32(smem_u32(&part_bad), r);
+    }
+    __syncthreads();
+    tma::cluster_sync();  // no block leaves while another reads its sum
+    const GradInfo r = make_info(sum, bad != 0u, loss_scale, max_norm);
+    if (rank == 0u && threadIdx.x == 0u) *info = r;
+    if (clip)
+        for (uint32_t c = rank; c < t.chunks; c += kSmallBlocks) scale_of(t.e[entry_of(t, c)], c, r.scale);
 }
 
 // ------------------------------------------------------------------- host
@@ -278,7 +332,7 @@ uint32_t resident_blocks() {
     int dev = 0, sms = 148;
     if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
         cudaGetLastError();
-    return std::min(kMaxBlocks, 4u * static_cast<uint32_t>(sms));
+    return std::min(kMaxBlocks, 6u * static_cast<uint32_t>(sms));
 }
 uint32_t type_bytes(uint32_t t) { return t == NERF_B200_F32 ? 4u : 2u; }
 bool valid_tensor(const NerfB200GradTensor& t) {
@@ -302,9 +356,12 @@ int outputs_apart(const NerfB200GradTensor* ts, uint32_t n) {
     if (!r) return -1;
     uint32_t m = 0;
     bool sorted = true;
+    uint64_t g_lo = ~0ull, g_hi = 0u;  // all gradients lie in here
     for (uint32_t i = 0; i < n; ++i) {
         if (ts[i].count == 0u) continue;
-        const uint64_t lo = reinterpret_cast<uint64_t>(ts[i].out);
+        const uint64_t g = reinterpret_cast<uint64_t>(ts[i].grad), lo = reinterpret_cast<uint64_t>(ts[i].out);
+        g_lo = std::min(g_lo, g);
+        g_hi = std::max(g_hi, g + ts[i].count * type_bytes(ts[i].dtype));
         r[m] = Range{lo, lo + ts[i].count * type_bytes(ts[i].out_dtype)};
         if (m && r[m].lo < r[m - 1u].lo) sorted = false;
         ++m;
@@ -312,7 +369,8 @@ int outputs_apart(const NerfB200GradTensor* ts, uint32_t n) {
     if (!sorted) std::sort(r, r + m, [](const Range& a, const Range& b) { return a.lo < b.lo; });
     bool apart = true;
     for (uint32_t i = 1; i < m && apart; ++i) apart = r[i - 1u].hi <= r[i].lo;
-    for (uint32_t i = 0; i < n && apart; ++i) {
+    const bool meet = m && g_lo < r[m - 1u].hi && r[0].lo < g_hi;  // else no gradient lies among the outputs
+    for (uint32_t i = 0; i < n && apart && meet; ++i) {
         if (ts[i].count == 0u || (ts[i].out == ts[i].grad && ts[i].dtype == ts[i].out_dtype)) continue;
         const uint64_t lo = reinterpret_cast<uint64_t>(ts[i].grad), hi = lo + ts[i].count * type_bytes(ts[i].dtype);
         const Range* q = std::upper_bound(r, r + m, lo, [](uint64_t v, const Range& a) { return v < a.hi; });  // first that ends after lo
@@ -353,17 +411,21 @@ template <uint32_t CAP>
 cudaError_t squares(const NerfB200GradTensor* ts, uint32_t n, uint32_t blocks, GradPartial* out, uint32_t* used, cudaStream_t s) {
     GradTable<CAP> t;
     fill_table(t, ts, n, blocks);
-    k_grad_squares<CAP><<<t.blocks, kThreads, 0, s>>>(t, out);
     *used = t.blocks;
-    return cudaGetLastError();
+    return launch_after(k_grad_squares<CAP>, dim3(t.blocks), kThreads, 0u, 1u, s, t, out);
 }
 template <uint32_t CAP>
 cudaError_t scales(const NerfB200GradTensor* ts, uint32_t n, uint32_t blocks, const GradPartial* p, uint32_t n_partials, float loss_scale,
                    float max_norm, GradInfo* info, cudaStream_t s) {
     GradTable<CAP> t;
     fill_table(t, ts, n, blocks);
-    k_grad_scale<CAP><<<t.blocks, kThreads, 0, s>>>(t, p, n_partials, loss_scale, max_norm, info);
-    return cudaGetLastError();
+    return launch_after(k_grad_scale<CAP>, dim3(t.blocks), kThreads, 0u, 1u, s, t, p, n_partials, loss_scale, max_norm, info);
+}
+template <uint32_t CAP>
+cudaError_t small(const NerfB200GradTensor* ts, uint32_t n, float loss_scale, bool clip, float max_norm, GradInfo* info, cudaStream_t s) {
+    GradTable<CAP> t;
+    fill_table(t, ts, n, 1u);
+    return launch_after(k_grad_small<CAP>, dim3(kSmallBlocks), kThreads, 0u, kSmallBlocks, s, t, loss_scale, max_norm, clip ? 1u : 0u, info);
 }
 
 uint32_t groups_of(uint32_t n) { return n == 0u ? 1u : (n + kTable - 1u) / kTable; }
@@ -385,6 +447,11 @@ NerfStatus norm_and_clip(const NerfB200GradTensor* ts, uint32_t n, float loss_sc
     }
     GradPartial* parts = static_cast<GradPartial*>(workspace);
     GradInfo* gi = reinterpret_cast<GradInfo*>(info);
+    if (n <= kTable && group_chunks(ts, n) <= kSmallChunks) {
+        const float most = clip ? max_norm : INFINITY;
+        const cudaError_t e = n <= 16u ? small<16u>(ts, n, loss_scale, clip, most, gi, s) : small<kTable>(ts, n, loss_scale, clip, most, gi, s);
+        return e == cudaSuccess ? NERF_STATUS_OK : NERF_STATUS_CUDA_ERROR;
+    }
     const uint32_t blocks = resident_blocks();
     uint32_t used = 0;
     for (uint32_t i = 0; i < n || i == 0u; i += kTable) {
@@ -396,8 +463,7 @@ NerfStatus norm_and_clip(const NerfB200GradTensor* ts, uint32_t n, float loss_sc
         used += more;
     }
     if (!clip) {
-        k_grad_finish<<<1, kThreads, 0, s>>>(parts, used, loss_scale, gi);
-        return cudaGetLastError() == cudaSuccess ? NERF_STATUS_OK : NERF_STATUS_CUDA_ERROR;
+        return launch_after(k_grad_finish, dim3(1), kThreads, 0u, 1u, s, static_cast<const GradPartial*>(parts), used, loss_scale, gi) == cudaSuccess ? NERF_STATUS_OK : NERF_STATUS_CUDA_ERROR;
     }
     for (uint32_t i = 0; i < n || i == 0u; i += kTable) {
         const uint32_t k = std::min(kTable, n - i);

@@ -437,6 +437,8 @@ __global__ void __launch_bounds__(GemmShape<BN, KIND, FEED>::kThreads, 1) k_gemm
     __syncthreads();
     if (S::kPair) tma::cluster_sync();  // the other CTA's barriers exist before anything signals them
     umma::fence_after_sync();
+    after_previous();
+    let_next_start();
     const uint32_t tmem = bar.tmem_base;
     const uint32_t tiles = g.tiles_m * g.tiles_n, items = tiles * g.splits;
     if (S::kRegs && warp < 4u) tma::registers_down<S::kRegsDown>();
@@ -834,6 +836,8 @@ __global__ void __launch_bounds__(ColsShape<BN, PLAIN>::kThreads) k_gemm_cols(co
     umma::fence_before_sync();
     __syncthreads();
     umma::fence_after_sync();
+    after_previous();
+    let_next_start();
     const uint32_t tmem = tmem_base;
 
     if ((!PLAIN && warp == 0u && lane == 0u) || (PLAIN && warp >= 8u)) {
@@ -970,18 +974,7 @@ cudaError_t launch_cols_t(const GemmArgs& g, const GemmMaps& maps, cudaStream_t 
         if (e != cudaSuccess) return e;
         done[dev] = true;
     }
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(g.tiles_m * g.tiles_n * g.splits);
-    cfg.blockDim = dim3(S::kThreads);
-    cfg.dynamicSmemBytes = S::kSmem;
-    cfg.stream = s;
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = g.splits;
-    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1u;
-    cfg.attrs = at;
-    cfg.numAttrs = g.splits > 1u ? 1u : 0u;
-    return cudaLaunchKernelEx(&cfg, k_gemm_cols<BN, PLAIN>, g, maps);
+    return launch_after(k_gemm_cols<BN, PLAIN>, dim3(g.tiles_m * g.tiles_n * g.splits), S::kThreads, S::kSmem, g.splits, s, g, maps);
 }
 
 // ------------------------------------------------- dz and its column sums
@@ -1003,6 +996,8 @@ NB_DEV void dz_row(uint32_t (&w)[4], const uint16_t* q, uint32_t have, bool vec)
 template <uint32_t ACT, bool VEC>
 __global__ void __launch_bounds__(256, 4) k_dz(const DzArgs a, uint32_t cg_log2) {
     __shared__ float sums[256][8];
+    after_previous();
+    let_next_start();
     const bool bf16 = a.bf16 != 0u;
     const uint32_t cg = 1u << cg_log2, gx = threadIdx.x & (cg - 1u), gy = threadIdx.x >> cg_log2, ny = 256u >> cg_log2;
     const uint32_t c0 = 8u * (blockIdx.x * cg + gx);
@@ -1064,25 +1059,46 @@ NB_DEV void grad_out(void* p, uint64_t i, float v, const GradReduceArgs& a) {
         *q = to_16(a.accumulate ? from_16(*q, a.bf16 != 0u) + v : v, a.bf16 != 0u);
     }
 }
-// Blocks below n_dw: one row group of 128 x 4 columns of dw each, in split
-// order; the others: 32 columns of db, eight warps each a range of the parts.
+// Blocks below n_dw: 32 rows x 4 columns of dw; the others: 32 columns of db.
+// Eight warps take an eighth of the parts each, all of a batch's loads in
+// flight, and the first adds the eight sums: a fixed order.
 __global__ void __launch_bounds__(256) k_grad_reduce(const GradReduceArgs a, uint32_t n_dw) {
+    __shared__ float4 ws[8][32];
+    const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
+    after_previous();
+    let_next_start();
     if (blockIdx.x < n_dw) {
+        const uint32_t per_tile = a.bn / 4u, quarter = blockIdx.x & 3u, idx = blockIdx.x >> 2;
         // half: 128 rows of a tile (a pair of CTAs leaves two)
-        const uint32_t per_tile = a.bn / 4u, idx = 2u * blockIdx.x + (threadIdx.x >> 7);
-        const uint32_t half = idx / per_tile, c4 = idx - half * per_tile, row = threadIdx.x & 127u;
+        const uint32_t half = idx / per_tile, c4 = idx - half * per_tile, row = 32u * quarter + lane;
         const uint32_t tiles = a.tiles_m * a.tiles_n, tile = half / a.ctas;
-        if (tile >= tiles) return;
         const uint32_t per = 16u * a.tiles_n, group = tile / per, first = 16u * group;
         const uint32_t gm = min(16u, a.tiles_m - first), r = tile - group * per;
         const uint32_t m = ((first + r % gm) * a.ctas + half % a.ctas) * kBM + row, n = (r / gm) * a.bn + 4u * c4;
-        if (m >= a.n_out || n >= a.n_in) return;
         const float4* src = reinterpret_cast<const float4*>(a.partials) + (static_cast<uint64_t>(half) * per_tile + c4) * kBM + row;
         const uint64_t step = static_cast<uint64_t>(tiles) * a.ctas * per_tile * kBM;
+        const uint32_t each = (a.splits + 7u) / 8u, k0 = min(a.splits, warp * each), k1 = min(a.splits, k0 + each);
         float4 t = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-        for (uint32_t k = 0; k < a.splits; ++k) {
-            const float4 v = __ldcs(src + k * step);
+        if (n < a.n_in) {
+            for (uint32_t k = k0; k < k1; k += 8u) {
+                float4 v[8];
+#pragma unroll
+                for (uint32_t j = 0; j < 8u; ++j) v[j] = k + j < k1 ? __ldcs(src + (k + j) * step) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+                for (uint32_t j = 0; j < 8u; ++j) {
+                    t.x += v[j].x;
+                    t.y += v[j].y;
+                    t.z += v[j].z;
+                    t.w += v[j].w;
+                }
+            }
+        }
+        ws[warp][lane] = t;
+        __syncthreads();
+        if (warp != 0u || m >= a.n_out || n >= a.n_in) return;
+#pragma unroll
+        for (uint32_t w = 1; w < 8u; ++w) {
+            const float4 v = ws[w][lane];
             t.x += v.x;
             t.y += v.y;
             t.z += v.z;
@@ -1094,20 +1110,23 @@ __global__ void __launch_bounds__(256) k_grad_reduce(const GradReduceArgs a, uin
             if (n + i < a.n_in) grad_out(a.dw, static_cast<uint64_t>(m) * a.n_in + n + i, o[i], a);
         return;
     }
-    __shared__ float ws[8][32];
-    const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5, c = 32u * (blockIdx.x - n_dw) + lane;
+    const uint32_t c = 32u * (blockIdx.x - n_dw) + lane;
     const uint32_t per = (a.parts + 7u) / 8u, p0 = min(a.parts, warp * per), p1 = min(a.parts, p0 + per);
     float t = 0.0f;
     if (c < a.n_out) {
-#pragma unroll 16
-        for (uint32_t p = p0; p < p1; ++p) t += a.db_part[static_cast<uint64_t>(p) * a.n_out + c];
+        for (uint32_t p = p0; p < p1; p += 16u) {
+            float v[16];
+#pragma unroll
+            for (uint32_t j = 0; j < 16u; ++j) v[j] = p + j < p1 ? a.db_part[static_cast<uint64_t>(p + j) * a.n_out + c] : 0.0f;
+#pragma unroll
+            for (uint32_t j = 0; j < 16u; ++j) t += v[j];
+        }
     }
-    ws[warp][lane] = t;
+    ws[warp][lane].x = t;
     __syncthreads();
     if (warp == 0u && c < a.n_out) {
-        t = ws[0][lane];
 #pragma unroll
-        for (uint32_t w = 1; w < 8u; ++w) t += ws[w][lane];
+        for (uint32_t w = 1; w < 8u; ++w) t += ws[w][lane].x;
         grad_out(a.db, c, t, a);
     }
 }
@@ -1130,18 +1149,7 @@ cudaError_t launch_gemm_t(const GemmArgs& g, const GemmMaps& maps, uint32_t bloc
         if (S::kRegs && static_cast<uint32_t>(fa.numRegs) * S::kThreads < S::kRegsNeeded) return cudaErrorInvalidConfiguration;
         done[dev] = true;
     }
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(blocks);
-    cfg.blockDim = dim3(S::kThreads);
-    cfg.dynamicSmemBytes = S::kSmem;
-    cfg.stream = s;
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = S::kPair ? 2u : 1u;
-    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1u;
-    cfg.attrs = at;
-    cfg.numAttrs = S::kPair ? 1u : 0u;
-    return cudaLaunchKernelEx(&cfg, k_gemm<BN, KIND, FEED>, g, maps);
+    return launch_after(k_gemm<BN, KIND, FEED>, dim3(blocks), S::kThreads, S::kSmem, S::kPair ? 2u : 1u, s, g, maps);
 }
 template <int KIND, int FEED>
 cudaError_t launch_gemm_bn(const GemmArgs& g, uint32_t bn, const GemmMaps& maps, uint32_t blocks, cudaStream_t s) {
@@ -1190,23 +1198,19 @@ cudaError_t launch_dz(const DzArgs& a, cudaStream_t s) {
     const dim3 grid((groups + (1u << log2) - 1u) >> log2, a.parts);
     const bool vec = a.dy.vec >= 8u && (a.act == kActNone || a.pre.vec >= 8u);
     switch (a.act) {
-        case kActRelu: vec ? k_dz<kActRelu, true><<<grid, 256, 0, s>>>(a, log2) : k_dz<kActRelu, false><<<grid, 256, 0, s>>>(a, log2); break;
-        case kActSilu: vec ? k_dz<kActSilu, true><<<grid, 256, 0, s>>>(a, log2) : k_dz<kActSilu, false><<<grid, 256, 0, s>>>(a, log2); break;
-        case kActGelu: vec ? k_dz<kActGelu, true><<<grid, 256, 0, s>>>(a, log2) : k_dz<kActGelu, false><<<grid, 256, 0, s>>>(a, log2); break;
-        case kActSigmoid:
-            vec ? k_dz<kActSigmoid, true><<<grid, 256, 0, s>>>(a, log2) : k_dz<kActSigmoid, false><<<grid, 256, 0, s>>>(a, log2);
-            break;
-        default: vec ? k_dz<kActNone, true><<<grid, 256, 0, s>>>(a, log2) : k_dz<kActNone, false><<<grid, 256, 0, s>>>(a, log2); break;
+        case kActRelu: return launch_after(vec ? k_dz<kActRelu, true> : k_dz<kActRelu, false>, grid, 256u, 0u, 1u, s, a, log2);
+        case kActSilu: return launch_after(vec ? k_dz<kActSilu, true> : k_dz<kActSilu, false>, grid, 256u, 0u, 1u, s, a, log2);
+        case kActGelu: return launch_after(vec ? k_dz<kActGelu, true> : k_dz<kActGelu, false>, grid, 256u, 0u, 1u, s, a, log2);
+        case kActSigmoid: return launch_after(vec ? k_dz<kActSigmoid, true> : k_dz<kActSigmoid, false>, grid, 256u, 0u, 1u, s, a, log2);
+        default: return launch_after(vec ? k_dz<kActNone, true> : k_dz<kActNone, false>, grid, 256u, 0u, 1u, s, a, log2);
     }
-    return cudaGetLastError();
 }
 
 cudaError_t launch_grad_reduce(const GradReduceArgs& a, cudaStream_t s) {
-    const uint32_t n_dw = a.dw ? (a.tiles_m * a.tiles_n * a.ctas * (a.bn / 4u) + 1u) / 2u : 0u;
+    const uint32_t n_dw = a.dw ? a.tiles_m * a.tiles_n * a.ctas * (a.bn / 4u) * 4u : 0u;
     const uint32_t n_db = a.db ? (a.n_out + 31u) / 32u : 0u;
     if (n_dw + n_db == 0u) return cudaSuccess;
-    k_grad_reduce<<<n_dw + n_db, 256, 0, s>>>(a, n_dw);
-    return cudaGetLastError();
+    return launch_after(k_grad_reduce, dim3(n_dw + n_db), 256u, 0u, 1u, s, a, n_dw);
 }
 
 }  // namespace nb

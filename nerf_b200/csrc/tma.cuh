@@ -159,5 +159,16 @@ NB_DEV float peer_f32(uint32_t addr, uint32_t rank) {
     return v;
 }
 
+NB_DEV double peer_f64(uint32_t addr, uint32_t rank) {
+    double v;
+    asm volatile("ld.shared::cluster.f64 %0, [%1];\n" : "=d"(v) : "r"(peer_addr(addr, rank)) : "memory");
+    return v;
+}
+NB_DEV uint32_t peer_u32(uint32_t addr, uint32_t rank) {
+    uint32_t v;
+    asm volatile("ld.shared::cluster.u32 %0, [%1];\n" : "=r"(v) : "r"(peer_addr(addr, rank)) : "memory");
+    return v;
+}
+
 }  // namespace tma
 }  // namespace nb
