@@ -83,6 +83,22 @@ struct GradReduceArgs {
 };
 cudaError_t launch_grad_reduce(const GradReduceArgs& a, cudaStream_t s);
 
+// The backward of a layer with n_in, n_out <= 128 in one pass
+// (linear_narrow.cu): dx, and one partial tile [in / 4][128][4] of dw and row
+// of db per CTA, as launch_grad_reduce reads them (one tile of 64 or 128
+// columns, splits = blocks).
+struct NarrowArgs {
+    uint32_t n, n_in, n_out, act, bf16;
+    MatrixView dx, res;  // res.ptr null: none
+    uint32_t dx_tma, res_tma;
+    float *partials, *db_part;  // db_part null: none
+    uint32_t* error;
+};
+struct NarrowMaps {
+    CUtensorMap dy, pre, x, w, dx, res;
+};
+cudaError_t launch_backward_narrow(const NarrowArgs& a, const NarrowMaps& maps, uint32_t blocks, cudaStream_t s);
+
 constexpr uint32_t kGemmBM = 128, kGemmBK = 64;
 
 }  // namespace nb

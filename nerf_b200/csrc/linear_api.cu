@@ -75,6 +75,9 @@ EncodeTiled encode_tiled() {
     }();
     return fn;
 }
+// Whether the copy unit can store into a matrix: it writes whole 16-byte
+// pieces, so a row must start and end with one.
+bool tma_rows(const MatrixView& m) { return m.ptr && m.vec >= 8u && m.cols % 8u == 0u; }
 // Boxes of box_rows x 64 values of a matrix, 128-byte swizzle, zero outside it.
 bool make_map(CUtensorMap* map, const MatrixView& m, uint32_t box_rows, bool bf16) {
     const EncodeTiled fn = encode_tiled();
@@ -138,6 +141,14 @@ GradPlan plan_grad(const NerfB200Linear& d, bool plain, uint32_t sms) {
     return p;
 }
 
+// Layers whose whole backward one kernel does in one pass over the rows.
+bool narrow(const NerfB200Linear& d) { return d.n_in <= 128u && d.n_out <= 128u; }
+uint32_t narrow_bn(const NerfB200Linear& d) { return d.n_in <= 64u ? 64u : 128u; }
+uint32_t narrow_blocks(const NerfB200Linear& d, uint32_t sms) {
+    const uint32_t tiles = ceil_div(d.n_rows, kGemmBM);
+    return tiles < sms ? tiles : sms;
+}
+
 struct BackwardPlan {
     uint32_t sms;
     bool dz_needed;                 // dz is not dy itself
@@ -162,11 +173,14 @@ BackwardPlan plan_backward(const NerfB200Linear& d) {
     p.o_dz = at;
     if (p.dz_needed) at += up(static_cast<uint64_t>(d.n_rows) * p.dz_ld * 2u, 256u);
     p.o_db = at;
-    at += up(static_cast<uint64_t>(p.parts) * d.n_out * 4u, 256u);
+    const uint32_t blocks = narrow(d) ? narrow_blocks(d, p.sms) : 0u;
+    at += up(static_cast<uint64_t>(p.parts > blocks ? p.parts : blocks) * d.n_out * 4u, 256u);
     p.o_dw = at;
-    // How the operands can be fed depends on the pointers: room for either way.
+    // How the operands can be fed depends on the pointers: room for every way.
     const uint64_t tma = plan_grad(d, false, p.sms).bytes, plain = plan_grad(d, true, p.sms).bytes;
-    at += tma > plain ? tma : plain;
+    const uint64_t one = static_cast<uint64_t>(blocks) * kGemmBM * narrow_bn(d) * 4u;
+    const uint64_t most = tma > plain ? tma : plain;
+    at += one > most ? one : most;
     p.bytes = at ? at : 256u;
     return p;
 }
@@ -197,9 +211,8 @@ cudaError_t run_gemm(GemmArgs& g, int kind, uint32_t bn, bool pair, uint32_t sms
     if (!plain && (!make_map(&maps.a, g.a, g.a_mn ? kGemmBK : g.a_box_rows, bf16) ||
                    !make_map(&maps.b, g.b, g.b_mn ? kGemmBK : pair ? bn / 2u : bn, bf16)))
         return cudaErrorNotSupported;
-    // The copy unit writes whole 16-byte pieces: a row must end with one.
-    g.y_tma = g.y.ptr && g.y.vec >= 8u && g.y.cols % 8u == 0u;
-    g.pre_tma = g.pre.ptr && g.pre.vec >= 8u && g.pre.cols % 8u == 0u;
+    g.y_tma = tma_rows(g.y);
+    g.pre_tma = tma_rows(g.pre);
     g.res_tma = g.res.ptr && g.res.vec >= 8u;
     if ((g.res_tma && !make_map(&maps.res, g.res, 32u, bf16)) || (g.y_tma && !make_map(&maps.y, g.y, 32u, bf16)) || (g.pre_tma && !make_map(&maps.pre, g.pre, 32u, bf16)))
         return cudaErrorNotSupported;
@@ -331,12 +344,56 @@ NERF_API NerfStatus nerf_b200_linear_backward(const NerfB200Linear* desc, const 
     unsigned char* ws = static_cast<unsigned char*>(workspace);
     const uint32_t bf16 = d.dtype == NERF_B200_BF16;
     const MatrixView dyv = view(dy, ld_or(d.ld_dy, d.n_out), d.n_rows, d.n_out);
+    GradReduceArgs r{};
+    r.n_out = d.n_out;
+    r.n_in = d.n_in;
+    r.f32 = d.grad_dtype == NERF_B200_F32;
+    r.bf16 = bf16;
+    r.accumulate = d.accumulate;
+    if (dbias) {
+        r.db_part = reinterpret_cast<float*>(ws + p.o_db);
+        r.parts = p.parts;
+        r.db = dbias;
+    }
+    const MatrixView xv = view(x, ld_or(d.ld_x, d.n_in), d.n_rows, d.n_in), wv = view(weight, ld_or(d.ld_weight, d.n_in), d.n_out, d.n_in);
+    const MatrixView prev = view(pre, ld_or(d.ld_pre, d.n_out), d.n_rows, d.n_out);
+    const MatrixView resv = view(dx_residual, ld_or(d.ld_residual, d.n_in), d.n_rows, d.n_in), dxv = view(dx, ld_or(d.ld_dx, d.n_in), d.n_rows, d.n_in);
+    if (dx && dweight && narrow(d) && dyv.vec >= 8u && xv.vec >= 8u && wv.vec >= 8u && (d.activation == kActNone || prev.vec >= 8u)) {
+        NarrowArgs a{};
+        a.n = d.n_rows;
+        a.n_in = d.n_in;
+        a.n_out = d.n_out;
+        a.act = d.activation;
+        a.bf16 = bf16;
+        a.dx = dxv;
+        a.res = resv;
+        a.dx_tma = tma_rows(dxv);
+        a.res_tma = resv.ptr && resv.vec >= 8u;
+        a.partials = reinterpret_cast<float*>(ws + p.o_dw);
+        a.db_part = dbias ? reinterpret_cast<float*>(ws + p.o_db) : nullptr;
+        a.error = error_word;
+        const uint32_t blocks = narrow_blocks(d, p.sms), ob = d.n_out <= 64u ? 64u : 128u;
+        NarrowMaps maps{};
+        const bool b = bf16 != 0u;
+        if (!make_map(&maps.dy, dyv, kGemmBM, b) || (a.act != kActNone && !make_map(&maps.pre, prev, kGemmBM, b)) ||
+            !make_map(&maps.x, xv, kGemmBM, b) || !make_map(&maps.w, wv, ob, b) || (a.dx_tma && !make_map(&maps.dx, dxv, 32u, b)) ||
+            (a.res_tma && !make_map(&maps.res, resv, 32u, b)))
+            return NERF_STATUS_CUDA_ERROR;
+        if (launch_backward_narrow(a, maps, blocks, s) != cudaSuccess) return NERF_STATUS_CUDA_ERROR;
+        r.partials = a.partials;
+        r.splits = blocks;
+        r.tiles_m = r.tiles_n = r.ctas = 1u;
+        r.bn = narrow_bn(d);
+        r.dw = dweight;
+        r.parts = blocks;
+        return launch_grad_reduce(r, s) == cudaSuccess ? NERF_STATUS_OK : NERF_STATUS_CUDA_ERROR;
+    }
     const bool dz_written = p.dz_needed && (dx || dweight);
     const MatrixView dzv = p.dz_needed ? view(ws + p.o_dz, p.dz_ld, d.n_rows, d.n_out) : dyv;
     if (dz_written || dbias) {
         DzArgs a{};
         a.dy = dyv;
-        a.pre = view(pre, ld_or(d.ld_pre, d.n_out), d.n_rows, d.n_out);
+        a.pre = prev;
         a.dz = dz_written ? ws + p.o_dz : nullptr;
         a.dz_ld = p.dz_ld;
         a.db_part = dbias ? reinterpret_cast<float*>(ws + p.o_db) : nullptr;
@@ -352,27 +409,21 @@ NERF_API NerfStatus nerf_b200_linear_backward(const NerfB200Linear* desc, const 
         g.N = d.n_in;
         g.K = d.n_out;
         g.a = dzv;
-        g.b = view(weight, ld_or(d.ld_weight, d.n_in), d.n_out, d.n_in);
+        g.b = wv;
         g.b_mn = 1u;
         g.bf16 = bf16;
-        g.res = view(dx_residual, ld_or(d.ld_residual, d.n_in), d.n_rows, d.n_in);
-        g.y = view(dx, ld_or(d.ld_dx, d.n_in), d.n_rows, d.n_in);
+        g.res = resv;
+        g.y = dxv;
         g.error = error_word;
         if (run_rows(g, p.sms, s) != cudaSuccess) return NERF_STATUS_CUDA_ERROR;
     }
-    GradReduceArgs r{};
-    r.n_out = d.n_out;
-    r.n_in = d.n_in;
-    r.f32 = d.grad_dtype == NERF_B200_F32;
-    r.bf16 = bf16;
-    r.accumulate = d.accumulate;
     if (dweight) {
         GemmArgs g{};
         g.M = d.n_out;
         g.N = d.n_in;
         g.K = d.n_rows;
         g.a = dzv;
-        g.b = view(x, ld_or(d.ld_x, d.n_in), d.n_rows, d.n_in);
+        g.b = xv;
         g.a_mn = g.b_mn = 1u;
         const GradPlan w = plan_grad(d, g.a.vec < 8u || g.b.vec < 8u, p.sms);
         g.tiles_m = w.tiles_m;
@@ -397,11 +448,6 @@ NERF_API NerfStatus nerf_b200_linear_backward(const NerfB200Linear* desc, const 
             r.bn = w.bn;
             r.dw = dweight;
         }
-    }
-    if (dbias) {
-        r.db_part = reinterpret_cast<float*>(ws + p.o_db);
-        r.parts = p.parts;
-        r.db = dbias;
     }
     return launch_grad_reduce(r, s) == cudaSuccess ? NERF_STATUS_OK : NERF_STATUS_CUDA_ERROR;
 }

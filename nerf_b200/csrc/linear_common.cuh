@@ -1,0 +1,264 @@
+// linear_common.cuh -- what the dense-layer kernels share: 16-bit values, the
+// activations, and the shared-memory slabs that epilogue warps read and write
+// global memory through.
+#pragma once
+#include <cuda_bf16.h>
+
+#include "linear.h"
+#include "tma.cuh"
+
+namespace nb {
+namespace {
+
+constexpr uint32_t kSlabBytes = 32u * 128u;  // one epilogue warp's 32 rows x 128 bytes
+__host__ __device__ constexpr uint32_t tmem_cols(uint32_t n) { return n <= 32u ? 32u : n <= 64u ? 64u : n <= 128u ? 128u : n <= 256u ? 256u : 512u; }
+// 64-row steps that a weight gradient's MMAs sum in tensor memory before the
+// sum moves to registers.  The tensor core's additions cut off instead of
+// rounding: 32 of them in a row are off by 6e-7 of the result, 512 by 1e-5.
+constexpr uint32_t kChunkSteps = 8;
+
+// ------------------------------------------------------------ 16-bit values
+NB_DEV float from_16(uint16_t v, bool bf16) {
+    if (bf16) return __uint_as_float(static_cast<uint32_t>(v) << 16);
+    return h2f_bits(v);
+}
+NB_DEV float2 unpack_16(uint32_t v, bool bf16) {
+    if (bf16) return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
+    return unpack_h2(v);
+}
+NB_DEV uint32_t pack_16(float lo, float hi, bool bf16) {
+    if (bf16) {
+        __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+        return *reinterpret_cast<uint32_t*>(&h);
+    }
+    return pack_h2(lo, hi);
+}
+NB_DEV uint16_t to_16(float v, bool bf16) { return static_cast<uint16_t>(pack_16(v, 0.0f, bf16) & 0xffffu); }
+
+// ------------------------------------------------------------- activations
+NB_DEV float sigmoid_f(float z) { return __fdividef(1.0f, 1.0f + __expf(-z)); }
+// Phi(z) and exp(-z^2 / 2).  erfc(x) = (a1 t + ... + a5 t^5) exp(-x^2) with
+// t = 1 / (1 + p x) (Abramowitz and Stegun, Handbook of Mathematical
+// Functions, 7.1.26: off by at most 1.5e-7, a thousandth of a step of the
+// 16-bit result).
+NB_DEV float phi_f(float z, float& e) {
+    const float x = fabsf(z) * 0.70710678118654752f;
+    const float t = __fdividef(1.0f, fmaf(0.3275911f, x, 1.0f));
+    float p = fmaf(1.061405429f, t, -1.453152027f);
+    p = fmaf(p, t, 1.421413741f);
+    p = fmaf(p, t, -0.284496736f);
+    p = fmaf(p, t, 0.254829592f);
+    e = __expf(-0.5f * z * z);
+    const float tail = 0.5f * p * t * e;
+    return z > 0.0f ? 1.0f - tail : tail;
+}
+NB_DEV float act_f(float z, uint32_t act) {
+    switch (act) {
+        case kActRelu: return z > 0.0f ? z : 0.0f;
+        case kActSilu: return z * sigmoid_f(z);
+        case kActGelu: {
+            float e;
+            return z * phi_f(z, e);
+        }
+        case kActSigmoid: return sigmoid_f(z);
+        default: return z;
+    }
+}
+// One activation over a register row: the choice is made once, not per value.
+template <int N>
+NB_DEV void act_row(float (&v)[N], uint32_t act) {
+    switch (act) {
+#define NB_ACT_ROW(kind)                                   \
+    case kind:                                             \
+        _Pragma("unroll") for (int i = 0; i < N; ++i) v[i] = act_f(v[i], kind); \
+        break;
+        NB_ACT_ROW(kActRelu)
+        NB_ACT_ROW(kActSilu)
+        NB_ACT_ROW(kActGelu)
+        NB_ACT_ROW(kActSigmoid)
+#undef NB_ACT_ROW
+        default: break;
+    }
+}
+// dy act'(z).  ReLU selects: a closed unit passes nothing, whatever dy holds.
+NB_DEV float dact_f(float dy, float z, uint32_t act) {
+    switch (act) {
+        case kActRelu: return z > 0.0f ? dy : 0.0f;
+        case kActSilu: {
+            const float s = sigmoid_f(z);
+            return dy * (s * (1.0f + z * (1.0f - s)));
+        }
+        case kActGelu: {
+            float e;
+            const float p = phi_f(z, e);
+            return dy * fmaf(z * 0.39894228040143268f, e, p);
+        }
+        case kActSigmoid: {
+            const float s = sigmoid_f(z);
+            return dy * (s * (1.0f - s));
+        }
+        default: return dy;
+    }
+}
+
+// Loads that read nothing and give zero where `on` is false: predicated, so
+// that a batch of them is in flight together (as branches each would wait for
+// the one before).
+NB_DEV uint32_t load_16(const uint16_t* q, bool on) {
+    uint32_t v;
+    asm volatile(
+        "{\n.reg .pred p;\n.reg .u16 h;\nsetp.ne.u32 p, %2, 0;\nmov.u16 h, 0;\n@p ld.global.u16 h, [%1];\ncvt.u32.u16 %0, h;\n}\n"
+        : "=r"(v)
+        : "l"(q), "r"(static_cast<uint32_t>(on)));
+    return v;
+}
+NB_DEV uint32_t load_32(const void* q, bool on) {
+    uint32_t v;
+    asm volatile("{\n.reg .pred p;\nsetp.ne.u32 p, %2, 0;\nmov.u32 %0, 0;\n@p ld.global.u32 %0, [%1];\n}\n"
+                 : "=r"(v)
+                 : "l"(q), "r"(static_cast<uint32_t>(on)));
+    return v;
+}
+
+// ------------------------------------------------- slabs: 32 rows x 128 bytes
+// A warp's shared-memory slab, 16-byte pieces swizzled by the row so that both
+// "one row a thread" and "eight threads a row" accesses are conflict-free.
+NB_DEV uint32_t slab_at(uint32_t row, uint32_t piece) { return row * 128u + ((piece ^ (row & 7u)) << 4); }
+
+// Global -> slab or back: `rows` rows of `cols` values of ES bytes (cols * ES
+// <= 128) at g, ld values apart; vec: every row's first value is 16-byte aligned.
+template <int ES, bool kStore>
+NB_DEV void slab_copy(unsigned char* slab, unsigned char* g, uint64_t ld, uint32_t rows, uint32_t cols, bool vec, uint32_t lane) {
+    constexpr uint32_t kPer = 16u / ES;
+    if (vec) {
+        const uint32_t p = lane & 7u, r0 = lane >> 3;
+        if (rows == 32u && cols * ES == 128u) {  // whole: eight pieces a lane in flight
+            unsigned char* q = g + (r0 * ld + p * kPer) * ES;
+            const uint64_t step = 4u * ld * ES;
+            uint4 u[8];
+            if (kStore) {
+#pragma unroll
+                for (uint32_t i = 0; i < 8u; ++i) u[i] = *reinterpret_cast<const uint4*>(slab + slab_at(r0 + 4u * i, p));
+#pragma unroll
+                for (uint32_t i = 0; i < 8u; ++i) *reinterpret_cast<uint4*>(q + i * step) = u[i];
+            } else {
+#pragma unroll
+                for (uint32_t i = 0; i < 8u; ++i) u[i] = *reinterpret_cast<const uint4*>(q + i * step);
+#pragma unroll
+                for (uint32_t i = 0; i < 8u; ++i) *reinterpret_cast<uint4*>(slab + slab_at(r0 + 4u * i, p)) = u[i];
+            }
+            return;
+        }
+#pragma unroll 1
+        for (uint32_t r = r0; r < rows; r += 4u) {
+            unsigned char* q = g + (r * ld + p * kPer) * ES;
+            unsigned char* l = slab + slab_at(r, p);
+            if ((p + 1u) * kPer <= cols) {
+                if (kStore) *reinterpret_cast<uint4*>(q) = *reinterpret_cast<const uint4*>(l);
+                else *reinterpret_cast<uint4*>(l) = *reinterpret_cast<const uint4*>(q);
+            } else {
+                for (uint32_t e = p * kPer; e < cols; ++e) {
+                    const uint32_t o = (e - p * kPer) * ES;
+                    if (ES == 2) {
+                        if (kStore) *reinterpret_cast<uint16_t*>(q + o) = *reinterpret_cast<const uint16_t*>(l + o);
+                        else *reinterpret_cast<uint16_t*>(l + o) = *reinterpret_cast<const uint16_t*>(q + o);
+                    } else {
+                        if (kStore) *reinterpret_cast<uint32_t*>(q + o) = *reinterpret_cast<const uint32_t*>(l + o);
+                        else *reinterpret_cast<uint32_t*>(l + o) = *reinterpret_cast<const uint32_t*>(q + o);
+                    }
+                }
+            }
+        }
+        return;
+    }
+    // A row is 32 words of the slab: lane i moves word i, as one or two values.
+    const bool words = ES == 4 || ((reinterpret_cast<uintptr_t>(g) & 3u) == 0u && (ld & 1u) == 0u);
+    const bool lo = ES == 4 ? lane < cols : 2u * lane < cols, hi = ES == 4 ? lane < cols : 2u * lane + 1u < cols;
+    const uint64_t step = ld * ES;
+    unsigned char* q = g + 4u * lane;
+    constexpr uint32_t kBatch = 8;
+#pragma unroll 1
+    for (uint32_t r0 = 0; r0 < rows; r0 += kBatch) {
+        const uint32_t in = rows - r0;
+        uint32_t w[kBatch];
+        unsigned char* l[kBatch];
+#pragma unroll
+        for (uint32_t j = 0; j < kBatch; ++j) l[j] = slab + slab_at(r0 + j, lane >> 2) + 4u * (lane & 3u);
+        if (kStore) {
+#pragma unroll
+            for (uint32_t j = 0; j < kBatch; ++j) w[j] = *reinterpret_cast<const uint32_t*>(l[j]);
+#pragma unroll
+            for (uint32_t j = 0; j < kBatch; ++j) {
+                unsigned char* p = q + j * step;
+                if (words && !(cols & 1u)) {
+                    if (hi && j < in) *reinterpret_cast<uint32_t*>(p) = w[j];
+                } else if (ES == 4) {
+                    if (lo && j < in) *reinterpret_cast<uint32_t*>(p) = w[j];
+                } else {
+                    if (lo && j < in) *reinterpret_cast<uint16_t*>(p) = static_cast<uint16_t>(w[j]);
+                    if (hi && j < in) reinterpret_cast<uint16_t*>(p)[1] = static_cast<uint16_t>(w[j] >> 16);
+                }
+            }
+        } else {
+#pragma unroll
+            for (uint32_t j = 0; j < kBatch; ++j) {
+                const uint16_t* p = reinterpret_cast<const uint16_t*>(q + j * step);
+                if (ES == 4 || (words && !(cols & 1u))) w[j] = load_32(p, hi && j < in);
+                else w[j] = load_16(p, lo && j < in) | (load_16(p + 1, hi && j < in) << 16);
+            }
+#pragma unroll
+            for (uint32_t j = 0; j < kBatch; ++j) *reinterpret_cast<uint32_t*>(l[j]) = w[j];
+        }
+        q += kBatch * step;
+    }
+}
+NB_DEV void slab_put(unsigned char* slab, uint32_t row, uint32_t piece, const uint32_t w[4]) {
+    *reinterpret_cast<uint4*>(slab + slab_at(row, piece)) = make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// 32 accumulator columns of this thread's row plus the bias.
+NB_DEV void load_z(float (&v)[32], uint32_t taddr, const uint16_t* bias, bool bf16) {
+    umma::tmem_ld32(taddr, v);
+#pragma unroll
+    for (uint32_t i = 0; i < 4u; ++i) {
+        const uint4 u = *reinterpret_cast<const uint4*>(bias + 8u * i);
+        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float2 b = unpack_16(w[j], bf16);
+            v[8 * i + 2 * j] += b.x;
+            v[8 * i + 2 * j + 1] += b.y;
+        }
+    }
+}
+// 32 values -> pieces 4 h .. 4 h + 3 of this thread's slab row.
+NB_DEV void slab_put32(unsigned char* slab, uint32_t lane, uint32_t h, const float (&v)[32], bool bf16) {
+#pragma unroll
+    for (uint32_t p = 0; p < 4u; ++p) {
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = pack_16(v[8 * p + 2 * i], v[8 * p + 2 * i + 1], bf16);
+        slab_put(slab, lane, 4u * h + p, w);
+    }
+}
+
+// The warp's slab -> 32 rows x 64 columns at (row, col) of an output.
+NB_DEV void slab_out(unsigned char* slab, const MatrixView& m, bool by_tma, const CUtensorMap* map, uint32_t row, uint32_t col,
+                     uint32_t rows, uint32_t cols, uint32_t lane) {
+    if (by_tma) {
+        umma::fence_async_smem();
+        __syncwarp();
+        if (lane == 0u) {
+            tma::store_2d(map, smem_u32(slab), static_cast<int32_t>(col), static_cast<int32_t>(row));
+            tma::store_commit();
+        }
+    } else {
+        __syncwarp();
+        unsigned char* dst = static_cast<unsigned char*>(const_cast<void*>(m.ptr)) + 2u * (row * m.ld + col);
+        slab_copy<2, true>(slab, dst, m.ld, rows, cols, m.vec >= 8u, lane);
+        __syncwarp();
+    }
+}
+
+}  // namespace
+}  // namespace nb

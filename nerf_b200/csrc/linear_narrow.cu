@@ -1,0 +1,344 @@
+// linear_narrow.cu -- the whole backward of a narrow layer (n_in, n_out <= 128)
+// in one pass over its rows.
+//
+//   dz = dy act'(pre),  dx = dz W + r,  dW = dz^T x,  db = column sums of dz
+//
+// A narrow layer's backward is bound by memory: 4 n_in n_out operations a row
+// against 2 (2 n_in + 2 n_out) bytes.  Written as separate kernels dz goes out
+// to memory and comes back twice; here it never leaves the SM.  Per 128-row
+// tile the copies bring dy, pre and x into shared memory as swizzled boxes,
+// four warps replace dy by dz in place and keep the column sums in registers,
+// and the tensor core reads the same dz boxes twice: K-major against W (kept
+// in shared memory for the CTA's life) for dx, MN-major against x for dW.  dx
+// is drained tile by tile by two groups of four warps in turn; dW accumulates
+// in tensor memory for four tiles (512 rows, see kChunkSteps) and then in the
+// groups' registers, half of the columns each, until the CTA has no tiles
+// left.  Each CTA leaves one partial dW and db, which k_grad_reduce adds in CTA
+// order.
+#include <atomic>
+
+#include "linear_common.cuh"
+
+namespace nb {
+namespace {
+
+constexpr uint32_t kRowsTile = 128;
+constexpr uint32_t kBoxBytes = kRowsTile * 128u;  // 128 rows x 64 values
+constexpr uint32_t kChunkTiles = kChunkSteps * 64u / kRowsTile;
+
+// OB, IB: n_out and n_in rounded up to 64 or 128.
+template <uint32_t OB, uint32_t IB>
+struct NarrowShape {
+    static constexpr uint32_t kDy = OB / 64u * kBoxBytes, kX = IB / 64u * kBoxBytes, kW = OB * IB * 2u;
+    static constexpr uint32_t kStage = kDy + kX;  // dy (then dz) and x, until the MMAs have read them
+    static constexpr uint32_t kStages = OB + IB == 128u ? 4u : OB + IB == 192u ? 3u - (OB == 128u ? 1u : 0u) : 2u;
+    static constexpr uint32_t kPres = OB + IB == 128u ? 3u : OB + IB == 192u ? 2u : 1u;  // pre, until dz is made
+    static constexpr uint32_t kSmem = 1024u + kStages * kStage + kPres * kDy + kW + 8u * kSlabBytes;
+    static_assert(kSmem <= 232448u - 512u, "shared memory of one CTA");
+};
+constexpr uint32_t kThreads = 512;
+
+struct NarrowBarriers {
+    uint64_t full[4], empty[4], dz[4];
+    uint64_t pre_full[3], pre_empty[3];
+    uint64_t d1_full[2], d1_empty[2], d2_full[2], d2_empty[2];
+    uint64_t res[8];
+    uint64_t w_full, drain;
+    uint32_t tmem_base;
+};
+
+template <uint32_t OB, uint32_t IB, uint32_t ACT>
+__global__ void __launch_bounds__(kThreads, 1) k_backward_narrow(const NarrowArgs a, const __grid_constant__ NarrowMaps maps) {
+    using S = NarrowShape<OB, IB>;
+    constexpr uint32_t kCols = tmem_cols(4u * IB);
+    extern __shared__ unsigned char smem_raw[];
+    __shared__ NarrowBarriers bar;
+    unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+    unsigned char* pres = smem + S::kStages * S::kStage;
+    unsigned char* w_s = pres + S::kPres * S::kDy;
+    unsigned char* slabs = w_s + S::kW;
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
+    const bool bf16 = a.bf16 != 0u;
+    const uint32_t tiles = (a.n + kRowsTile - 1u) / kRowsTile;
+    const uint32_t mine = blockIdx.x < tiles ? (tiles - 1u - blockIdx.x) / gridDim.x + 1u : 0u;  // this CTA's tiles
+
+    if (threadIdx.x == 0u) {
+        for (uint32_t i = 0; i < S::kStages; ++i) {
+            umma::mbar_init(&bar.full[i], 1u);
+            umma::mbar_init(&bar.empty[i], 1u);
+            umma::mbar_init(&bar.dz[i], 4u);
+        }
+        for (uint32_t i = 0; i < S::kPres; ++i) {
+            umma::mbar_init(&bar.pre_full[i], 1u);
+            umma::mbar_init(&bar.pre_empty[i], 4u);
+        }
+        for (uint32_t i = 0; i < 2u; ++i) {
+            umma::mbar_init(&bar.d1_full[i], 1u);
+            umma::mbar_init(&bar.d1_empty[i], 4u);
+            umma::mbar_init(&bar.d2_full[i], 1u);
+            umma::mbar_init(&bar.d2_empty[i], 8u);
+        }
+        for (uint32_t i = 0; i < 8u; ++i) umma::mbar_init(&bar.res[i], 1u);
+        umma::mbar_init(&bar.w_full, 1u);
+        umma::mbar_init(&bar.drain, 1u);
+        umma::fence_mbar_init();
+    }
+    if (warp == 2u) {
+        umma::tmem_alloc(&bar.tmem_base, kCols);
+        umma::tmem_relinquish();
+    }
+    umma::fence_before_sync();
+    __syncthreads();
+    umma::fence_after_sync();
+    after_previous();
+    let_next_start();
+    const uint32_t tmem1 = bar.tmem_base, tmem2 = tmem1 + 2u * IB;  // dx and dW accumulators, two each
+
+    if (warp == 0u && lane == 0u) {
+        // ---- copies
+        tma::expect_tx(&bar.w_full, S::kW);
+        for (uint32_t j = 0; j < IB / 64u; ++j) tma::load_2d(smem_u32(w_s + j * OB * 128u), &maps.w, 64 * j, 0, &bar.w_full);
+        uint32_t i = 0;
+        bool ok = true;
+        for (; i < mine; ++i) {
+            const uint32_t s = i % S::kStages, p = i % S::kPres;
+            const int32_t row = static_cast<int32_t>((blockIdx.x + i * gridDim.x) * kRowsTile);
+            if (!tma::wait(&bar.empty[s], (i / S::kStages + 1u) & 1u) ||
+                (ACT != kActNone && !tma::wait(&bar.pre_empty[p], (i / S::kPres + 1u) & 1u))) {
+                ok = false;
+                break;
+            }
+            unsigned char* st = smem + s * S::kStage;
+            tma::expect_tx(&bar.full[s], S::kStage);
+            for (uint32_t j = 0; j < OB / 64u; ++j) tma::load_2d(smem_u32(st + j * kBoxBytes), &maps.dy, 64 * j, row, &bar.full[s]);
+            for (uint32_t j = 0; j < IB / 64u; ++j) tma::load_2d(smem_u32(st + S::kDy + j * kBoxBytes), &maps.x, 64 * j, row, &bar.full[s]);
+            if (ACT != kActNone) {
+                tma::expect_tx(&bar.pre_full[p], S::kDy);
+                for (uint32_t j = 0; j < OB / 64u; ++j)
+                    tma::load_2d(smem_u32(pres + p * S::kDy + j * kBoxBytes), &maps.pre, 64 * j, row, &bar.pre_full[p]);
+            }
+        }
+        if (!ok) {  // copies in flight: wait for them before the shared memory goes
+            atomicOr(a.error, 1u);
+            tma::wait(&bar.w_full, 0u);
+            for (uint32_t k = i > S::kStages ? i - S::kStages : 0u; k < i; ++k) tma::wait(&bar.full[k % S::kStages], (k / S::kStages) & 1u);
+            if (ACT != kActNone)
+                for (uint32_t k = i > S::kPres ? i - S::kPres : 0u; k < i; ++k) tma::wait(&bar.pre_full[k % S::kPres], (k / S::kPres) & 1u);
+        }
+    } else if (warp == 1u && lane == 0u) {
+        // ---- MMA issuer
+        const uint32_t id1 = tma::idesc_16bit(128u, IB, 0u, 1u, a.bf16), id2 = tma::idesc_16bit(128u, IB, 1u, 1u, a.bf16);
+        const uint32_t w_at = smem_u32(w_s);
+        bool ok = tma::wait(&bar.w_full, 0u);
+        for (uint32_t i = 0; i < mine && ok; ++i) {
+            const uint32_t s = i % S::kStages, b = i & 1u, c = i / kChunkTiles;
+            const bool first = i % kChunkTiles == 0u, last = i % kChunkTiles == kChunkTiles - 1u || i + 1u == mine;
+            if (!tma::wait(&bar.full[s], (i / S::kStages) & 1u) || !tma::wait(&bar.dz[s], (i / S::kStages) & 1u) ||
+                !tma::wait(&bar.d1_empty[b], (i / 2u + 1u) & 1u) || (first && !tma::wait(&bar.d2_empty[c & 1u], (c / 2u + 1u) & 1u))) {
+                ok = false;
+                break;
+            }
+            umma::fence_after_sync();
+            const uint32_t dz = smem_u32(smem + s * S::kStage), x = dz + S::kDy;
+#pragma unroll
+            for (uint32_t k = 0; k < OB / 16u; ++k)  // dx: K = n_out
+                umma::mma_f16(tmem1 + b * IB, tma::desc_sw128(dz + (k >> 2) * kBoxBytes + 32u * (k & 3u), 16u, 1024u),
+                              tma::desc_sw128(w_at + 2048u * k, OB * 128u, 1024u), id1, k > 0u ? 1u : 0u);
+            umma::commit(&bar.d1_full[b]);
+#pragma unroll
+            for (uint32_t k = 0; k < kRowsTile / 16u; ++k)
+                // dW: K = rows.  With 64 output columns the accumulator's lanes 64.. hold products of the x boxes that
+                // follow dz in the stage; nothing reads them.
+                umma::mma_f16(tmem2 + (c & 1u) * IB, tma::desc_sw128(dz + 2048u * k, kBoxBytes, 1024u),
+                              tma::desc_sw128(x + 2048u * k, kBoxBytes, 1024u), id2, !first || k > 0u ? 1u : 0u);
+            if (last) umma::commit(&bar.d2_full[c & 1u]);
+            umma::commit(&bar.empty[s]);
+        }
+        if (!ok) {
+            atomicOr(a.error, 1u);
+            umma::commit(&bar.drain);
+            tma::wait(&bar.drain, 0u);
+        }
+    } else if (warp >= 4u && warp < 8u) {
+        // ---- dz in place of dy; a thread keeps to one 8-column piece
+        constexpr uint32_t kPieces = OB / 8u, kStep = 128u / kPieces;
+        const uint32_t t = threadIdx.x - 128u, p = t % kPieces, r0 = t / kPieces, box = (p >> 3) * kBoxBytes;
+        float sums[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        bool ok = true;
+        for (uint32_t i = 0; i < mine; ++i) {
+            const uint32_t s = i % S::kStages, ps = i % S::kPres;
+            ok = tma::wait(&bar.full[s], (i / S::kStages) & 1u) && (ACT == kActNone || tma::wait(&bar.pre_full[ps], (i / S::kPres) & 1u));
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) {
+                atomicOr(a.error, 1u);
+                break;
+            }
+            unsigned char* d = smem + s * S::kStage + box;
+            const unsigned char* z = pres + ps * S::kDy + box;
+#pragma unroll 4
+            for (uint32_t k = 0; k < kRowsTile / kStep; ++k) {
+                const uint32_t at = slab_at(r0 + k * kStep, p & 7u);
+                const uint4 ud = *reinterpret_cast<const uint4*>(d + at);
+                const uint4 uz = ACT != kActNone ? *reinterpret_cast<const uint4*>(z + at) : make_uint4(0u, 0u, 0u, 0u);
+                const uint32_t dw[4] = {ud.x, ud.y, ud.z, ud.w}, zw[4] = {uz.x, uz.y, uz.z, uz.w};
+                uint32_t o[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const float2 dd = unpack_16(dw[j], bf16), zz = unpack_16(zw[j], bf16);
+                    const float f0 = dact_f(dd.x, zz.x, ACT), f1 = dact_f(dd.y, zz.y, ACT);
+                    sums[2 * j] += f0;
+                    sums[2 * j + 1] += f1;
+                    o[j] = pack_16(f0, f1, bf16);  // the tensor cores take 16-bit operands
+                }
+                if (ACT != kActNone) *reinterpret_cast<uint4*>(d + at) = make_uint4(o[0], o[1], o[2], o[3]);
+            }
+            umma::fence_async_smem();
+            __syncwarp();
+            if (lane == 0u) {
+                tma::arrive(&bar.dz[s]);
+                if (ACT != kActNone) tma::arrive(&bar.pre_empty[ps]);
+            }
+        }
+        if (a.db_part) {
+            // A column's sums over the threads that kept to its piece, through the room of pre.  Every warp comes to
+            // both barriers, also one whose wait ran out.
+            float* acc = reinterpret_cast<float*>(pres);
+            asm volatile("bar.sync 1, 128;\n" ::: "memory");
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (ok) acc[t * 9u + j] = sums[j];
+            asm volatile("bar.sync 1, 128;\n" ::: "memory");
+            for (uint32_t c = t; c < a.n_out && ok; c += 128u) {
+                float v = 0.0f;
+                for (uint32_t k = 0; k < kStep; ++k) v += acc[(k * kPieces + (c >> 3)) * 9u + (c & 7u)];
+                a.db_part[static_cast<uint64_t>(blockIdx.x) * a.n_out + c] = v;
+            }
+        }
+    } else if (warp >= 8u) {
+        // ---- epilogue: group h takes every other tile's dx, and half of the columns of every dW chunk
+        constexpr uint32_t kHalf = IB / 2u;
+        const uint32_t q = warp & 3u, h = (warp >> 2) - 2u, row = 32u * q + lane, lane_base = (32u * q) << 16;
+        unsigned char* slab = slabs + (warp - 8u) * kSlabBytes;
+        float s[kHalf];
+#pragma unroll
+        for (uint32_t i = 0; i < kHalf; ++i) s[i] = 0.0f;
+        uint32_t res_parity = 0;
+        bool ok = true;
+        for (uint32_t i = 0; i < mine && ok; ++i) {
+            if ((i & 1u) == h) {
+                const uint32_t m0 = (blockIdx.x + i * gridDim.x) * kRowsTile + 32u * q;
+                const uint32_t rows = m0 < a.n ? min(32u, a.n - m0) : 0u;
+                ok = __all_sync(0xffffffffu, tma::wait(&bar.d1_full[h], (i / 2u) & 1u));
+                if (!ok) break;
+                umma::fence_after_sync();
+                for (uint32_t c0 = 0; c0 < IB && c0 < a.n_in; c0 += 64u) {
+                    const uint32_t cols = min(64u, a.n_in - c0);
+                    if (lane == 0u) {
+                        tma::store_wait_read<0>();
+                        if (a.res_tma && rows) {
+                            tma::expect_tx(&bar.res[warp - 8u], kSlabBytes);
+                            tma::load_2d(smem_u32(slab), &maps.res, c0, m0, &bar.res[warp - 8u]);
+                        }
+                    }
+                    __syncwarp();
+                    if (a.res.ptr && !a.res_tma) {
+                        unsigned char* src = static_cast<unsigned char*>(const_cast<void*>(a.res.ptr)) + 2u * (m0 * a.res.ld + c0);
+                        slab_copy<2, false>(slab, src, a.res.ld, rows, cols, a.res.vec >= 8u, lane);
+                        __syncwarp();
+                    }
+                    if (a.res_tma && rows) {
+                        if (!tma::wait(&bar.res[warp - 8u], res_parity)) atomicOr(a.error, 1u);
+                        res_parity ^= 1u;
+                        __syncwarp();
+                    }
+#pragma unroll
+                    for (uint32_t g = 0; g < 2u; ++g) {
+                        float v[32];
+                        umma::tmem_ld32(tmem1 + h * IB + c0 + 32u * g + lane_base, v);
+                        if (a.res.ptr) {
+#pragma unroll
+                            for (uint32_t p = 0; p < 4u; ++p) {
+                                const uint4 u = *reinterpret_cast<const uint4*>(slab + slab_at(lane, 4u * g + p));
+                                const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+                                for (int j = 0; j < 4; ++j) {
+                                    const float2 f = unpack_16(w[j], bf16);
+                                    v[8 * p + 2 * j] += f.x;
+                                    v[8 * p + 2 * j + 1] += f.y;
+                                }
+                            }
+                        }
+                        slab_put32(slab, lane, g, v, bf16);
+                    }
+                    slab_out(slab, a.dx, a.dx_tma != 0u, &maps.dx, m0, c0, rows, cols, lane);
+                }
+                umma::fence_before_sync();
+                __syncwarp();
+                if (lane == 0u) tma::arrive(&bar.d1_empty[h]);
+            }
+            if (i % kChunkTiles == kChunkTiles - 1u || i + 1u == mine) {
+                const uint32_t c = i / kChunkTiles;
+                ok = __all_sync(0xffffffffu, tma::wait(&bar.d2_full[c & 1u], (c / 2u) & 1u));
+                if (!ok) break;
+                umma::fence_after_sync();
+#pragma unroll
+                for (uint32_t k = 0; k < kHalf; k += 32u) {
+                    float v[32];
+                    umma::tmem_ld32(tmem2 + (c & 1u) * IB + h * kHalf + k + lane_base, v);
+#pragma unroll
+                    for (uint32_t j = 0; j < 32u; ++j) s[k + j] += v[j];
+                }
+                umma::fence_before_sync();
+                __syncwarp();
+                if (lane == 0u) tma::arrive(&bar.d2_empty[c & 1u]);
+            }
+        }
+        if (!ok) atomicOr(a.error, 1u);
+        if (row < OB) {
+            float4* dst = reinterpret_cast<float4*>(a.partials) + (static_cast<uint64_t>(blockIdx.x) * (IB / 4u) + h * (kHalf / 4u)) * 128u + row;
+#pragma unroll
+            for (uint32_t k = 0; k < kHalf / 4u; ++k) dst[k * 128u] = make_float4(s[4 * k], s[4 * k + 1], s[4 * k + 2], s[4 * k + 3]);
+        }
+        if (lane == 0u) tma::store_wait_all();
+    }
+    __syncwarp();
+    umma::fence_before_sync();
+    __syncthreads();
+    if (warp == 2u) umma::tmem_dealloc(tmem1, kCols);
+}
+
+template <uint32_t OB, uint32_t IB, uint32_t ACT>
+cudaError_t launch_t(const NarrowArgs& a, const NarrowMaps& maps, uint32_t blocks, cudaStream_t s) {
+    constexpr uint32_t smem = NarrowShape<OB, IB>::kSmem;
+    static std::atomic<bool> done[64];  // the attribute belongs to the device
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+    if (!done[dev]) {
+        e = cudaFuncSetAttribute(k_backward_narrow<OB, IB, ACT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        if (e != cudaSuccess) return e;
+        done[dev] = true;
+    }
+    return launch_after(k_backward_narrow<OB, IB, ACT>, dim3(blocks), kThreads, smem, 1u, s, a, maps);
+}
+template <uint32_t OB, uint32_t IB>
+cudaError_t launch_act(const NarrowArgs& a, const NarrowMaps& maps, uint32_t blocks, cudaStream_t s) {
+    switch (a.act) {
+        case kActRelu: return launch_t<OB, IB, kActRelu>(a, maps, blocks, s);
+        case kActSilu: return launch_t<OB, IB, kActSilu>(a, maps, blocks, s);
+        case kActGelu: return launch_t<OB, IB, kActGelu>(a, maps, blocks, s);
+        case kActSigmoid: return launch_t<OB, IB, kActSigmoid>(a, maps, blocks, s);
+        default: return launch_t<OB, IB, kActNone>(a, maps, blocks, s);
+    }
+}
+
+}  // namespace
+
+cudaError_t launch_backward_narrow(const NarrowArgs& a, const NarrowMaps& maps, uint32_t blocks, cudaStream_t s) {
+    if (a.n == 0u || a.n_in == 0u || a.n_out == 0u || a.n_in > 128u || a.n_out > 128u) return cudaErrorInvalidValue;
+    if (a.n_out <= 64u) return a.n_in <= 64u ? launch_act<64u, 64u>(a, maps, blocks, s) : launch_act<64u, 128u>(a, maps, blocks, s);
+    return a.n_in <= 64u ? launch_act<128u, 64u>(a, maps, blocks, s) : launch_act<128u, 128u>(a, maps, blocks, s);
+}
+
+}  // namespace nb
