@@ -103,8 +103,8 @@ NB_DEV void fill_box(unsigned char* box, const MatrixView& m, uint32_t row0, uin
 // ------------------------------------------------------------------ the GEMM
 struct Barriers {
     uint64_t full[kMaxStages], empty[kMaxStages];
-    uint64_t acc_full[2], acc_empty[2];
-    uint64_t res[8];  // an epilogue warp's residual rows have arrived
+    uint64_t acc_full[4], acc_empty[4];
+    uint64_t res[16];  // an epilogue warp's residual rows have arrived
     uint64_t drain;
     uint32_t tmem_base;
 };
@@ -123,10 +123,14 @@ struct GemmShape {
     static constexpr bool kPair = FEED == kFeedPair, kPlain = FEED == kFeedPlain;
     static constexpr uint32_t kBoxN = kPair ? BN / 2u : BN;  // rows of B in this CTA's shared memory
     static constexpr uint32_t kStageBytes = kStageBytesA + kBoxN * 128u;
-    static constexpr uint32_t kStages = kPlain ? 2u : kPair ? 5u : BN >= 256u ? 3u : BN >= 128u ? 4u : 5u;
-    static constexpr uint32_t kSlabs = kPlain ? 1u : 2u;  // per epilogue warp
-    static constexpr uint32_t kSmem = 1024u + kStages * kStageBytes + 8u * kSlabs * kSlabBytes + 2u * BN * 2u;
-    static constexpr uint32_t kThreads = kPlain ? 384u + 32u * kLoadWarps : 384u;
+    // Epilogue groups of four warps, an accumulator each: tiles of up to 128
+    // columns are bound by memory and by the latency of their epilogues.
+    static constexpr uint32_t kGroups = KIND == kGemmRows && BN <= 128u && !kPlain ? 4u : 2u;
+    static constexpr uint32_t kStages = kPlain ? 2u : kPair ? 5u : BN >= 128u ? 3u : 4u;
+    static constexpr uint32_t kSlabs = 2u;  // per epilogue warp
+    static constexpr uint32_t kSmem = 1024u + kStages * kStageBytes + 4u * kGroups * kSlabs * kSlabBytes + kGroups * BN * 2u;
+    static constexpr uint32_t kFirstLoader = 4u + 4u * kGroups;
+    static constexpr uint32_t kThreads = 32u * (kFirstLoader + (kPlain ? kLoadWarps : 0u));
     // Weight gradients of 256 columns keep 128 sums a thread: registers move
     // from the copying and issuing warps to the two groups that sum.
     static constexpr bool kRegs = KIND == kGemmGrad && BN == 256u && !kPlain;
@@ -135,20 +139,20 @@ struct GemmShape {
     static_assert(kSmem <= 232448u - 512u, "shared memory of one CTA");
 };
 
-// Warps: 0 operand copies, 1 MMA, 2 tensor-memory allocation, 4-7 and 8-11 two
-// epilogue groups that take turns (item i of the CTA: group and accumulator
-// i & 1), 12.. operand loads (kFeedPlain).
+// Warps: 0 operand copies, 1 MMA, 2 tensor-memory allocation, from 4 on the
+// epilogue groups of four, which take turns (item i of the CTA: group and
+// accumulator i % kGroups), then the operand loads (kFeedPlain).
 template <uint32_t BN, int KIND, int FEED>
 __global__ void __launch_bounds__(GemmShape<BN, KIND, FEED>::kThreads, 1) k_gemm(const GemmArgs g, const __grid_constant__ GemmMaps maps) {
     using S = GemmShape<BN, KIND, FEED>;
     constexpr uint32_t kStages = S::kStages, kStageBytes = S::kStageBytes;
-    constexpr uint32_t kCols = tmem_cols(2u * BN);
+    constexpr uint32_t kCols = tmem_cols(S::kGroups * BN);
     constexpr uint32_t kCtas = S::kPair ? 2u : 1u;
     extern __shared__ unsigned char smem_raw[];
     __shared__ Barriers bar;
     unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     unsigned char* slabs = smem + kStages * kStageBytes;
-    uint16_t* bias_all = reinterpret_cast<uint16_t*>(slabs + 8u * S::kSlabs * kSlabBytes);
+    uint16_t* bias_all = reinterpret_cast<uint16_t*>(slabs + 4u * S::kGroups * S::kSlabs * kSlabBytes);
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
     const bool bf16 = g.bf16 != 0u;
     const uint32_t rank = S::kPair ? tma::cluster_rank() : 0u;
@@ -159,11 +163,11 @@ __global__ void __launch_bounds__(GemmShape<BN, KIND, FEED>::kThreads, 1) k_gemm
             umma::mbar_init(&bar.full[i], S::kPlain ? 32u * kLoadWarps : 1u);
             umma::mbar_init(&bar.empty[i], 1u);
         }
-        for (uint32_t i = 0; i < 2u; ++i) {
+        for (uint32_t i = 0; i < S::kGroups; ++i) {
             umma::mbar_init(&bar.acc_full[i], 1u);
             umma::mbar_init(&bar.acc_empty[i], (KIND == kGemmGrad ? 8u : 4u) * kCtas);
         }
-        for (uint32_t i = 0; i < 8u; ++i) umma::mbar_init(&bar.res[i], 1u);
+        for (uint32_t i = 0; i < 4u * S::kGroups; ++i) umma::mbar_init(&bar.res[i], 1u);
         umma::mbar_init(&bar.drain, 1u);
         umma::fence_mbar_init();
         if (!S::kPlain) {
@@ -191,7 +195,7 @@ __global__ void __launch_bounds__(GemmShape<BN, KIND, FEED>::kThreads, 1) k_gemm
     const uint32_t tiles = g.tiles_m * g.tiles_n, items = tiles * g.splits;
     if (S::kRegs && warp < 4u) tma::registers_down<S::kRegsDown>();
 
-    if ((!S::kPlain && warp == 0u && lane == 0u) || (S::kPlain && warp >= 12u)) {
+    if ((!S::kPlain && warp == 0u && lane == 0u) || (S::kPlain && warp >= S::kFirstLoader)) {
         // ---- producer: one thread issuing tensor copies, or warps of loads
         uint32_t stage = 0, parity = 1u, issued = 0;
         bool ok = true;
@@ -210,7 +214,7 @@ __global__ void __launch_bounds__(GemmShape<BN, KIND, FEED>::kThreads, 1) k_gemm
                 unsigned char* sb = sa + kStageBytesA;
                 const uint32_t k0 = ks * kBK;
                 if (S::kPlain) {
-                    const uint32_t tid = threadIdx.x - 384u;
+                    const uint32_t tid = threadIdx.x - 32u * S::kFirstLoader;
                     if (g.a_mn) {
                         for (uint32_t j = 0; j < kBM / 64u; ++j) fill_box<kBK>(sa + j * 8192u, g.a, k0, m0 + 64u * j, tid);
                     } else {
@@ -297,7 +301,7 @@ __global__ void __launch_bounds__(GemmShape<BN, KIND, FEED>::kThreads, 1) k_gemm
                 if (S::kPair) tma::commit_pair(&bar.acc_full[acc]);
                 else umma::commit(&bar.acc_full[acc]);
             }
-            acc ^= 1u;
+            acc = acc + 1u == S::kGroups ? 0u : acc + 1u;
             if (acc == 0u) acc_parity ^= 1u;
             }
         }
@@ -403,7 +407,7 @@ __global__ void __launch_bounds__(GemmShape<BN, KIND, FEED>::kThreads, 1) k_gemm
                 __syncwarp();
             }
         }
-    } else if (KIND == kGemmRows && warp >= 4u && warp < 12u) {
+    } else if (KIND == kGemmRows && warp >= 4u && warp < S::kFirstLoader) {
         // ---- epilogue: warp q of a group drains rows 32 q .. 32 q + 31 of the tile
         const uint32_t q = warp & 3u, acc = (warp >> 2) - 1u;
         unsigned char* my_slabs = slabs + (warp - 4u) * S::kSlabs * kSlabBytes;
@@ -412,15 +416,18 @@ __global__ void __launch_bounds__(GemmShape<BN, KIND, FEED>::kThreads, 1) k_gemm
         const uint32_t acc_empty = S::kPair ? tma::peer_addr(smem_u32(&bar.acc_empty[acc]), 0u) : 0u;
         uint32_t parity = 0, res_parity = 0, slab_i = 0, bias_n = ~0u;
         bool ok = true;  // after a wait that ran out the warp only keeps the named barriers' count
-        // A slab that no store of this warp still reads.
-        const auto next_slab = [&]() -> unsigned char* {
-            if (lane == 0u) tma::store_wait_read<S::kSlabs - 1u>();
+        // The next slab, when no store of this warp still reads it (ahead: slabs taken since the last store).
+        const auto next_slab = [&](uint32_t ahead) -> unsigned char* {
+            if (lane == 0u) {
+                if (ahead) tma::store_wait_read<S::kSlabs - 2u>();
+                else tma::store_wait_read<S::kSlabs - 1u>();
+            }
             __syncwarp();
             unsigned char* p = my_slabs + slab_i * kSlabBytes;
-            if (S::kSlabs > 1u) slab_i ^= 1u;
+            slab_i = slab_i + 1u == S::kSlabs ? 0u : slab_i + 1u;
             return p;
         };
-        for (uint32_t it = first_item + acc * item_step; it < items; it += 2u * item_step) {
+        for (uint32_t it = first_item + acc * item_step; it < items; it += S::kGroups * item_step) {
             const uint32_t split = it / tiles, tile = it - split * tiles;
             uint32_t tm, tn;
             tile_of(g, tile, tm, tn);
@@ -436,7 +443,7 @@ __global__ void __launch_bounds__(GemmShape<BN, KIND, FEED>::kThreads, 1) k_gemm
             if (g.res_tma && lane == 0u) {
                 // The residual of this group's next tile (and of its first) on its way to the L2 cache.
                 for (uint32_t w = it == first_item + acc * item_step ? 0u : 1u; w < 2u; ++w) {
-                    const uint32_t jt = it + 2u * w * item_step;
+                    const uint32_t jt = it + S::kGroups * w * item_step;
                     if (jt >= items) break;
                     uint32_t jm, jn;
                     tile_of(g, jt, jm, jn);
@@ -452,68 +459,38 @@ __global__ void __launch_bounds__(GemmShape<BN, KIND, FEED>::kThreads, 1) k_gemm
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) continue;
             umma::fence_after_sync();
-            {
-                for (uint32_t c0 = 0; c0 < BN && n0 + c0 < g.N; c0 += 64u) {
-                    const uint32_t cols = min(64u, g.N - n0 - c0);
-                    // The residual's rows come straight into the slab of the output, where this thread's
-                    // row replaces them; the copy runs while z is made.
-                    unsigned char* slab = nullptr;
-                    if (S::kSlabs > 1u || !g.pre.ptr) {
-                        slab = next_slab();
-                        if (g.res_tma && rows && lane == 0u) {
-                            tma::expect_tx(&bar.res[warp - 4u], kSlabBytes);
-                            tma::load_2d(smem_u32(slab), &maps.res, static_cast<int32_t>(n0 + c0), static_cast<int32_t>(m0), &bar.res[warp - 4u]);
-                        }
-                    }
-                    if (g.pre.ptr) {
-                        unsigned char* slab_z = next_slab();
+#pragma unroll 1
+            for (uint32_t c0 = 0; c0 < BN && n0 + c0 < g.N; c0 += 64u) {
+                const uint32_t cols = min(64u, g.N - n0 - c0);
+                unsigned char* slab_z = g.pre.ptr ? next_slab(0u) : nullptr;
+                unsigned char* slab = next_slab(g.pre.ptr ? 1u : 0u);
+                // The residual's rows come straight into the slab of the output, where this thread's row replaces
+                // them; the copy runs while z is made.
+                if (g.res_tma && rows && lane == 0u) {
+                    tma::expect_tx(&bar.res[warp - 4u], kSlabBytes);
+                    tma::load_2d(smem_u32(slab), &maps.res, static_cast<int32_t>(n0 + c0), static_cast<int32_t>(m0), &bar.res[warp - 4u]);
+                }
+                if (g.res.ptr && !g.res_tma) {
+                    unsigned char* src = static_cast<unsigned char*>(const_cast<void*>(g.res.ptr)) + 2u * (m0 * g.res.ld + n0 + c0);
+                    slab_copy<2, false>(slab, src, g.res.ld, rows, cols, g.res.vec >= 8u, lane);
+                    __syncwarp();
+                }
 #pragma unroll
-                        for (uint32_t h = 0; h < 2u; ++h) {
-                            float v[32];
-                            load_z(v, taddr + c0 + 32u * h, bias_s + c0 + 32u * h, bf16);
-                            slab_put32(slab_z, lane, h, v, bf16);
-                        }
-                        slab_out(slab_z, g.pre, g.pre_tma != 0u, &maps.pre, m0, n0 + c0, rows, cols, lane);
-                        if (S::kSlabs == 1u) {
-                            slab = next_slab();
-                            if (g.res_tma && rows && lane == 0u) {
-                                tma::expect_tx(&bar.res[warp - 4u], kSlabBytes);
-                                tma::load_2d(smem_u32(slab), &maps.res, static_cast<int32_t>(n0 + c0), static_cast<int32_t>(m0), &bar.res[warp - 4u]);
-                            }
-                        }
-                    }
-                    if (g.res.ptr && !g.res_tma) {
-                        unsigned char* src = static_cast<unsigned char*>(const_cast<void*>(g.res.ptr)) + 2u * (m0 * g.res.ld + n0 + c0);
-                        slab_copy<2, false>(slab, src, g.res.ld, rows, cols, g.res.vec >= 8u, lane);
+                for (uint32_t h = 0; h < 2u; ++h) {
+                    float v[32];
+                    load_z(v, taddr + c0 + 32u * h, bias_s + c0 + 32u * h, bf16);
+                    if (g.pre.ptr) slab_put32(slab_z, lane, h, v, bf16);
+                    act_row(v, g.act);
+                    if (h == 0u && g.res_tma && rows) {
+                        if (!tma::wait(&bar.res[warp - 4u], res_parity)) atomicOr(g.error, 1u);
+                        res_parity ^= 1u;
                         __syncwarp();
                     }
-#pragma unroll
-                    for (uint32_t h = 0; h < 2u; ++h) {
-                        float v[32];
-                        load_z(v, taddr + c0 + 32u * h, bias_s + c0 + 32u * h, bf16);
-                        act_row(v, g.act);
-                        if (h == 0u && g.res_tma && rows) {
-                            if (!tma::wait(&bar.res[warp - 4u], res_parity)) atomicOr(g.error, 1u);
-                            res_parity ^= 1u;
-                            __syncwarp();
-                        }
-                        if (g.res.ptr) {
-#pragma unroll
-                            for (uint32_t p = 0; p < 4u; ++p) {
-                                const uint4 u = *reinterpret_cast<const uint4*>(slab + slab_at(lane, 4u * h + p));
-                                const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-                                for (int i = 0; i < 4; ++i) {
-                                    const float2 f = unpack_16(w[i], bf16);
-                                    v[8 * p + 2 * i] += f.x;
-                                    v[8 * p + 2 * i + 1] += f.y;
-                                }
-                            }
-                        }
-                        slab_put32(slab, lane, h, v, bf16);
-                    }
-                    slab_out(slab, g.y, g.y_tma != 0u, &maps.y, m0, n0 + c0, rows, cols, lane);
+                    if (g.res.ptr) slab_add32(slab, lane, h, v, bf16);
+                    slab_put32(slab, lane, h, v, bf16);
                 }
+                if (g.pre.ptr) slab_out(slab_z, g.pre, g.pre_tma != 0u, &maps.pre, m0, n0 + c0, rows, cols, lane);
+                slab_out(slab, g.y, g.y_tma != 0u, &maps.y, m0, n0 + c0, rows, cols, lane);
             }
             umma::fence_before_sync();
             __syncwarp();

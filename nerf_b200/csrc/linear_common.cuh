@@ -231,7 +231,8 @@ NB_DEV void load_z(float (&v)[32], uint32_t taddr, const uint16_t* bias, bool bf
         }
     }
 }
-// 32 values -> pieces 4 h .. 4 h + 3 of this thread's slab row.
+// 32 values -> pieces 4 h .. 4 h + 3 of this thread's slab row, and the row's
+// values added to v.
 NB_DEV void slab_put32(unsigned char* slab, uint32_t lane, uint32_t h, const float (&v)[32], bool bf16) {
 #pragma unroll
     for (uint32_t p = 0; p < 4u; ++p) {
@@ -239,6 +240,19 @@ NB_DEV void slab_put32(unsigned char* slab, uint32_t lane, uint32_t h, const flo
 #pragma unroll
         for (int i = 0; i < 4; ++i) w[i] = pack_16(v[8 * p + 2 * i], v[8 * p + 2 * i + 1], bf16);
         slab_put(slab, lane, 4u * h + p, w);
+    }
+}
+NB_DEV void slab_add32(const unsigned char* slab, uint32_t lane, uint32_t h, float (&v)[32], bool bf16) {
+#pragma unroll
+    for (uint32_t p = 0; p < 4u; ++p) {
+        const uint4 u = *reinterpret_cast<const uint4*>(slab + slab_at(lane, 4u * h + p));
+        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float2 f = unpack_16(w[i], bf16);
+            v[8 * p + 2 * i] += f.x;
+            v[8 * p + 2 * i + 1] += f.y;
+        }
     }
 }
 

@@ -231,6 +231,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_backward_narrow(const NarrowArg
                 ok = __all_sync(0xffffffffu, tma::wait(&bar.d1_full[h], (i / 2u) & 1u));
                 if (!ok) break;
                 umma::fence_after_sync();
+#pragma unroll 1
                 for (uint32_t c0 = 0; c0 < IB && c0 < a.n_in; c0 += 64u) {
                     const uint32_t cols = min(64u, a.n_in - c0);
                     if (lane == 0u) {
@@ -255,19 +256,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_backward_narrow(const NarrowArg
                     for (uint32_t g = 0; g < 2u; ++g) {
                         float v[32];
                         umma::tmem_ld32(tmem1 + h * IB + c0 + 32u * g + lane_base, v);
-                        if (a.res.ptr) {
-#pragma unroll
-                            for (uint32_t p = 0; p < 4u; ++p) {
-                                const uint4 u = *reinterpret_cast<const uint4*>(slab + slab_at(lane, 4u * g + p));
-                                const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-                                for (int j = 0; j < 4; ++j) {
-                                    const float2 f = unpack_16(w[j], bf16);
-                                    v[8 * p + 2 * j] += f.x;
-                                    v[8 * p + 2 * j + 1] += f.y;
-                                }
-                            }
-                        }
+                        if (a.res.ptr) slab_add32(slab, lane, g, v, bf16);
                         slab_put32(slab, lane, g, v, bf16);
                     }
                     slab_out(slab, a.dx, a.dx_tma != 0u, &maps.dx, m0, c0, rows, cols, lane);
