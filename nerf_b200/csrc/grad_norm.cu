@@ -223,25 +223,40 @@ NB_DEV void store_one(void* p, uint64_t i, float v) {
     else if (OUT == NERF_B200_F16) static_cast<__half*>(p)[i] = __float2half_rn(v);
     else static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
 }
+// A lane's load is as wide as makes its store 16 bytes: 8 bytes of 16-bit
+// gradients that become fp32, else 16.
 template <uint32_t TYPE, uint32_t OUT>
 NB_DEV void chunk_scale(const GradEntry& e, uint64_t e0, uint64_t e1, float scale) {
-    constexpr uint32_t V = Vec<TYPE>::kN, B = Vec<TYPE>::kBytes, OB = OUT == NERF_B200_F32 ? 4u : 2u;
+    constexpr uint32_t B = Vec<TYPE>::kBytes, OB = OUT == NERF_B200_F32 ? 4u : 2u;
+    constexpr uint32_t V = 16u / OB, kLoad = V * B, kDeep = kFlight * 16u / kLoad;  // values and bytes a load, loads in flight
     const uint64_t addr = reinterpret_cast<uint64_t>(e.g) + e0 * B;
-    const uint32_t n = static_cast<uint32_t>(e1 - e0), head = min(n, ((16u - (static_cast<uint32_t>(addr) & 15u)) & 15u) / B);
+    const uint32_t n = static_cast<uint32_t>(e1 - e0), head = min(n, ((kLoad - (static_cast<uint32_t>(addr) & (kLoad - 1u))) & (kLoad - 1u)) / B);
     const uint32_t n_vec = (n - head) / V, tail0 = head + n_vec * V;
-    const uint4* q = reinterpret_cast<const uint4*>(addr + head * B);
+    const unsigned char* q = reinterpret_cast<const unsigned char*>(addr + head * B);
     unsigned char* o = static_cast<unsigned char*>(e.out) + (e0 + head) * OB;
     const bool wide = (reinterpret_cast<uint64_t>(o) & 15u) == 0u;
     const uint32_t t = threadIdx.x;
-    for (uint32_t i = t; i < n_vec; i += kFlight * kThreads) {
-        uint4 u[kFlight];
+    for (uint32_t i = t; i < n_vec; i += kDeep * kThreads) {
+        uint4 u[kDeep];
 #pragma unroll
-        for (uint32_t j = 0; j < kFlight; ++j) u[j] = i + j * kThreads < n_vec ? __ldcs(q + i + j * kThreads) : make_uint4(0u, 0u, 0u, 0u);
+        for (uint32_t j = 0; j < kDeep; ++j) {
+            const uint32_t at = i + j * kThreads;
+            u[j] = make_uint4(0u, 0u, 0u, 0u);
+            if (at < n_vec) {
+                if (kLoad == 16u) {
+                    u[j] = __ldcs(reinterpret_cast<const uint4*>(q) + at);
+                } else {
+                    const uint2 d = __ldcs(reinterpret_cast<const uint2*>(q) + at);
+                    u[j].x = d.x;
+                    u[j].y = d.y;
+                }
+            }
+        }
 #pragma unroll
-        for (uint32_t j = 0; j < kFlight; ++j) {
+        for (uint32_t j = 0; j < kDeep; ++j) {
             const uint32_t at = i + j * kThreads;
             if (at >= n_vec) break;
-            float v[V];
+            float v[8];
             Vec<TYPE>::unpack(u[j], v);
 #pragma unroll
             for (uint32_t k = 0; k < V; ++k) v[k] *= scale;
@@ -249,14 +264,11 @@ NB_DEV void chunk_scale(const GradEntry& e, uint64_t e0, uint64_t e1, float scal
 #pragma unroll
                 for (uint32_t k = 0; k < V; ++k) store_one<OUT>(o, at * V + k, v[k]);
             } else if (OUT == NERF_B200_F32) {
-                float4* d = reinterpret_cast<float4*>(o) + at * (V / 4u);
-#pragma unroll
-                for (uint32_t k = 0; k < V / 4u; ++k) __stcs(d + k, make_float4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]));
-            } else if (V == 8u) {
+                __stcs(reinterpret_cast<float4*>(o) + at, make_float4(v[0], v[1], v[2], v[3]));
+            } else {
                 uint32_t w[4];
 #pragma unroll
-                for (int k = 0; k < 4; ++k)
-                    w[k] = OUT == NERF_B200_F16 ? pack_h2(v[(2 * k) % V], v[(2 * k + 1) % V]) : pack_bf(v[(2 * k) % V], v[(2 * k + 1) % V]);
+                for (int k = 0; k < 4; ++k) w[k] = OUT == NERF_B200_F16 ? pack_h2(v[2 * k], v[2 * k + 1]) : pack_bf(v[2 * k], v[2 * k + 1]);
                 __stcs(reinterpret_cast<uint4*>(o) + at, make_uint4(w[0], w[1], w[2], w[3]));
             }
         }

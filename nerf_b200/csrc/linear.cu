@@ -316,7 +316,8 @@ __global__ void __launch_bounds__(GemmShape<BN, KIND, FEED>::kThreads, 1) k_gemm
         // h BN / 2 .. in registers, rows 32 q .. 32 q + 31 of the tile a warp
         constexpr uint32_t kHalf = BN / 2u;
         const uint32_t q = warp & 3u, h = (warp >> 2) - 1u, row = 32u * q + lane;
-        unsigned char* slab = slabs + (warp - 4u) * S::kSlabs * kSlabBytes;
+        unsigned char* my_slabs = slabs + (warp - 4u) * S::kSlabs * kSlabBytes;
+        uint32_t slab_i = 0;
         if (S::kRegs) tma::registers_up<S::kRegsUp>();
         uint32_t acc = 0, parity = 0;
         bool ok = true;
@@ -364,49 +365,78 @@ __global__ void __launch_bounds__(GemmShape<BN, KIND, FEED>::kThreads, 1) k_gemm
                     if (n0 + 4u * i < g.N) dst[i * kBM] = make_float4(s[4 * i], s[4 * i + 1], s[4 * i + 2], s[4 * i + 3]);
                 continue;
             }
-            // The gradient itself, 32 columns at a time: 128 or 64 bytes a row of the slab.
+            // The gradient itself, 128 bytes a row of the slab at a time: 32 fp32 columns or 64 of 16 bits (32 of a tile
+            // whose halves have no more).
             const uint32_t es = g.dw_f32 ? 4u : 2u;
-#pragma unroll
-            for (uint32_t c0 = 0; c0 < kHalf; c0 += 32u) {
-                if (n0 + c0 >= g.N) break;
-                const uint32_t cols = min(32u, g.N - n0 - c0);
+            constexpr uint32_t kWide16 = kHalf < 64u ? kHalf : 64u;
+            const auto out = [&](unsigned char* slab, uint32_t c0, uint32_t wide, auto put) {
+                const uint32_t cols = min(wide, g.N - n0 - c0);
                 unsigned char* at = static_cast<unsigned char*>(g.dw) + (static_cast<uint64_t>(m0) * g.N + n0 + c0) * es;
                 if (g.accumulate) {
                     if (g.dw_f32) slab_copy<4, false>(slab, at, g.N, rows, cols, g.dw_vec != 0u, lane);
                     else slab_copy<2, false>(slab, at, g.N, rows, cols, g.dw_vec != 0u, lane);
                     __syncwarp();
                 }
-                if (g.dw_f32) {
-#pragma unroll
-                    for (uint32_t p = 0; p < 8u; ++p) {
-                        float4* l = reinterpret_cast<float4*>(slab + slab_at(lane, p));
-                        float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                        if (g.accumulate) o = *l;
-                        const uint32_t i = c0 + 4u * p;
-                        *l = make_float4(o.x + s[i], o.y + s[i + 1], o.z + s[i + 2], o.w + s[i + 3]);
+                put(slab);
+                if (g.dw_tma) {
+                    umma::fence_async_smem();
+                    __syncwarp();
+                    if (lane == 0u && rows) {
+                        tma::store_2d(&maps.y, smem_u32(slab), static_cast<int32_t>(n0 + c0), static_cast<int32_t>(m0));
+                        tma::store_commit();
                     }
                 } else {
-#pragma unroll
-                    for (uint32_t p = 0; p < 4u; ++p) {
-                        uint4* l = reinterpret_cast<uint4*>(slab + slab_at(lane, p));
-                        uint4 o = make_uint4(0u, 0u, 0u, 0u);
-                        if (g.accumulate) o = *l;
-                        const uint32_t ow[4] = {o.x, o.y, o.z, o.w};
-                        uint32_t w[4];
-#pragma unroll
-                        for (uint32_t i = 0; i < 4u; ++i) {
-                            const float2 f = unpack_16(ow[i], bf16);
-                            w[i] = pack_16(f.x + s[c0 + 8u * p + 2u * i], f.y + s[c0 + 8u * p + 2u * i + 1u], bf16);
-                        }
-                        *l = make_uint4(w[0], w[1], w[2], w[3]);
-                    }
+                    __syncwarp();
+                    if (g.dw_f32) slab_copy<4, true>(slab, at, g.N, rows, cols, g.dw_vec != 0u, lane);
+                    else slab_copy<2, true>(slab, at, g.N, rows, cols, g.dw_vec != 0u, lane);
+                    __syncwarp();
                 }
+            };
+            const auto free_slab = [&]() -> unsigned char* {
+                if (lane == 0u) tma::store_wait_read<S::kSlabs - 1u>();
                 __syncwarp();
-                if (g.dw_f32) slab_copy<4, true>(slab, at, g.N, rows, cols, g.dw_vec != 0u, lane);
-                else slab_copy<2, true>(slab, at, g.N, rows, cols, g.dw_vec != 0u, lane);
-                __syncwarp();
+                slab_i ^= 1u;
+                return my_slabs + slab_i * kSlabBytes;
+            };
+            if (g.dw_f32) {
+#pragma unroll
+                for (uint32_t c0 = 0; c0 < kHalf; c0 += 32u) {
+                    if (n0 + c0 >= g.N) break;
+                    out(free_slab(), c0, 32u, [&](unsigned char* slab) {
+#pragma unroll
+                        for (uint32_t p = 0; p < 8u; ++p) {
+                            float4* l = reinterpret_cast<float4*>(slab + slab_at(lane, p));
+                            float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                            if (g.accumulate) o = *l;
+                            const uint32_t i = c0 + 4u * p;
+                            *l = make_float4(o.x + s[i], o.y + s[i + 1], o.z + s[i + 2], o.w + s[i + 3]);
+                        }
+                    });
+                }
+            } else {
+#pragma unroll
+                for (uint32_t c0 = 0; c0 < kHalf; c0 += kWide16) {
+                    if (n0 + c0 >= g.N) break;
+                    out(free_slab(), c0, kWide16, [&](unsigned char* slab) {
+#pragma unroll
+                        for (uint32_t p = 0; p < kWide16 / 8u; ++p) {
+                            uint4* l = reinterpret_cast<uint4*>(slab + slab_at(lane, p));
+                            uint4 o = make_uint4(0u, 0u, 0u, 0u);
+                            if (g.accumulate) o = *l;
+                            const uint32_t ow[4] = {o.x, o.y, o.z, o.w};
+                            uint32_t w[4];
+#pragma unroll
+                            for (uint32_t i = 0; i < 4u; ++i) {
+                                const float2 f = unpack_16(ow[i], bf16);
+                                w[i] = pack_16(f.x + s[c0 + 8u * p + 2u * i], f.y + s[c0 + 8u * p + 2u * i + 1u], bf16);
+                            }
+                            *l = make_uint4(w[0], w[1], w[2], w[3]);
+                        }
+                    });
+                }
             }
         }
+        if (lane == 0u) tma::store_wait_all();
     } else if (KIND == kGemmRows && warp >= 4u && warp < S::kFirstLoader) {
         // ---- epilogue: warp q of a group drains rows 32 q .. 32 q + 31 of the tile
         const uint32_t q = warp & 3u, acc = (warp >> 2) - 1u;
@@ -523,7 +553,7 @@ __global__ void __launch_bounds__(GemmShape<BN, KIND, FEED>::kThreads, 1) k_gemm
 template <uint32_t BN, bool PLAIN>
 struct ColsShape {
     static constexpr uint32_t kStageBytes = kStageBytesA + BN * 128u;
-    static constexpr uint32_t kStages = 4u;
+    static constexpr uint32_t kStages = 4u;  // two or three CTAs an SM: the next launch's start while this one's end
     static constexpr uint32_t kSmem = 1024u + kStages * kStageBytes;
     static constexpr uint32_t kThreads = PLAIN ? 256u + 32u * kLoadWarps : 256u;
     static_assert(BN * kBM * 4u <= kStages * kStageBytes, "the partial tile takes the stages' place");

@@ -40,14 +40,14 @@ struct GemmArgs {
     // epilogue of a weight gradient: partials when splits > 1, else dw (+)= D
     float* partials;
     void* dw;
-    uint32_t dw_f32, dw_vec, accumulate;
+    uint32_t dw_f32, dw_vec, dw_tma, accumulate;
     uint32_t* error;
 };
 
 enum GemmKind : int { kGemmRows = 0, kGemmGrad = 1 };
 
 struct GemmMaps {
-    CUtensorMap a, b, y, pre, res;
+    CUtensorMap a, b, y, pre, res;  // y: of a weight gradient dw
 };
 // How a product's operands reach shared memory: copied for one CTA a tile,
 // copied for a pair of CTAs on one 256 x 256 tile, or loaded by warps.

@@ -78,14 +78,16 @@ EncodeTiled encode_tiled() {
 // Whether the copy unit can store into a matrix: it writes whole 16-byte
 // pieces, so a row must start and end with one.
 bool tma_rows(const MatrixView& m) { return m.ptr && m.vec >= 8u && m.cols % 8u == 0u; }
-// Boxes of box_rows x 64 values of a matrix, 128-byte swizzle, zero outside it.
-bool make_map(CUtensorMap* map, const MatrixView& m, uint32_t box_rows, bool bf16) {
+// Boxes of box_rows x box_cols values of a matrix, 128-byte swizzle, zero outside it.
+bool make_map(CUtensorMap* map, const MatrixView& m, uint32_t box_rows, bool bf16, bool f32 = false, uint32_t box_cols = 64u) {
     const EncodeTiled fn = encode_tiled();
     if (!fn) return false;
     const cuuint64_t dims[2] = {m.cols, m.rows};
-    const cuuint64_t strides[1] = {m.ld * 2u};
-    const cuuint32_t box[2] = {64u, box_rows}, elem[2] = {1u, 1u};
-    return fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2u, const_cast<void*>(m.ptr), dims, strides,
+    const cuuint64_t strides[1] = {m.ld * (f32 ? 4u : 2u)};
+    const cuuint32_t box[2] = {box_cols, box_rows}, elem[2] = {1u, 1u};
+    const CUtensorMapDataType type =
+        f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+    return fn(map, type, 2u, const_cast<void*>(m.ptr), dims, strides,
               box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
@@ -94,10 +96,14 @@ bool make_map(CUtensorMap* map, const MatrixView& m, uint32_t box_rows, bool bf1
 // Tile width of an activation product: the number of waves of 128 x bn tiles
 // times the time of one, which grows with bn and has a part (the row panel's
 // copy) that does not.
-uint32_t pick_bn(uint32_t tiles_m, uint32_t n, uint32_t sms) {
-    uint32_t best = 256u;
+// Up to K = 256 the epilogues take the time, and 128 columns have twice the
+// epilogue warps (65536 x 256 -> 256 with residual 27.9 us with 128 columns and
+// 31.5 with 256; at K = 512 both take 29.2).
+uint32_t pick_bn(uint32_t tiles_m, uint32_t n, uint32_t k, bool plain, uint32_t sms) {
+    const uint32_t widest = k <= 256u && !plain ? 128u : 256u;
+    uint32_t best = widest;
     uint64_t cost = ~0ull;
-    for (uint32_t bn = 256u; bn >= 64u; bn /= 2u) {
+    for (uint32_t bn = widest; bn >= 64u; bn /= 2u) {
         if (bn > 64u && bn / 2u >= n) continue;  // half of it holds every column
         const uint64_t tiles = static_cast<uint64_t>(tiles_m) * ceil_div(n, bn);
         const uint64_t c = ((tiles + sms - 1u) / sms) * (bn + 64u);
@@ -216,6 +222,15 @@ cudaError_t run_gemm(GemmArgs& g, int kind, uint32_t bn, bool pair, uint32_t sms
     g.res_tma = g.res.ptr && g.res.vec >= 8u;
     if ((g.res_tma && !make_map(&maps.res, g.res, 32u, bf16)) || (g.y_tma && !make_map(&maps.y, g.y, 32u, bf16)) || (g.pre_tma && !make_map(&maps.pre, g.pre, 32u, bf16)))
         return cudaErrorNotSupported;
+    g.dw_tma = kind == kGemmGrad && g.splits == 1u && g.dw_vec;
+    if (g.dw_tma) {
+        MatrixView dw{};
+        dw.ptr = g.dw;
+        dw.ld = g.N;
+        dw.rows = g.M;
+        dw.cols = g.N;
+        if (!make_map(&maps.y, dw, 32u, bf16, g.dw_f32 != 0u, g.dw_f32 || bn == 64u ? 32u : 64u)) return cudaErrorNotSupported;
+    }
     const uint64_t items = static_cast<uint64_t>(g.tiles_m) * g.tiles_n * g.splits, slots = pair ? sms / 2u : sms;
     const uint32_t blocks = static_cast<uint32_t>(items < slots ? items : slots) * (pair ? 2u : 1u);
     return launch_gemm(g, kind, bn, plain ? kFeedPlain : pair ? kFeedPair : kFeedTma, maps, blocks, s);
@@ -256,7 +271,7 @@ cudaError_t run_rows(GemmArgs& g, uint32_t sms, cudaStream_t s) {
     const bool pair = g.a.vec >= 8u && g.b.vec >= 8u && pair_pays(g.M, g.N, g.K, sms);
     if (!pair && cols_pay(g.M, g.N, g.K, sms)) return run_cols(g, s, sms);
     g.tiles_m = ceil_div(g.M, pair ? 2u * kGemmBM : kGemmBM);
-    const uint32_t bn = pair ? kGemmPairBN : pick_bn(g.tiles_m, g.N, sms);
+    const uint32_t bn = pair ? kGemmPairBN : pick_bn(g.tiles_m, g.N, g.K, g.a.vec < 8u || g.b.vec < 8u, sms);
     g.tiles_n = ceil_div(g.N, bn);
     g.splits = 1u;
     g.k_steps = g.steps_per_split = ceil_div(g.K, kGemmBK);
