@@ -20,8 +20,8 @@
 //               and half of B, so the tensor cores read 8 KB of shared memory
 //               per 64 cycles of MMA and SM instead of 12 KB, more than it
 //               delivers (128 bytes a cycle).
-//   kFeedPlain  rows that do not start on 16-byte boundaries, which the tensor
-//               copy unit cannot address: eight more warps load them.
+//   kFeedRaw    rows that do not start on 16-byte boundaries: copied raw,
+//               and moved into place by eight more warps.
 #include <atomic>
 
 #include "linear_common.cuh"
@@ -34,75 +34,98 @@ constexpr uint32_t kStageBytesA = kBM * 128u;
 constexpr uint32_t kMaxStages = 8;
 
 
-// ------------------------------------------------------------- operand boxes
+// ------------------------------------------------------------- raw operands
+// A box of an operand whose rows do not start on 16-byte boundaries.  Eight rows
+// of any length are a multiple of 16 bytes, so the rows r, r + 8, r + 16, ...
+// all lie alike: one copy takes a box's rows of one residue mod 8, 72 (K-major)
+// or 136 (MN-major) values each from the 16-byte boundary before the first one
+// wanted.  Warp w moves the rows of residue w into the swizzled box: a
+// shared-memory read or two, a permute and a write a row, and no trip to memory.
+// The copies' price is by the copy (a thread gets one off about every 128
+// cycles), so the operands' are issued by a warp each.  2000 x 4000 -> 4000 with
+// rows 4001 apart took 356 us with loads to registers instead, and 430 us with
+// 16-byte asynchronous copies by the warps that move the rows.
 constexpr uint32_t kLoadWarps = 8;
+constexpr uint32_t kRawRing = 2;  // steps of raw copies in shared memory
 
-// ROWS x 64 values at (row0, col0) of a matrix -> a swizzled box, zero outside
-// the matrix, by kLoadWarps warps.
-template <uint32_t ROWS>
-NB_DEV void fill_box(unsigned char* box, const MatrixView& m, uint32_t row0, uint32_t col0, uint32_t tid) {
-    const uint16_t* base = static_cast<const uint16_t*>(m.ptr);
-    const uint32_t have = col0 < m.cols ? min(64u, m.cols - col0) : 0u;
-    if (m.vec >= 8u && (have & 7u) == 0u) {
-        // Whole 16-byte pieces: eight threads a row.
-#pragma unroll 4
-        for (uint32_t c = tid; c < ROWS * 8u; c += kLoadWarps * 32u) {
-            const uint32_t r = c >> 3, p = c & 7u;
-            const uint64_t gr = static_cast<uint64_t>(row0) + r;
-            uint4 u = make_uint4(0u, 0u, 0u, 0u);
-            if (gr < m.rows && 8u * p < have) u = *reinterpret_cast<const uint4*>(base + gr * m.ld + col0 + 8u * p);
-            *reinterpret_cast<uint4*>(box + slab_at(r, p)) = u;
-        }
+// Bytes of one residue's copy: of n rows (K-major), of 64 rows x 128 columns (MN-major).
+constexpr uint32_t kRawMn = 8u * kRawColsMn * 2u;
+__host__ __device__ constexpr uint32_t raw_tx(uint32_t mn, uint32_t n) { return mn ? kRawMn : n / 8u * kRawColsK * 2u; }
+__host__ __device__ constexpr uint32_t raw_slot(uint32_t mn, uint32_t n) { return (raw_tx(mn, n) + 127u) / 128u * 128u; }
+__host__ __device__ constexpr uint32_t raw_bytes(uint32_t n) { return 8u * (raw_slot(0u, n) > kRawMn ? raw_slot(0u, n) : kRawMn); }
+
+// One thread: the copies of a box (mn: 64 rows from k0, columns from n0; else n rows from n0, columns from k0).
+NB_DEV void raw_load(unsigned char* raw, const CUtensorMap* map, const MatrixView& m, uint32_t mn, uint32_t n, uint32_t n0, uint32_t k0,
+                     uint64_t* mbar) {
+    if (m.rows < 8u) {  // nothing is copied (the rows behind the last whole group of eight are loaded)
+        tma::expect_tx(mbar, 0u);
         return;
     }
-    // A warp every eighth row, lane i the values 2 i and 2 i + 1: one 32-bit
-    // load where every row starts on a word, else two of 16 bits.  A batch of
-    // rows is in flight before the first is stored, and only a box over the
-    // matrix's last rows looks at each row: the instructions a row are what
-    // bounds this path.
-    static_assert(kLoadWarps == 8u, "the swizzle of a warp's rows is the same");
-    constexpr uint32_t kBatch = ROWS / kLoadWarps < 16u ? ROWS / kLoadWarps : 16u;
-    const uint32_t lane = tid & 31u, warp = tid >> 5;
-    const bool lo = 2u * lane < have, hi = 2u * lane + 1u < have, words = m.vec >= 2u && !(have & 1u);
-    const uint64_t step = kLoadWarps * m.ld;
-    unsigned char* dst = box + slab_at(warp, lane >> 2) + 4u * (lane & 3u);
-    const uint16_t* q = base + (static_cast<uint64_t>(row0) + warp) * m.ld + col0 + 2u * lane;
+    const uint32_t slot = raw_slot(mn, n), row0 = mn ? k0 : n0, col0 = mn ? n0 : k0;
+    const uint32_t off = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(m.ptr) & 15u) / 2u;
+    tma::expect_tx(mbar, 8u * raw_tx(mn, n));
+    for (uint32_t i = 0; i < 8u; ++i)
+        tma::load_2d(smem_u32(raw + i * slot), map, static_cast<int32_t>((off + i * static_cast<uint32_t>(m.ld) + col0) & ~7u),
+                     static_cast<int32_t>(row0 >> 3), mbar);
+}
+// ROWS rows of 64 values, their residue-w rows: raw (pitch words a row) -> box; and the row of residue w behind the
+// whole groups of eight, if it is one of them.
+template <uint32_t ROWS>
+NB_DEV void raw_rows(unsigned char* box, const uint32_t* raw, uint32_t pitch, uint32_t shift, const MatrixView& m, uint32_t row0, uint32_t col0,
+                     uint32_t w, uint32_t lane) {
+    constexpr uint32_t kAll = ROWS / 8u, kBatch = kAll < 16u ? kAll : 16u;
+    static_assert(kAll % kBatch == 0u, "whole batches");
+    const uint32_t have = col0 < m.cols ? min(64u, m.cols - col0) : 0u, whole = m.rows < 8u ? 0u : have;
+    const uint32_t mask = (2u * lane < whole ? 0xffffu : 0u) | (2u * lane + 1u < whole ? 0xffff0000u : 0u);
+    const uint32_t lane_at = 4u * (lane & 3u);
+    unsigned char* dst = box + slab_at(w, lane >> 2) + lane_at;
+    const uint32_t* src = raw + lane + (shift >> 1);
 #pragma unroll 1
-    for (uint32_t r0 = warp; r0 < ROWS; r0 += kLoadWarps * kBatch) {
-        const uint32_t in = row0 + r0 < m.rows ? m.rows - row0 - r0 : 0u;  // matrix rows from r0 on
-        uint32_t w[kBatch], v[kBatch];
-        if (in > (kBatch - 1u) * kLoadWarps) {
-            if (words) {
+    for (uint32_t g = 0; g < kAll; g += kBatch) {
+        uint32_t v[kBatch];
 #pragma unroll
-                for (uint32_t j = 0; j < kBatch; ++j) w[j] = load_32(q + j * step, hi);
-            } else {
+        for (uint32_t j = 0; j < kBatch; ++j) v[j] = src[j * pitch];
+        if (shift & 1u) {
+            uint32_t u[kBatch];
 #pragma unroll
-                for (uint32_t j = 0; j < kBatch; ++j) {
-                    w[j] = load_16(q + j * step, lo);
-                    v[j] = load_16(q + j * step + 1, hi);
-                }
-            }
-        } else {
+            for (uint32_t j = 0; j < kBatch; ++j) u[j] = src[j * pitch + 1u];
 #pragma unroll
-            for (uint32_t j = 0; j < kBatch; ++j) {
-                w[j] = load_16(q + j * step, lo && j * kLoadWarps < in);
-                v[j] = load_16(q + j * step + 1, hi && j * kLoadWarps < in);
-            }
-        }
-        if (!words || in <= (kBatch - 1u) * kLoadWarps) {
-#pragma unroll
-            for (uint32_t j = 0; j < kBatch; ++j) w[j] |= v[j] << 16;
+            for (uint32_t j = 0; j < kBatch; ++j) v[j] = __byte_perm(v[j], u[j], 0x5432);
         }
 #pragma unroll
-        for (uint32_t j = 0; j < kBatch; ++j) *reinterpret_cast<uint32_t*>(dst + j * kLoadWarps * 128u) = w[j];
-        q += kBatch * step;
-        dst += kBatch * kLoadWarps * 128u;
+        for (uint32_t j = 0; j < kBatch; ++j) *reinterpret_cast<uint32_t*>(dst + j * 1024u) = v[j] & mask;
+        src += kBatch * pitch;
+        dst += kBatch * 1024u;
+    }
+    const uint32_t r = (m.rows & ~7u) + w;
+    if (r < m.rows && r >= row0 && r < row0 + ROWS) {
+        const uint16_t* q = static_cast<const uint16_t*>(m.ptr) + r * m.ld + col0 + 2u * lane;
+        *reinterpret_cast<uint32_t*>(box + slab_at(r - row0, lane >> 2) + lane_at) =
+            load_16(q, 2u * lane < have) | (load_16(q + 1, 2u * lane + 1u < have) << 16);
+    }
+}
+// Warp w's part of a box of N rows or columns.
+template <uint32_t N>
+NB_DEV void raw_box(unsigned char* box, const unsigned char* raw, const MatrixView& m, uint32_t mn, uint32_t n0, uint32_t k0, uint32_t w,
+                    uint32_t lane) {
+    // From the boundary to the first value wanted (n0 and k0 are multiples of 8).
+    const uint32_t shift = ((static_cast<uint32_t>(reinterpret_cast<uintptr_t>(m.ptr)) >> 1) + w * static_cast<uint32_t>(m.ld)) & 7u;
+    const uint32_t* src = reinterpret_cast<const uint32_t*>(raw + w * raw_slot(mn, N));
+    if (mn) {
+        if constexpr (N >= 64u) {
+#pragma unroll
+            for (uint32_t j = 0; j < N / 64u; ++j)
+                raw_rows<kBK>(box + j * 8192u, src + 32u * j, kRawColsMn / 2u, shift, m, k0, n0 + 64u * j, w, lane);
+        }
+    } else {
+        raw_rows<N>(box, src, kRawColsK / 2u, shift, m, n0, k0, w, lane);
     }
 }
 
 // ------------------------------------------------------------------ the GEMM
 struct Barriers {
     uint64_t full[kMaxStages], empty[kMaxStages];
+    uint64_t raw_full[2][kRawRing], raw_empty[2][kRawRing];  // of A and of B
     uint64_t acc_full[4], acc_empty[4];
     uint64_t res[16];  // an epilogue warp's residual rows have arrived
     uint64_t drain;
@@ -120,20 +143,22 @@ NB_DEV void tile_of(const GemmArgs& g, uint32_t t, uint32_t& tm, uint32_t& tn) {
 
 template <uint32_t BN, int KIND, int FEED>
 struct GemmShape {
-    static constexpr bool kPair = FEED == kFeedPair, kPlain = FEED == kFeedPlain;
+    static constexpr bool kPair = FEED == kFeedPair, kRaw = FEED == kFeedRaw;
     static constexpr uint32_t kBoxN = kPair ? BN / 2u : BN;  // rows of B in this CTA's shared memory
     static constexpr uint32_t kStageBytes = kStageBytesA + kBoxN * 128u;
     // Epilogue groups of four warps, an accumulator each: tiles of up to 128
     // columns are bound by memory and by the latency of their epilogues.
-    static constexpr uint32_t kGroups = KIND == kGemmRows && BN <= 128u && !kPlain ? 4u : 2u;
-    static constexpr uint32_t kStages = kPlain ? 2u : kPair ? 5u : BN >= 128u ? 3u : 4u;
+    static constexpr uint32_t kGroups = KIND == kGemmRows && BN <= 128u && !kRaw ? 4u : 2u;
+    static constexpr uint32_t kRawBytes = raw_bytes(kBM) + raw_bytes(kBoxN);  // raw copies of a step
+    static constexpr uint32_t kRaws = kRaw ? kRawRing * kRawBytes : 0u;
+    static constexpr uint32_t kStages = kRaw ? 2u : kPair ? 5u : BN >= 128u ? 3u : 4u;
     static constexpr uint32_t kSlabs = 2u;  // per epilogue warp
-    static constexpr uint32_t kSmem = 1024u + kStages * kStageBytes + 4u * kGroups * kSlabs * kSlabBytes + kGroups * BN * 2u;
+    static constexpr uint32_t kSmem = 1024u + kStages * kStageBytes + kRaws + 4u * kGroups * kSlabs * kSlabBytes + kGroups * BN * 2u;
     static constexpr uint32_t kFirstLoader = 4u + 4u * kGroups;
-    static constexpr uint32_t kThreads = 32u * (kFirstLoader + (kPlain ? kLoadWarps : 0u));
+    static constexpr uint32_t kThreads = 32u * (kFirstLoader + (kRaw ? kLoadWarps : 0u));
     // Weight gradients of 256 columns keep 128 sums a thread: registers move
     // from the copying and issuing warps to the two groups that sum.
-    static constexpr bool kRegs = KIND == kGemmGrad && BN == 256u && !kPlain;
+    static constexpr bool kRegs = KIND == kGemmGrad && BN == 256u;
     static constexpr int kRegsDown = 40, kRegsUp = 208;
     static constexpr uint32_t kRegsNeeded = 128u * kRegsDown + 256u * kRegsUp;  // of the block's at launch
     static_assert(kSmem <= 232448u - 512u, "shared memory of one CTA");
@@ -141,7 +166,7 @@ struct GemmShape {
 
 // Warps: 0 operand copies, 1 MMA, 2 tensor-memory allocation, from 4 on the
 // epilogue groups of four, which take turns (item i of the CTA: group and
-// accumulator i % kGroups), then the operand loads (kFeedPlain).
+// accumulator i % kGroups), then the ones that place raw copies (kFeedRaw).
 template <uint32_t BN, int KIND, int FEED>
 __global__ void __launch_bounds__(GemmShape<BN, KIND, FEED>::kThreads, 1) k_gemm(const GemmArgs g, const __grid_constant__ GemmMaps maps) {
     using S = GemmShape<BN, KIND, FEED>;
@@ -151,7 +176,8 @@ __global__ void __launch_bounds__(GemmShape<BN, KIND, FEED>::kThreads, 1) k_gemm
     extern __shared__ unsigned char smem_raw[];
     __shared__ Barriers bar;
     unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-    unsigned char* slabs = smem + kStages * kStageBytes;
+    unsigned char* raws = smem + kStages * kStageBytes;
+    unsigned char* slabs = raws + S::kRaws;
     uint16_t* bias_all = reinterpret_cast<uint16_t*>(slabs + 4u * S::kGroups * S::kSlabs * kSlabBytes);
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
     const bool bf16 = g.bf16 != 0u;
@@ -160,8 +186,14 @@ __global__ void __launch_bounds__(GemmShape<BN, KIND, FEED>::kThreads, 1) k_gemm
 
     if (threadIdx.x == 0u) {
         for (uint32_t i = 0; i < kStages; ++i) {
-            umma::mbar_init(&bar.full[i], S::kPlain ? 32u * kLoadWarps : 1u);
+            umma::mbar_init(&bar.full[i], S::kRaw ? kLoadWarps + (g.a_raw && g.b_raw ? 0u : 1u) : 1u);
             umma::mbar_init(&bar.empty[i], 1u);
+        }
+        for (uint32_t i = 0; S::kRaw && i < kRawRing; ++i) {
+            for (uint32_t o = 0; o < 2u; ++o) {
+                umma::mbar_init(&bar.raw_full[o][i], 1u);
+                umma::mbar_init(&bar.raw_empty[o][i], kLoadWarps);
+            }
         }
         for (uint32_t i = 0; i < S::kGroups; ++i) {
             umma::mbar_init(&bar.acc_full[i], 1u);
@@ -170,7 +202,7 @@ __global__ void __launch_bounds__(GemmShape<BN, KIND, FEED>::kThreads, 1) k_gemm
         for (uint32_t i = 0; i < 4u * S::kGroups; ++i) umma::mbar_init(&bar.res[i], 1u);
         umma::mbar_init(&bar.drain, 1u);
         umma::fence_mbar_init();
-        if (!S::kPlain) {
+        if (!S::kRaw) {
             tma::prefetch_map(&maps.a);
             tma::prefetch_map(&maps.b);
         }
@@ -195,56 +227,43 @@ __global__ void __launch_bounds__(GemmShape<BN, KIND, FEED>::kThreads, 1) k_gemm
     const uint32_t tiles = g.tiles_m * g.tiles_n, items = tiles * g.splits;
     if (S::kRegs && warp < 4u) tma::registers_down<S::kRegsDown>();
 
-    if ((!S::kPlain && warp == 0u && lane == 0u) || (S::kPlain && warp >= S::kFirstLoader)) {
-        // ---- producer: one thread issuing tensor copies, or warps of loads
+    if ((warp == 0u || warp == 3u) && lane == 0u) {
+        // ---- producers: warp 0 issues the copies of A, warp 3 those of B
+        const uint32_t op = warp == 0u ? 0u : 1u;
+        const bool raw = S::kRaw && (op ? g.b_raw : g.a_raw);
+        const MatrixView& m = op ? g.b : g.a;
+        const CUtensorMap* map = op ? &maps.b : &maps.a;
+        const uint32_t mn = op ? g.b_mn : g.a_mn, width = op ? S::kBoxN : kBM;
+        const uint32_t bytes_a = g.a_mn ? kStageBytesA : g.a_box_rows * 128u, bytes_b = S::kBoxN * 128u;
+        // What one arrival announces at a stage's barrier: of two copied operands A's producer both (of a pair the
+        // leading CTA's for both CTAs), of one copied operand its own producer.
+        const uint32_t bytes = !S::kRaw ? bytes_a + bytes_b : op ? bytes_b : bytes_a;
+        const bool announce = S::kRaw ? !raw : op == 0u && rank == 0u;
         uint32_t stage = 0, parity = 1u, issued = 0;
         bool ok = true;
         for (uint32_t it = first_item; it < items && ok; it += item_step) {
             const uint32_t split = it / tiles;
             uint32_t tm, tn;
             tile_of(g, it - split * tiles, tm, tn);
-            const uint32_t m0 = (tm * kCtas + rank) * kBM, n0 = tn * BN + rank * S::kBoxN;
+            const uint32_t at = op ? tn * BN + rank * S::kBoxN : (tm * kCtas + rank) * kBM;  // the box's rows or columns
             const uint32_t ks1 = min(g.k_steps, (split + 1u) * g.steps_per_split);
             for (uint32_t ks = split * g.steps_per_split; ks < ks1; ++ks) {
-                if (!tma::wait(&bar.empty[stage], parity)) {
-                    ok = false;
-                    break;
-                }
-                unsigned char* sa = smem + stage * kStageBytes;
-                unsigned char* sb = sa + kStageBytesA;
                 const uint32_t k0 = ks * kBK;
-                if (S::kPlain) {
-                    const uint32_t tid = threadIdx.x - 32u * S::kFirstLoader;
-                    if (g.a_mn) {
-                        for (uint32_t j = 0; j < kBM / 64u; ++j) fill_box<kBK>(sa + j * 8192u, g.a, k0, m0 + 64u * j, tid);
-                    } else {
-                        fill_box<kBM>(sa, g.a, m0, k0, tid);
-                    }
-                    if (g.b_mn) {
-                        for (uint32_t j = 0; j < BN / 64u; ++j) fill_box<kBK>(sb + j * 8192u, g.b, k0, n0 + 64u * j, tid);
-                    } else {
-                        fill_box<BN>(sb, g.b, n0, k0, tid);
-                    }
-                    umma::fence_async_smem();
-                    tma::arrive(&bar.full[stage]);
+                if (raw) {
+                    const uint32_t r = issued % kRawRing;
+                    ok = tma::wait(&bar.raw_empty[op][r], (issued / kRawRing + 1u) & 1u);
+                    if (!ok) break;
+                    raw_load(raws + r * S::kRawBytes + op * raw_bytes(kBM), map, m, mn, width, at, k0, &bar.raw_full[op][r]);
                 } else {
-                    const uint32_t bytes = (g.a_mn ? kStageBytesA : g.a_box_rows * 128u) + S::kBoxN * 128u;
-                    // Of a pair both CTAs' copies are counted by the leading CTA's barrier.
-                    if (rank == 0u) tma::expect_tx(&bar.full[stage], kCtas * bytes);
+                    ok = tma::wait(&bar.empty[stage], parity);
+                    if (!ok) break;
+                    unsigned char* dst = smem + stage * kStageBytes + op * kStageBytesA;
+                    if (announce) tma::expect_tx(&bar.full[stage], kCtas * bytes);
                     const uint32_t full = S::kPair ? tma::peer_addr(smem_u32(&bar.full[stage]), 0u) : 0u;
-                    const auto load = [&](unsigned char* dst, const CUtensorMap* map, uint32_t x, uint32_t y) {
-                        if (S::kPair) tma::load_2d_pair(smem_u32(dst), map, x, y, full);
-                        else tma::load_2d(smem_u32(dst), map, x, y, &bar.full[stage]);
-                    };
-                    if (g.a_mn) {
-                        for (uint32_t j = 0; j < kBM / 64u; ++j) load(sa + j * 8192u, &maps.a, m0 + 64u * j, k0);
-                    } else {
-                        load(sa, &maps.a, k0, m0);
-                    }
-                    if (g.b_mn) {
-                        for (uint32_t j = 0; j < S::kBoxN / 64u; ++j) load(sb + j * 8192u, &maps.b, n0 + 64u * j, k0);
-                    } else {
-                        load(sb, &maps.b, k0, n0);
+                    for (uint32_t j = 0; j < (mn ? width / 64u : 1u); ++j) {
+                        const uint32_t x = mn ? at + 64u * j : k0, y = mn ? k0 : at;
+                        if (S::kPair) tma::load_2d_pair(smem_u32(dst + j * 8192u), map, x, y, full);
+                        else tma::load_2d(smem_u32(dst + j * 8192u), map, x, y, &bar.full[stage]);
                     }
                 }
                 ++issued;
@@ -254,12 +273,50 @@ __global__ void __launch_bounds__(GemmShape<BN, KIND, FEED>::kThreads, 1) k_gemm
                 }
             }
         }
-        if (!ok) {
+        if (!ok) {  // copies in flight: wait for them before the shared memory goes
             atomicOr(g.error, 1u);
-            if (!S::kPlain && rank == 0u)  // copies in flight: wait for them before the shared memory goes
+            if (raw) {
+                for (uint32_t i = issued > kRawRing ? issued - kRawRing : 0u; i < issued; ++i)
+                    tma::wait(&bar.raw_full[op][i % kRawRing], (i / kRawRing) & 1u);
+            } else if (rank == 0u) {
                 for (uint32_t i = issued > kStages ? issued - kStages : 0u; i < issued; ++i)
                     tma::wait(&bar.full[i % kStages], (i / kStages) & 1u);
+            }
         }
+    } else if (S::kRaw && warp >= S::kFirstLoader) {
+        // ---- raw copies into place
+        const uint32_t w = warp - S::kFirstLoader;
+        uint32_t i = 0;
+        bool ok = true;
+        for (uint32_t it = first_item; it < items && ok; it += item_step) {
+            const uint32_t split = it / tiles;
+            uint32_t tm, tn;
+            tile_of(g, it - split * tiles, tm, tn);
+            const uint32_t ks1 = min(g.k_steps, (split + 1u) * g.steps_per_split);
+            for (uint32_t ks = split * g.steps_per_split; ks < ks1; ++ks, ++i) {
+                const uint32_t stage = i % kStages, r = i % kRawRing, turn = (i / kRawRing) & 1u;
+                ok = tma::wait(&bar.empty[stage], (i / kStages + 1u) & 1u) && (!g.a_raw || tma::wait(&bar.raw_full[0][r], turn)) &&
+                     (!g.b_raw || tma::wait(&bar.raw_full[1][r], turn));
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                unsigned char* sa = smem + stage * kStageBytes;
+                const unsigned char* src = raws + r * S::kRawBytes;
+                if (g.a_raw) {
+                    raw_box<kBM>(sa, src, g.a, g.a_mn, tm * kBM, ks * kBK, w, lane);
+                    __syncwarp();
+                    if (lane == 0u) tma::arrive(&bar.raw_empty[0][r]);
+                }
+                if (g.b_raw) {
+                    raw_box<BN>(sa + kStageBytesA, src + raw_bytes(kBM), g.b, g.b_mn, tn * BN, ks * kBK, w, lane);
+                    __syncwarp();
+                    if (lane == 0u) tma::arrive(&bar.raw_empty[1][r]);
+                }
+                umma::fence_async_smem();
+                __syncwarp();
+                if (lane == 0u) tma::arrive(&bar.full[stage]);
+            }
+        }
+        if (!ok) atomicOr(g.error, 1u);
     } else if (warp == 1u && lane == 0u && rank == 0u) {
         // ---- MMA issuer (of a pair: the leading CTA's)
         const uint32_t idesc = tma::idesc_16bit(kBM * kCtas, BN, g.a_mn, g.b_mn, g.bf16);
@@ -550,21 +607,23 @@ __global__ void __launch_bounds__(GemmShape<BN, KIND, FEED>::kThreads, 1) k_gemm
 // CTAs takes one tile, each a part of K.  Every CTA leaves its partial tile in
 // its own shared memory, and the cluster adds them in rank order over
 // distributed shared memory: no workspace, and the same bits every time.
-template <uint32_t BN, bool PLAIN>
+template <uint32_t BN, bool RAW>
 struct ColsShape {
     static constexpr uint32_t kStageBytes = kStageBytesA + BN * 128u;
-    static constexpr uint32_t kStages = 4u;  // two or three CTAs an SM: the next launch's start while this one's end
-    static constexpr uint32_t kSmem = 1024u + kStages * kStageBytes;
-    static constexpr uint32_t kThreads = PLAIN ? 256u + 32u * kLoadWarps : 256u;
+    static constexpr uint32_t kStages = RAW && BN == 128u ? 2u : 4u;  // two or three CTAs an SM: the next launch's start while this one's end
+    static constexpr uint32_t kRawBytes = raw_bytes(kBM) + raw_bytes(BN);  // raw copies of a step
+    static constexpr uint32_t kSmem = 1024u + kStages * kStageBytes + (RAW ? kRawRing * kRawBytes : 0u);
+    static constexpr uint32_t kThreads = RAW ? 256u + 32u * kLoadWarps : 256u;
+    static_assert(kSmem <= 232448u - 512u, "shared memory of one CTA");
     static_assert(BN * kBM * 4u <= kStages * kStageBytes, "the partial tile takes the stages' place");
 };
 
-template <uint32_t BN, bool PLAIN>
-__global__ void __launch_bounds__(ColsShape<BN, PLAIN>::kThreads) k_gemm_cols(const GemmArgs g, const __grid_constant__ GemmMaps maps) {
-    using S = ColsShape<BN, PLAIN>;
+template <uint32_t BN, bool RAW>
+__global__ void __launch_bounds__(ColsShape<BN, RAW>::kThreads) k_gemm_cols(const GemmArgs g, const __grid_constant__ GemmMaps maps) {
+    using S = ColsShape<BN, RAW>;
     constexpr uint32_t kStages = S::kStages, kStageBytes = S::kStageBytes, kCols = tmem_cols(BN);
     extern __shared__ unsigned char smem_raw[];
-    __shared__ uint64_t full[kStages], empty[kStages], acc_full, drain;
+    __shared__ uint64_t full[kStages], empty[kStages], raw_full[2][kRawRing], raw_empty[2][kRawRing], acc_full, drain;
     __shared__ uint32_t tmem_base, failed;
     unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
@@ -576,8 +635,14 @@ __global__ void __launch_bounds__(ColsShape<BN, PLAIN>::kThreads) k_gemm_cols(co
 
     if (threadIdx.x == 0u) {
         for (uint32_t i = 0; i < kStages; ++i) {
-            umma::mbar_init(&full[i], PLAIN ? 32u * kLoadWarps : 1u);
+            umma::mbar_init(&full[i], RAW ? kLoadWarps + (g.a_raw && g.b_raw ? 0u : 1u) : 1u);
             umma::mbar_init(&empty[i], 1u);
+        }
+        for (uint32_t i = 0; RAW && i < kRawRing; ++i) {
+            for (uint32_t o = 0; o < 2u; ++o) {
+                umma::mbar_init(&raw_full[o][i], 1u);
+                umma::mbar_init(&raw_empty[o][i], kLoadWarps);
+            }
         }
         umma::mbar_init(&acc_full, 1u);
         umma::mbar_init(&drain, 1u);
@@ -595,43 +660,64 @@ __global__ void __launch_bounds__(ColsShape<BN, PLAIN>::kThreads) k_gemm_cols(co
     let_next_start();
     const uint32_t tmem = tmem_base;
 
-    if ((!PLAIN && warp == 0u && lane == 0u) || (PLAIN && warp >= 8u)) {
+    unsigned char* raws = smem + kStages * kStageBytes;
+
+    if ((warp == 0u || warp == 3u) && lane == 0u) {
+        // As in k_gemm: warp 0 issues the copies of the weight, warp 3 those of the rows.
+        const uint32_t op = warp == 0u ? 0u : 1u;
+        const bool raw = RAW && (op ? g.b_raw : g.a_raw);
+        const MatrixView& m = op ? g.b : g.a;
+        const CUtensorMap* map = op ? &maps.b : &maps.a;
+        const uint32_t mn = op ? 0u : g.a_mn, width = op ? BN : kBM, at = op ? n0 : m0;
+        const uint32_t bytes = !RAW ? kStageBytes : op ? BN * 128u : kStageBytesA;
+        const bool announce = RAW ? !raw : op == 0u;
         uint32_t issued = 0;
         bool ok = true;
         for (uint32_t ks = ks0; ks < ks1; ++ks, ++issued) {
-            const uint32_t stage = issued % kStages;
-            if (!tma::wait(&empty[stage], (issued / kStages + 1u) & 1u)) {
-                ok = false;
-                break;
-            }
-            unsigned char* sa = smem + stage * kStageBytes;
-            unsigned char* sb = sa + kStageBytesA;
             const uint32_t k0 = ks * kBK;
-            if (PLAIN) {
-                const uint32_t tid = threadIdx.x - 256u;
-                if (g.a_mn) {
-                    for (uint32_t j = 0; j < kBM / 64u; ++j) fill_box<kBK>(sa + j * 8192u, g.a, k0, m0 + 64u * j, tid);
-                } else {
-                    fill_box<kBM>(sa, g.a, m0, k0, tid);
-                }
-                fill_box<BN>(sb, g.b, n0, k0, tid);
-                umma::fence_async_smem();
-                tma::arrive(&full[stage]);
+            if (raw) {
+                const uint32_t r = issued % kRawRing;
+                ok = tma::wait(&raw_empty[op][r], (issued / kRawRing + 1u) & 1u);
+                if (!ok) break;
+                raw_load(raws + r * S::kRawBytes + op * raw_bytes(kBM), map, m, mn, width, at, k0, &raw_full[op][r]);
             } else {
-                tma::expect_tx(&full[stage], kStageBytes);
-                if (g.a_mn) {
-                    for (uint32_t j = 0; j < kBM / 64u; ++j) tma::load_2d(smem_u32(sa + j * 8192u), &maps.a, m0 + 64u * j, k0, &full[stage]);
-                } else {
-                    tma::load_2d(smem_u32(sa), &maps.a, k0, m0, &full[stage]);
-                }
-                tma::load_2d(smem_u32(sb), &maps.b, k0, n0, &full[stage]);
+                const uint32_t stage = issued % kStages;
+                ok = tma::wait(&empty[stage], (issued / kStages + 1u) & 1u);
+                if (!ok) break;
+                unsigned char* dst = smem + stage * kStageBytes + op * kStageBytesA;
+                if (announce) tma::expect_tx(&full[stage], bytes);
+                for (uint32_t j = 0; j < (mn ? width / 64u : 1u); ++j)
+                    tma::load_2d(smem_u32(dst + j * 8192u), map, mn ? at + 64u * j : k0, mn ? k0 : at, &full[stage]);
             }
         }
         if (!ok) {
             atomicOr(g.error, 1u);
-            if (!PLAIN)
-                for (uint32_t i = issued > kStages ? issued - kStages : 0u; i < issued; ++i) tma::wait(&full[i % kStages], (i / kStages) & 1u);
+            const uint32_t ring = raw ? kRawRing : kStages;
+            for (uint32_t i = issued > ring ? issued - ring : 0u; i < issued; ++i)
+                tma::wait(raw ? &raw_full[op][i % ring] : &full[i % ring], (i / ring) & 1u);
         }
+    } else if (RAW && warp >= 8u) {
+        const uint32_t w = warp - 8u;
+        bool ok = true;
+        for (uint32_t i = 0; ks0 + i < ks1; ++i) {
+            const uint32_t stage = i % kStages, r = i % kRawRing, turn = (i / kRawRing) & 1u, k0 = (ks0 + i) * kBK;
+            ok = tma::wait(&empty[stage], (i / kStages + 1u) & 1u) && (!g.a_raw || tma::wait(&raw_full[0][r], turn)) &&
+                 (!g.b_raw || tma::wait(&raw_full[1][r], turn));
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            unsigned char* sa = smem + stage * kStageBytes;
+            const unsigned char* src = raws + r * S::kRawBytes;
+            if (g.a_raw) raw_box<kBM>(sa, src, g.a, g.a_mn, m0, k0, w, lane);
+            if (g.b_raw) raw_box<BN>(sa + kStageBytesA, src + raw_bytes(kBM), g.b, 0u, n0, k0, w, lane);
+            umma::fence_async_smem();
+            __syncwarp();
+            if (lane == 0u) {
+                if (g.a_raw) tma::arrive(&raw_empty[0][r]);
+                if (g.b_raw) tma::arrive(&raw_empty[1][r]);
+                tma::arrive(&full[stage]);
+            }
+        }
+        if (!ok) atomicOr(g.error, 1u);
     } else if (warp == 1u && lane == 0u) {
         const uint32_t idesc = tma::idesc_16bit(kBM, BN, g.a_mn, 0u, g.bf16);
         bool ok = true;
@@ -716,20 +802,20 @@ __global__ void __launch_bounds__(ColsShape<BN, PLAIN>::kThreads) k_gemm_cols(co
     if (warp == 2u) umma::tmem_dealloc(tmem, kCols);
 }
 
-template <uint32_t BN, bool PLAIN>
+template <uint32_t BN, bool RAW>
 cudaError_t launch_cols_t(const GemmArgs& g, const GemmMaps& maps, cudaStream_t s) {
-    using S = ColsShape<BN, PLAIN>;
+    using S = ColsShape<BN, RAW>;
     static std::atomic<bool> done[64];
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
     if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
     if (!done[dev]) {
-        e = cudaFuncSetAttribute(k_gemm_cols<BN, PLAIN>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
+        e = cudaFuncSetAttribute(k_gemm_cols<BN, RAW>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
         if (e != cudaSuccess) return e;
         done[dev] = true;
     }
-    return launch_after(k_gemm_cols<BN, PLAIN>, dim3(g.tiles_m * g.tiles_n * g.splits), S::kThreads, S::kSmem, g.splits, s, g, maps);
+    return launch_after(k_gemm_cols<BN, RAW>, dim3(g.tiles_m * g.tiles_n * g.splits), S::kThreads, S::kSmem, g.splits, s, g, maps);
 }
 
 // ------------------------------------------------- dz and its column sums
@@ -906,25 +992,19 @@ cudaError_t launch_gemm_t(const GemmArgs& g, const GemmMaps& maps, uint32_t bloc
     }
     return launch_after(k_gemm<BN, KIND, FEED>, dim3(blocks), S::kThreads, S::kSmem, S::kPair ? 2u : 1u, s, g, maps);
 }
-template <int KIND, int FEED>
-cudaError_t launch_gemm_bn(const GemmArgs& g, uint32_t bn, const GemmMaps& maps, uint32_t blocks, cudaStream_t s) {
-    switch (bn) {
-        case 64u: return launch_gemm_t<64u, KIND, FEED>(g, maps, blocks, s);
-        case 128u: return launch_gemm_t<128u, KIND, FEED>(g, maps, blocks, s);
-        case 256u:
-            if constexpr (KIND == kGemmRows || FEED != kFeedPlain) return launch_gemm_t<256u, KIND, FEED>(g, maps, blocks, s);
-            return cudaErrorInvalidValue;
-        default: return cudaErrorInvalidValue;
-    }
-}
 template <int KIND>
 cudaError_t launch_gemm_kind(const GemmArgs& g, uint32_t bn, int feed, const GemmMaps& maps, uint32_t blocks, cudaStream_t s) {
-    switch (feed) {
-        case kFeedTma: return launch_gemm_bn<KIND, kFeedTma>(g, bn, maps, blocks, s);
-        case kFeedPlain: return launch_gemm_bn<KIND, kFeedPlain>(g, bn, maps, blocks, s);
-        default:
-            if (bn != kGemmPairBN || (blocks & 1u)) return cudaErrorInvalidValue;
-            return launch_gemm_t<kGemmPairBN, KIND, kFeedPair>(g, maps, blocks, s);
+    if (feed == kFeedPair)
+        return bn == kGemmPairBN && !(blocks & 1u) ? launch_gemm_t<kGemmPairBN, KIND, kFeedPair>(g, maps, blocks, s) : cudaErrorInvalidValue;
+    if (feed == kFeedRaw) {
+        if (bn == 64u) return launch_gemm_t<64u, KIND, kFeedRaw>(g, maps, blocks, s);
+        return bn == kGemmRawBN ? launch_gemm_t<kGemmRawBN, KIND, kFeedRaw>(g, maps, blocks, s) : cudaErrorInvalidValue;
+    }
+    switch (bn) {
+        case 64u: return launch_gemm_t<64u, KIND, kFeedTma>(g, maps, blocks, s);
+        case 128u: return launch_gemm_t<128u, KIND, kFeedTma>(g, maps, blocks, s);
+        case 256u: return launch_gemm_t<256u, KIND, kFeedTma>(g, maps, blocks, s);
+        default: return cudaErrorInvalidValue;
     }
 }
 
@@ -935,13 +1015,13 @@ cudaError_t launch_gemm(const GemmArgs& g, int kind, uint32_t bn, int feed, cons
                              : launch_gemm_kind<kGemmGrad>(g, bn, feed, maps, blocks, s);
 }
 
-cudaError_t launch_gemm_cols(const GemmArgs& g, uint32_t bn, bool plain_loads, const GemmMaps& maps, cudaStream_t s) {
+cudaError_t launch_gemm_cols(const GemmArgs& g, uint32_t bn, bool raw, const GemmMaps& maps, cudaStream_t s) {
     if (g.splits == 0u || g.splits > kColsMaxCluster || g.b_mn) return cudaErrorInvalidValue;
     switch (bn) {
-        case 16u: return plain_loads ? launch_cols_t<16u, true>(g, maps, s) : launch_cols_t<16u, false>(g, maps, s);
-        case 32u: return plain_loads ? launch_cols_t<32u, true>(g, maps, s) : launch_cols_t<32u, false>(g, maps, s);
-        case 64u: return plain_loads ? launch_cols_t<64u, true>(g, maps, s) : launch_cols_t<64u, false>(g, maps, s);
-        case 128u: return plain_loads ? launch_cols_t<128u, true>(g, maps, s) : launch_cols_t<128u, false>(g, maps, s);
+        case 16u: return raw ? launch_cols_t<16u, true>(g, maps, s) : launch_cols_t<16u, false>(g, maps, s);
+        case 32u: return raw ? launch_cols_t<32u, true>(g, maps, s) : launch_cols_t<32u, false>(g, maps, s);
+        case 64u: return raw ? launch_cols_t<64u, true>(g, maps, s) : launch_cols_t<64u, false>(g, maps, s);
+        case 128u: return raw ? launch_cols_t<128u, true>(g, maps, s) : launch_cols_t<128u, false>(g, maps, s);
         default: return cudaErrorInvalidValue;
     }
 }

@@ -24,6 +24,7 @@ struct MatrixView {
 struct GemmArgs {
     MatrixView a, b;
     uint32_t M, N, K;
+    uint32_t a_raw, b_raw; // 1: rows off 16-byte boundaries, which the tensor copy unit cannot address
     uint32_t a_mn, b_mn;   // 1: stored [K][.]
     uint32_t a_box_rows;   // rows of a K-major A box (fewer than 128 when M is)
     uint32_t tiles_m, tiles_n;
@@ -50,16 +51,18 @@ struct GemmMaps {
     CUtensorMap a, b, y, pre, res;  // y: of a weight gradient dw
 };
 // How a product's operands reach shared memory: copied for one CTA a tile,
-// copied for a pair of CTAs on one 256 x 256 tile, or loaded by warps.
-enum GemmFeed : int { kFeedTma = 0, kFeedPair = 1, kFeedPlain = 2 };
-constexpr uint32_t kGemmPairBN = 256;
-
+// copied for a pair of CTAs on one 256 x 256 tile, or (one of them at least)
+// copied raw and moved into place by warps.
+enum GemmFeed : int { kFeedTma = 0, kFeedPair = 1, kFeedRaw = 2 };
+constexpr uint32_t kGemmPairBN = 256, kGemmRawBN = 128;  // the widest tile of raw copies
+// Values a row of a raw box: 64 or 128 and what rounding its start down adds.
+constexpr uint32_t kRawColsK = 72, kRawColsMn = 136;
 cudaError_t launch_gemm(const GemmArgs& g, int kind, uint32_t bn, int feed, const GemmMaps& maps, uint32_t blocks, cudaStream_t s);
 // Few rows: D^T[n][m], the weight's rows along the tensor core's 128, the
 // activations' rows along its columns, K split over a cluster of CTAs.  In the
 // arguments A is the weight and M its rows; y, res and pre are [N][M].
 constexpr uint32_t kColsMaxCluster = 8;
-cudaError_t launch_gemm_cols(const GemmArgs& g, uint32_t bn, bool plain_loads, const GemmMaps& maps, cudaStream_t s);
+cudaError_t launch_gemm_cols(const GemmArgs& g, uint32_t bn, bool raw, const GemmMaps& maps, cudaStream_t s);
 // dz = dy act'(pre) (16-bit, rows dz_ld apart; null: not written), and the
 // column sums of dz before rounding over each of `parts` row ranges
 // ([parts][cols] fp32; null: none).

@@ -10,7 +10,7 @@ namespace {
 
 constexpr uint32_t kMaxWidth = 1u << 20;        // n_in, n_out
 constexpr uint32_t kMaxRows = 0x7FFFFFFFu;      // tensor-copy coordinates are signed 32-bit
-constexpr uint64_t kMaxLd = 1ull << 30;         // row strides of the tensor copies stay far below their 2^40 bytes
+constexpr uint64_t kMaxLd = 1ull << 27;         // eight rows fit the tensor copies' signed 32-bit coordinates
 
 uint64_t up(uint64_t v, uint64_t a) { return (v + a - 1u) / a * a; }
 uint32_t ceil_div(uint64_t a, uint64_t b) { return static_cast<uint32_t>((a + b - 1u) / b); }
@@ -92,6 +92,28 @@ bool make_map(CUtensorMap* map, const MatrixView& m, uint32_t box_rows, bool bf1
               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// The map of a raw operand: groups of eight rows of `ld` values, from the
+// 16-byte boundary at or before the first value, are the map's rows, so that a
+// box takes every eighth row.  The last group ends with its last row's last
+// value: nothing behind it is read.
+bool make_raw_map(CUtensorMap* map, const MatrixView& m, uint32_t box_cols, uint32_t box_rows, bool bf16) {
+    if (m.rows < 8u) return true;  // nothing is copied
+    const EncodeTiled fn = encode_tiled();
+    if (!fn) return false;
+    const uintptr_t at = reinterpret_cast<uintptr_t>(m.ptr), start = at & ~static_cast<uintptr_t>(15u);
+    const cuuint64_t dims[2] = {(at - start) / 2u + 7u * m.ld + m.cols, m.rows / 8u};
+    const cuuint64_t strides[1] = {m.ld * 16u};
+    const cuuint32_t box[2] = {box_cols, box_rows}, elem[2] = {1u, 1u};
+    return fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2u, reinterpret_cast<void*>(start), dims, strides,
+              box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+// An operand's map (mn as in GemmArgs, n the box's rows of a K-major one).
+bool make_operand_map(CUtensorMap* map, const MatrixView& m, uint32_t raw, bool mn, uint32_t n, bool bf16) {
+    if (raw) return make_raw_map(map, m, mn ? kRawColsMn : kRawColsK, mn ? kGemmBK / 8u : n / 8u, bf16);
+    return make_map(map, m, mn ? kGemmBK : n, bf16);
+}
+
 // ------------------------------------------------------------------- plans
 // Tile width of an activation product: the number of waves of 128 x bn tiles
 // times the time of one, which grows with bn and has a part (the row panel's
@@ -99,8 +121,8 @@ bool make_map(CUtensorMap* map, const MatrixView& m, uint32_t box_rows, bool bf1
 // Up to K = 256 the epilogues take the time, and 128 columns have twice the
 // epilogue warps (65536 x 256 -> 256 with residual 27.9 us with 128 columns and
 // 31.5 with 256; at K = 512 both take 29.2).
-uint32_t pick_bn(uint32_t tiles_m, uint32_t n, uint32_t k, bool plain, uint32_t sms) {
-    const uint32_t widest = k <= 256u && !plain ? 128u : 256u;
+uint32_t pick_bn(uint32_t tiles_m, uint32_t n, uint32_t k, bool raw, uint32_t sms) {
+    const uint32_t widest = raw ? kGemmRawBN : k <= 256u ? 128u : 256u;
     uint32_t best = widest;
     uint64_t cost = ~0ull;
     for (uint32_t bn = widest; bn >= 64u; bn /= 2u) {
@@ -127,11 +149,10 @@ struct GradPlan {
     uint32_t bn, tiles_m, tiles_n, splits, k_steps, steps_per_split;
     uint64_t bytes;  // partial tiles
 };
-GradPlan plan_grad(const NerfB200Linear& d, bool plain, uint32_t sms) {
+GradPlan plan_grad(const NerfB200Linear& d, bool raw, uint32_t sms) {
     GradPlan p{};
-    p.pair = !plain && pair_pays(d.n_out, d.n_in, d.n_rows, sms);
-    // 256 columns need registers that the loading warps hold in a plain product.
-    p.bn = d.n_in <= 64u ? 64u : d.n_in <= 128u || plain ? 128u : 256u;
+    p.pair = !raw && pair_pays(d.n_out, d.n_in, d.n_rows, sms);
+    p.bn = d.n_in <= 64u ? 64u : d.n_in <= 128u || raw ? kGemmRawBN : 256u;
     p.tiles_m = ceil_div(d.n_out, p.pair ? 2u * kGemmBM : kGemmBM);
     p.tiles_n = ceil_div(d.n_in, p.bn);
     p.k_steps = ceil_div(d.n_rows, kGemmBK);
@@ -183,9 +204,9 @@ BackwardPlan plan_backward(const NerfB200Linear& d) {
     at += up(static_cast<uint64_t>(p.parts > blocks ? p.parts : blocks) * d.n_out * 4u, 256u);
     p.o_dw = at;
     // How the operands can be fed depends on the pointers: room for every way.
-    const uint64_t tma = plan_grad(d, false, p.sms).bytes, plain = plan_grad(d, true, p.sms).bytes;
+    const uint64_t tma = plan_grad(d, false, p.sms).bytes, raw = plan_grad(d, true, p.sms).bytes;
     const uint64_t one = static_cast<uint64_t>(blocks) * kGemmBM * narrow_bn(d) * 4u;
-    const uint64_t most = tma > plain ? tma : plain;
+    const uint64_t most = tma > raw ? tma : raw;
     at += one > most ? one : most;
     p.bytes = at ? at : 256u;
     return p;
@@ -206,16 +227,19 @@ bool valid_shape(const NerfB200Linear& d) {
     return d.ld_residual <= kMaxLd;  // as wide as the output it joins: checked by the calls
 }
 
-// The product with its operands' and outputs' maps; loads by warps where an
-// operand's rows do not start on 16-byte boundaries.  pair: the tiles are
-// those of a pair of CTAs.
+// The product with its operands' and outputs' maps; raw copies of an operand
+// whose rows do not start on 16-byte boundaries.  pair: the tiles are those of
+// a pair of CTAs.
 cudaError_t run_gemm(GemmArgs& g, int kind, uint32_t bn, bool pair, uint32_t sms, cudaStream_t s) {
     GemmMaps maps{};
-    const bool plain = g.a.vec < 8u || g.b.vec < 8u, bf16 = g.bf16 != 0u;
-    if (plain && pair) return cudaErrorInvalidValue;
-    g.a_box_rows = g.M >= kGemmBM ? kGemmBM : static_cast<uint32_t>(up(g.M, 8u));
-    if (!plain && (!make_map(&maps.a, g.a, g.a_mn ? kGemmBK : g.a_box_rows, bf16) ||
-                   !make_map(&maps.b, g.b, g.b_mn ? kGemmBK : pair ? bn / 2u : bn, bf16)))
+    const bool bf16 = g.bf16 != 0u;
+    g.a_raw = g.a.vec < 8u;
+    g.b_raw = g.b.vec < 8u;
+    const bool raw = g.a_raw || g.b_raw;
+    if (raw && pair) return cudaErrorInvalidValue;
+    g.a_box_rows = g.M >= kGemmBM || g.a_raw ? kGemmBM : static_cast<uint32_t>(up(g.M, 8u));
+    if (!make_operand_map(&maps.a, g.a, g.a_raw, g.a_mn, g.a_box_rows, bf16) ||
+        !make_operand_map(&maps.b, g.b, g.b_raw, g.b_mn, pair ? bn / 2u : bn, bf16))
         return cudaErrorNotSupported;
     g.y_tma = tma_rows(g.y);
     g.pre_tma = tma_rows(g.pre);
@@ -233,7 +257,7 @@ cudaError_t run_gemm(GemmArgs& g, int kind, uint32_t bn, bool pair, uint32_t sms
     }
     const uint64_t items = static_cast<uint64_t>(g.tiles_m) * g.tiles_n * g.splits, slots = pair ? sms / 2u : sms;
     const uint32_t blocks = static_cast<uint32_t>(items < slots ? items : slots) * (pair ? 2u : 1u);
-    return launch_gemm(g, kind, bn, plain ? kFeedPlain : pair ? kFeedPair : kFeedTma, maps, blocks, s);
+    return launch_gemm(g, kind, bn, raw ? kFeedRaw : pair ? kFeedPair : kFeedTma, maps, blocks, s);
 }
 // Few rows (run_cols) or tiles of 128 (run_rows)?  The first where every row
 // fits one column tile, or where the 128-row tiles would leave half of the SMs
@@ -261,10 +285,12 @@ cudaError_t run_cols(const GemmArgs& rows, cudaStream_t s, uint32_t sms) {
     g.steps_per_split = ceil_div(g.k_steps, splits);
     g.splits = ceil_div(g.k_steps, g.steps_per_split);
     GemmMaps maps{};
-    const bool plain = g.a.vec < 8u || g.b.vec < 8u, bf16 = g.bf16 != 0u;
-    if (!plain && (!make_map(&maps.a, g.a, g.a_mn ? kGemmBK : kGemmBM, bf16) || !make_map(&maps.b, g.b, bn, bf16)))
+    const bool bf16 = g.bf16 != 0u;
+    g.a_raw = g.a.vec < 8u;
+    g.b_raw = g.b.vec < 8u;
+    if (!make_operand_map(&maps.a, g.a, g.a_raw, g.a_mn, kGemmBM, bf16) || !make_operand_map(&maps.b, g.b, g.b_raw, false, bn, bf16))
         return cudaErrorNotSupported;
-    return launch_gemm_cols(g, bn, plain, maps, s);
+    return launch_gemm_cols(g, bn, g.a_raw || g.b_raw, maps, s);
 }
 // y = act(a b^T + bias) + res: picks the kernel, fills in the tiles and runs it.
 cudaError_t run_rows(GemmArgs& g, uint32_t sms, cudaStream_t s) {
