@@ -100,6 +100,20 @@ struct NarrowArgs {
 struct NarrowMaps {
     CUtensorMap dy, pre, x, w, dx, res;
 };
+// The input gradient of a layer with n_in, n_out <= 256, making dz on the way
+// (linear_dx.cu): dx, dz (null: dy itself), and eight parts of db a CTA.  Of the
+// maps w has boxes of 64 x 64, the others as for the narrow backward.
+constexpr uint32_t kDxMaxWidth = 256, kDxPartsPerBlock = 8;
+struct DxArgs {
+    uint32_t n, n_in, n_out, act, bf16;
+    MatrixView dx, res;  // res.ptr null: none
+    uint32_t dx_tma, res_tma;
+    void* dz;
+    uint64_t dz_ld;
+    float* db_part;  // null: none
+    uint32_t* error;
+};
+cudaError_t launch_dx(const DxArgs& a, const NarrowMaps& maps, uint32_t blocks, cudaStream_t s);
 cudaError_t launch_backward_narrow(const NarrowArgs& a, const NarrowMaps& maps, uint32_t blocks, cudaStream_t s);
 
 constexpr uint32_t kGemmBM = 128, kGemmBK = 64;

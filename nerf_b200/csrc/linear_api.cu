@@ -171,7 +171,9 @@ GradPlan plan_grad(const NerfB200Linear& d, bool raw, uint32_t sms) {
 // Layers whose whole backward one kernel does in one pass over the rows.
 bool narrow(const NerfB200Linear& d) { return d.n_in <= 128u && d.n_out <= 128u; }
 uint32_t narrow_bn(const NerfB200Linear& d) { return d.n_in <= 64u ? 64u : 128u; }
-uint32_t narrow_blocks(const NerfB200Linear& d, uint32_t sms) {
+// Layers whose input gradient makes dz on the way.
+bool dz_on_the_way(const NerfB200Linear& d) { return d.n_in <= kDxMaxWidth && d.n_out <= kDxMaxWidth; }
+uint32_t row_blocks(const NerfB200Linear& d, uint32_t sms) {  // of kernels with a CTA a 128-row tile
     const uint32_t tiles = ceil_div(d.n_rows, kGemmBM);
     return tiles < sms ? tiles : sms;
 }
@@ -200,12 +202,12 @@ BackwardPlan plan_backward(const NerfB200Linear& d) {
     p.o_dz = at;
     if (p.dz_needed) at += up(static_cast<uint64_t>(d.n_rows) * p.dz_ld * 2u, 256u);
     p.o_db = at;
-    const uint32_t blocks = narrow(d) ? narrow_blocks(d, p.sms) : 0u;
-    at += up(static_cast<uint64_t>(p.parts > blocks ? p.parts : blocks) * d.n_out * 4u, 256u);
+    const uint32_t blocks = dz_on_the_way(d) ? row_blocks(d, p.sms) : 0u;
+    at += up(static_cast<uint64_t>(p.parts > kDxPartsPerBlock * blocks ? p.parts : kDxPartsPerBlock * blocks) * d.n_out * 4u, 256u);
     p.o_dw = at;
     // How the operands can be fed depends on the pointers: room for every way.
     const uint64_t tma = plan_grad(d, false, p.sms).bytes, raw = plan_grad(d, true, p.sms).bytes;
-    const uint64_t one = static_cast<uint64_t>(blocks) * kGemmBM * narrow_bn(d) * 4u;
+    const uint64_t one = narrow(d) ? static_cast<uint64_t>(blocks) * kGemmBM * narrow_bn(d) * 4u : 0u;
     const uint64_t most = tma > raw ? tma : raw;
     at += one > most ? one : most;
     p.bytes = at ? at : 256u;
@@ -277,9 +279,10 @@ cudaError_t run_cols(const GemmArgs& rows, cudaStream_t s, uint32_t sms) {
     g.tiles_m = ceil_div(g.M, kGemmBM);
     g.tiles_n = ceil_div(g.N, bn);
     g.k_steps = ceil_div(g.K, kGemmBK);
-    // As many parts of K as fill the SMs once, each at least two steps.
-    const uint64_t tiles = static_cast<uint64_t>(g.tiles_m) * g.tiles_n;
-    uint64_t splits = tiles >= sms ? 1u : sms / tiles;
+    // As many parts of K as fill the SMs, which hold two CTAs each but of the widest tile, and each part at least two
+    // steps (19 rows through 4096 x 4096: 10.0 us with 256 CTAs, 11.1 with 128; 100 rows: 28 us with 256, 15 with 128).
+    const uint64_t tiles = static_cast<uint64_t>(g.tiles_m) * g.tiles_n, room = bn <= 64u ? 2u * sms : sms;
+    uint64_t splits = tiles >= room ? 1u : room / tiles;
     if (splits > kColsMaxCluster) splits = kColsMaxCluster;
     if (splits > ceil_div(g.k_steps, 2u)) splits = ceil_div(g.k_steps, 2u);
     g.steps_per_split = ceil_div(g.k_steps, splits);
@@ -399,7 +402,15 @@ NERF_API NerfStatus nerf_b200_linear_backward(const NerfB200Linear* desc, const 
     const MatrixView xv = view(x, ld_or(d.ld_x, d.n_in), d.n_rows, d.n_in), wv = view(weight, ld_or(d.ld_weight, d.n_in), d.n_out, d.n_in);
     const MatrixView prev = view(pre, ld_or(d.ld_pre, d.n_out), d.n_rows, d.n_out);
     const MatrixView resv = view(dx_residual, ld_or(d.ld_residual, d.n_in), d.n_rows, d.n_in), dxv = view(dx, ld_or(d.ld_dx, d.n_in), d.n_rows, d.n_in);
-    if (dx && dweight && narrow(d) && dyv.vec >= 8u && xv.vec >= 8u && wv.vec >= 8u && (d.activation == kActNone || prev.vec >= 8u)) {
+    const uint32_t blocks = row_blocks(d, p.sms);
+    const bool b = bf16 != 0u, copied = dyv.vec >= 8u && wv.vec >= 8u && (d.activation == kActNone || prev.vec >= 8u);
+    NarrowMaps maps{};
+    const auto make_maps = [&](uint32_t w_rows) {
+        return make_map(&maps.dy, dyv, kGemmBM, b) && (d.activation == kActNone || make_map(&maps.pre, prev, kGemmBM, b)) &&
+               make_map(&maps.w, wv, w_rows, b) && (!tma_rows(dxv) || make_map(&maps.dx, dxv, 32u, b)) &&
+               (!resv.ptr || resv.vec < 8u || make_map(&maps.res, resv, 32u, b));
+    };
+    if (dx && dweight && narrow(d) && copied && xv.vec >= 8u) {
         NarrowArgs a{};
         a.n = d.n_rows;
         a.n_in = d.n_in;
@@ -413,13 +424,7 @@ NERF_API NerfStatus nerf_b200_linear_backward(const NerfB200Linear* desc, const 
         a.partials = reinterpret_cast<float*>(ws + p.o_dw);
         a.db_part = dbias ? reinterpret_cast<float*>(ws + p.o_db) : nullptr;
         a.error = error_word;
-        const uint32_t blocks = narrow_blocks(d, p.sms), ob = d.n_out <= 64u ? 64u : 128u;
-        NarrowMaps maps{};
-        const bool b = bf16 != 0u;
-        if (!make_map(&maps.dy, dyv, kGemmBM, b) || (a.act != kActNone && !make_map(&maps.pre, prev, kGemmBM, b)) ||
-            !make_map(&maps.x, xv, kGemmBM, b) || !make_map(&maps.w, wv, ob, b) || (a.dx_tma && !make_map(&maps.dx, dxv, 32u, b)) ||
-            (a.res_tma && !make_map(&maps.res, resv, 32u, b)))
-            return NERF_STATUS_CUDA_ERROR;
+        if (!make_maps(d.n_out <= 64u ? 64u : 128u) || !make_map(&maps.x, xv, kGemmBM, b)) return NERF_STATUS_CUDA_ERROR;
         if (launch_backward_narrow(a, maps, blocks, s) != cudaSuccess) return NERF_STATUS_CUDA_ERROR;
         r.partials = a.partials;
         r.splits = blocks;
@@ -429,9 +434,29 @@ NERF_API NerfStatus nerf_b200_linear_backward(const NerfB200Linear* desc, const 
         r.parts = blocks;
         return launch_grad_reduce(r, s) == cudaSuccess ? NERF_STATUS_OK : NERF_STATUS_CUDA_ERROR;
     }
+    const bool on_the_way = dx && dz_on_the_way(d) && copied && (p.dz_needed || dbias);
+    if (on_the_way) {
+        DxArgs a{};
+        a.n = d.n_rows;
+        a.n_in = d.n_in;
+        a.n_out = d.n_out;
+        a.act = d.activation;
+        a.bf16 = bf16;
+        a.dx = dxv;
+        a.res = resv;
+        a.dx_tma = tma_rows(dxv);
+        a.res_tma = resv.ptr && resv.vec >= 8u;
+        a.dz = p.dz_needed && dweight ? ws + p.o_dz : nullptr;
+        a.dz_ld = p.dz_ld;
+        a.db_part = dbias ? reinterpret_cast<float*>(ws + p.o_db) : nullptr;
+        a.error = error_word;
+        if (!make_maps(64u)) return NERF_STATUS_CUDA_ERROR;
+        if (launch_dx(a, maps, blocks, s) != cudaSuccess) return NERF_STATUS_CUDA_ERROR;
+        r.parts = kDxPartsPerBlock * blocks;
+    }
     const bool dz_written = p.dz_needed && (dx || dweight);
     const MatrixView dzv = p.dz_needed ? view(ws + p.o_dz, p.dz_ld, d.n_rows, d.n_out) : dyv;
-    if (dz_written || dbias) {
+    if (!on_the_way && (dz_written || dbias)) {
         DzArgs a{};
         a.dy = dyv;
         a.pre = prev;
@@ -444,7 +469,7 @@ NERF_API NerfStatus nerf_b200_linear_backward(const NerfB200Linear* desc, const 
         a.act = d.activation;
         if (launch_dz(a, s) != cudaSuccess) return NERF_STATUS_CUDA_ERROR;
     }
-    if (dx) {
+    if (dx && !on_the_way) {
         GemmArgs g{};
         g.M = d.n_rows;
         g.N = d.n_in;

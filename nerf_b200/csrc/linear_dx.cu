@@ -1,0 +1,279 @@
+// linear_dx.cu -- the input gradient of a layer with n_in, n_out <= 256,
+// making dz on the way.
+//
+//   dz = dy act'(pre),  dx = dz W + r,  and the column sums of dz
+//
+// One column tile holds all of dx, so every row's dz is needed in one place
+// only: the copies bring boxes of dy, pre and W, eight warps replace dy by dz in
+// place, write it out once for the weight gradient and keep its column sums in
+// registers, and the tensor core reads it from shared memory.  As a pass of its
+// own dz costs a read of dy and pre and, for the product, one of dz more.
+// Wider layers have several column tiles and would make dz in each.
+//
+// Warps: 0 copies of dy and pre, 1 MMA, 2 tensor-memory allocation, 3 copies of
+// W, 4-11 dz, 12-19 two epilogue groups in turn.
+#include <atomic>
+
+#include "linear_common.cuh"
+
+namespace nb {
+namespace {
+
+constexpr uint32_t kRows = 128, kBox = kRows * 128u;  // 128 rows x 64 values
+constexpr uint32_t kDzWarps = 8, kThreads = 32u * (4u + kDzWarps + 8u);
+constexpr uint32_t kMaxK = 4;  // 64-value steps of n_out
+static_assert(kDxPartsPerBlock == kDzWarps, "one part of db a warp");
+
+template <uint32_t IB>
+struct DxShape {
+    static constexpr uint32_t kStage = 2u * kBox + IB * 128u;  // dy (then dz), pre, 64 rows of W
+    static constexpr uint32_t kStages = IB == 256u ? 3u : 4u;
+    static constexpr uint32_t kSmem = 1024u + kStages * kStage + 8u * kSlabBytes;
+    static_assert(kSmem <= 232448u - 512u, "shared memory of one CTA");
+};
+struct DxBarriers {
+    uint64_t full[4], empty[4], dz[4];
+    uint64_t acc_full[2], acc_empty[2];
+    uint64_t res[8];
+    uint64_t drain;
+    uint32_t tmem_base;
+};
+
+template <uint32_t IB, uint32_t ACT>
+__global__ void __launch_bounds__(kThreads, 1) k_dx(const DxArgs a, const __grid_constant__ NarrowMaps maps) {
+    using S = DxShape<IB>;
+    constexpr uint32_t kCols = tmem_cols(2u * IB);
+    extern __shared__ unsigned char smem_raw[];
+    __shared__ DxBarriers bar;
+    unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+    unsigned char* slabs = smem + S::kStages * S::kStage;
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
+    const bool bf16 = a.bf16 != 0u;
+    const uint32_t tiles = (a.n + kRows - 1u) / kRows, k_steps = (a.n_out + 63u) / 64u;
+    const uint32_t mine = blockIdx.x < tiles ? (tiles - 1u - blockIdx.x) / gridDim.x + 1u : 0u;  // this CTA's tiles
+
+    if (threadIdx.x == 0u) {
+        for (uint32_t i = 0; i < S::kStages; ++i) {
+            umma::mbar_init(&bar.full[i], 1u);
+            umma::mbar_init(&bar.empty[i], 1u);
+            umma::mbar_init(&bar.dz[i], kDzWarps);
+        }
+        for (uint32_t i = 0; i < 2u; ++i) {
+            umma::mbar_init(&bar.acc_full[i], 1u);
+            umma::mbar_init(&bar.acc_empty[i], 4u);
+        }
+        for (uint32_t i = 0; i < 8u; ++i) umma::mbar_init(&bar.res[i], 1u);
+        umma::mbar_init(&bar.drain, 1u);
+        umma::fence_mbar_init();
+    }
+    if (warp == 2u) {
+        umma::tmem_alloc(&bar.tmem_base, kCols);
+        umma::tmem_relinquish();
+    }
+    umma::fence_before_sync();
+    __syncthreads();
+    umma::fence_after_sync();
+    after_previous();
+    let_next_start();
+    const uint32_t tmem = bar.tmem_base, steps = mine * k_steps;
+
+    if ((warp == 0u || warp == 3u) && lane == 0u) {
+        // ---- copies
+        const uint32_t bytes = kBox * (ACT != kActNone ? 2u : 1u) + IB * 128u;
+        uint32_t i = 0;
+        bool ok = true;
+        for (; i < steps; ++i) {
+            const uint32_t s = i % S::kStages, ks = i % k_steps;
+            const int32_t row = static_cast<int32_t>((blockIdx.x + i / k_steps * gridDim.x) * kRows);
+            ok = tma::wait(&bar.empty[s], (i / S::kStages + 1u) & 1u);
+            if (!ok) break;
+            unsigned char* st = smem + s * S::kStage;
+            if (warp == 0u) {
+                tma::expect_tx(&bar.full[s], bytes);
+                tma::load_2d(smem_u32(st), &maps.dy, 64 * ks, row, &bar.full[s]);
+                if (ACT != kActNone) tma::load_2d(smem_u32(st + kBox), &maps.pre, 64 * ks, row, &bar.full[s]);
+            } else {
+                for (uint32_t j = 0; j < IB / 64u; ++j) tma::load_2d(smem_u32(st + 2u * kBox + j * 8192u), &maps.w, 64 * j, 64 * ks, &bar.full[s]);
+            }
+        }
+        if (!ok) {  // copies in flight: wait for them before the shared memory goes
+            atomicOr(a.error, 1u);
+            for (uint32_t k = i > S::kStages ? i - S::kStages : 0u; k < i; ++k) tma::wait(&bar.full[k % S::kStages], (k / S::kStages) & 1u);
+        }
+    } else if (warp == 1u && lane == 0u) {
+        // ---- MMA issuer
+        const uint32_t idesc = tma::idesc_16bit(128u, IB, 0u, 1u, a.bf16);
+        bool ok = true;
+        for (uint32_t i = 0; i < steps && ok; ++i) {
+            const uint32_t s = i % S::kStages, ks = i % k_steps, t = i / k_steps, b = t & 1u;
+            if ((ks == 0u && !tma::wait(&bar.acc_empty[b], (t / 2u + 1u) & 1u)) || !tma::wait(&bar.full[s], (i / S::kStages) & 1u) ||
+                !tma::wait(&bar.dz[s], (i / S::kStages) & 1u)) {
+                ok = false;
+                break;
+            }
+            umma::fence_after_sync();
+            const uint32_t dz = smem_u32(smem + s * S::kStage), w = dz + 2u * kBox;
+#pragma unroll
+            for (uint32_t k = 0; k < 4u; ++k)
+                umma::mma_f16(tmem + b * IB, tma::desc_sw128(dz + 32u * k, 16u, 1024u), tma::desc_sw128(w + 2048u * k, 8192u, 1024u), idesc,
+                              ks > 0u || k > 0u ? 1u : 0u);
+            umma::commit(&bar.empty[s]);
+            if (ks + 1u == k_steps) umma::commit(&bar.acc_full[b]);
+        }
+        if (!ok) {
+            atomicOr(a.error, 1u);
+            umma::commit(&bar.drain);
+            tma::wait(&bar.drain, 0u);
+        }
+    } else if (warp >= 4u && warp < 4u + kDzWarps) {
+        // ---- dz in place of dy, out to memory, and its column sums: a thread keeps to one 8-column piece of each step
+        constexpr uint32_t kStep = 4u * kDzWarps;  // rows at a time
+        const uint32_t t = threadIdx.x - 128u, p = t & 7u, r0 = t >> 3;
+        float sums[kMaxK][8];
+#pragma unroll
+        for (uint32_t k = 0; k < kMaxK; ++k)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) sums[k][j] = 0.0f;
+        bool ok = true;
+        for (uint32_t tile = 0; tile < mine && ok; ++tile) {
+            const uint64_t row0 = static_cast<uint64_t>(blockIdx.x + tile * gridDim.x) * kRows + r0;
+#pragma unroll
+            for (uint32_t ks = 0; ks < kMaxK; ++ks) {
+                if (ks >= k_steps || !ok) break;
+                const uint32_t i = tile * k_steps + ks, s = i % S::kStages;
+                ok = __all_sync(0xffffffffu, tma::wait(&bar.full[s], (i / S::kStages) & 1u));
+                if (!ok) break;
+                unsigned char* d = smem + s * S::kStage;
+                const unsigned char* z = d + kBox;
+                uint16_t* out = a.dz ? static_cast<uint16_t*>(a.dz) + row0 * a.dz_ld + 64u * ks + 8u * p : nullptr;
+                const bool cols = 64u * ks + 8u * p < a.n_out;  // rows of dz are padded to a multiple of 8 values
+#pragma unroll
+                for (uint32_t k = 0; k < kRows / kStep; ++k) {
+                    const uint32_t at = slab_at(r0 + kStep * k, p);
+                    const uint4 ud = *reinterpret_cast<const uint4*>(d + at);
+                    const uint4 uz = ACT != kActNone ? *reinterpret_cast<const uint4*>(z + at) : make_uint4(0u, 0u, 0u, 0u);
+                    const uint32_t dw[4] = {ud.x, ud.y, ud.z, ud.w}, zw[4] = {uz.x, uz.y, uz.z, uz.w};
+                    uint32_t o[4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const float2 dd = unpack_16(dw[j], bf16), zz = unpack_16(zw[j], bf16);
+                        const float f0 = dact_f(dd.x, zz.x, ACT), f1 = dact_f(dd.y, zz.y, ACT);
+                        sums[ks][2 * j] += f0;
+                        sums[ks][2 * j + 1] += f1;
+                        o[j] = pack_16(f0, f1, bf16);  // the tensor cores take 16-bit operands
+                    }
+                    if (ACT != kActNone) {
+                        const uint4 u = make_uint4(o[0], o[1], o[2], o[3]);
+                        *reinterpret_cast<uint4*>(d + at) = u;
+                        if (out && cols && row0 + kStep * k < a.n) *reinterpret_cast<uint4*>(out + kStep * k * a.dz_ld) = u;
+                    }
+                }
+                umma::fence_async_smem();
+                __syncwarp();
+                if (lane == 0u) tma::arrive(&bar.dz[s]);
+            }
+        }
+        if (!ok) atomicOr(a.error, 1u);
+        if (a.db_part) {  // one part a warp: four of its lanes hold each column
+            float* part = a.db_part + static_cast<uint64_t>(kDzWarps * blockIdx.x + warp - 4u) * a.n_out;
+#pragma unroll
+            for (uint32_t k = 0; k < kMaxK; ++k) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    float v = sums[k][j];
+                    v += __shfl_xor_sync(0xffffffffu, v, 8);
+                    v += __shfl_xor_sync(0xffffffffu, v, 16);
+                    const uint32_t c = 64u * k + 8u * p + j;
+                    if (lane < 8u && c < a.n_out) part[c] = v;
+                }
+            }
+        }
+    } else if (warp >= 4u + kDzWarps) {
+        // ---- epilogue: group h takes every other tile
+        const uint32_t e = warp - 4u - kDzWarps, q = warp & 3u, h = e >> 2, taddr = tmem + h * IB + ((32u * q) << 16);
+        unsigned char* slab = slabs + e * kSlabBytes;
+        uint32_t res_parity = 0;
+        for (uint32_t i = h; i < mine; i += 2u) {
+            const uint32_t m0 = (blockIdx.x + i * gridDim.x) * kRows + 32u * q;
+            const uint32_t rows = m0 < a.n ? min(32u, a.n - m0) : 0u;
+            if (!__all_sync(0xffffffffu, tma::wait(&bar.acc_full[h], (i / 2u) & 1u))) {
+                atomicOr(a.error, 1u);
+                break;
+            }
+            umma::fence_after_sync();
+#pragma unroll 1
+            for (uint32_t c0 = 0; c0 < IB && c0 < a.n_in; c0 += 64u) {
+                const uint32_t cols = min(64u, a.n_in - c0);
+                if (lane == 0u) {
+                    tma::store_wait_read<0>();
+                    if (a.res_tma && rows) {
+                        tma::expect_tx(&bar.res[e], kSlabBytes);
+                        tma::load_2d(smem_u32(slab), &maps.res, c0, m0, &bar.res[e]);
+                    }
+                }
+                __syncwarp();
+                if (a.res.ptr && !a.res_tma) {
+                    unsigned char* src = static_cast<unsigned char*>(const_cast<void*>(a.res.ptr)) + 2u * (m0 * a.res.ld + c0);
+                    slab_copy<2, false>(slab, src, a.res.ld, rows, cols, a.res.vec >= 8u, lane);
+                    __syncwarp();
+                }
+                if (a.res_tma && rows) {
+                    if (!tma::wait(&bar.res[e], res_parity)) atomicOr(a.error, 1u);
+                    res_parity ^= 1u;
+                    __syncwarp();
+                }
+#pragma unroll
+                for (uint32_t g = 0; g < 2u; ++g) {
+                    float v[32];
+                    umma::tmem_ld32(taddr + c0 + 32u * g, v);
+                    if (a.res.ptr) slab_add32(slab, lane, g, v, bf16);
+                    slab_put32(slab, lane, g, v, bf16);
+                }
+                slab_out(slab, a.dx, a.dx_tma != 0u, &maps.dx, m0, c0, rows, cols, lane);
+            }
+            umma::fence_before_sync();
+            __syncwarp();
+            if (lane == 0u) tma::arrive(&bar.acc_empty[h]);
+        }
+        if (lane == 0u) tma::store_wait_all();
+    }
+    __syncwarp();
+    umma::fence_before_sync();
+    __syncthreads();
+    if (warp == 2u) umma::tmem_dealloc(tmem, kCols);
+}
+
+template <uint32_t IB, uint32_t ACT>
+cudaError_t launch_t(const DxArgs& a, const NarrowMaps& maps, uint32_t blocks, cudaStream_t s) {
+    constexpr uint32_t smem = DxShape<IB>::kSmem;
+    static std::atomic<bool> done[64];  // the attribute belongs to the device
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+    if (!done[dev]) {
+        e = cudaFuncSetAttribute(k_dx<IB, ACT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        if (e != cudaSuccess) return e;
+        done[dev] = true;
+    }
+    return launch_after(k_dx<IB, ACT>, dim3(blocks), kThreads, smem, 1u, s, a, maps);
+}
+template <uint32_t IB>
+cudaError_t launch_act(const DxArgs& a, const NarrowMaps& maps, uint32_t blocks, cudaStream_t s) {
+    switch (a.act) {
+        case kActRelu: return launch_t<IB, kActRelu>(a, maps, blocks, s);
+        case kActSilu: return launch_t<IB, kActSilu>(a, maps, blocks, s);
+        case kActGelu: return launch_t<IB, kActGelu>(a, maps, blocks, s);
+        case kActSigmoid: return launch_t<IB, kActSigmoid>(a, maps, blocks, s);
+        default: return launch_t<IB, kActNone>(a, maps, blocks, s);
+    }
+}
+
+}  // namespace
+
+cudaError_t launch_dx(const DxArgs& a, const NarrowMaps& maps, uint32_t blocks, cudaStream_t s) {
+    if (a.n == 0u || a.n_in == 0u || a.n_out == 0u || a.n_in > kDxMaxWidth || a.n_out > 64u * kMaxK) return cudaErrorInvalidValue;
+    return a.n_in <= 128u ? launch_act<128u>(a, maps, blocks, s) : launch_act<256u>(a, maps, blocks, s);
+}
+
+}  // namespace nb

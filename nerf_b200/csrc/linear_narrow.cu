@@ -7,7 +7,7 @@
 // against 2 (2 n_in + 2 n_out) bytes.  Written as separate kernels dz goes out
 // to memory and comes back twice; here it never leaves the SM.  Per 128-row
 // tile the copies bring dy, pre and x into shared memory as swizzled boxes,
-// four warps replace dy by dz in place and keep the column sums in registers,
+// four or eight warps replace dy by dz in place and keep the column sums in registers,
 // and the tensor core reads the same dz boxes twice: K-major against W (kept
 // in shared memory for the CTA's life) for dx, MN-major against x for dW.  dx
 // is drained tile by tile by two groups of four warps in turn; dW accumulates
@@ -34,9 +34,10 @@ struct NarrowShape {
     static constexpr uint32_t kStages = OB + IB == 128u ? 4u : OB + IB == 192u ? 3u - (OB == 128u ? 1u : 0u) : 2u;
     static constexpr uint32_t kPres = OB + IB == 128u ? 3u : OB + IB == 192u ? 2u : 1u;  // pre, until dz is made
     static constexpr uint32_t kSmem = 1024u + kStages * kStage + kPres * kDy + kW + 8u * kSlabBytes;
+    static constexpr uint32_t kDzWarps = IB == 64u ? 8u : 4u;  // eight where the sums of dW leave registers for them
+    static constexpr uint32_t kThreads = 32u * (4u + kDzWarps + 8u);
     static_assert(kSmem <= 232448u - 512u, "shared memory of one CTA");
 };
-constexpr uint32_t kThreads = 512;
 
 struct NarrowBarriers {
     uint64_t full[4], empty[4], dz[4];
@@ -48,7 +49,7 @@ struct NarrowBarriers {
 };
 
 template <uint32_t OB, uint32_t IB, uint32_t ACT>
-__global__ void __launch_bounds__(kThreads, 1) k_backward_narrow(const NarrowArgs a, const __grid_constant__ NarrowMaps maps) {
+__global__ void __launch_bounds__(NarrowShape<OB, IB>::kThreads, 1) k_backward_narrow(const NarrowArgs a, const __grid_constant__ NarrowMaps maps) {
     using S = NarrowShape<OB, IB>;
     constexpr uint32_t kCols = tmem_cols(4u * IB);
     extern __shared__ unsigned char smem_raw[];
@@ -66,11 +67,11 @@ __global__ void __launch_bounds__(kThreads, 1) k_backward_narrow(const NarrowArg
         for (uint32_t i = 0; i < S::kStages; ++i) {
             umma::mbar_init(&bar.full[i], 1u);
             umma::mbar_init(&bar.empty[i], 1u);
-            umma::mbar_init(&bar.dz[i], 4u);
+            umma::mbar_init(&bar.dz[i], S::kDzWarps);
         }
         for (uint32_t i = 0; i < S::kPres; ++i) {
             umma::mbar_init(&bar.pre_full[i], 1u);
-            umma::mbar_init(&bar.pre_empty[i], 4u);
+            umma::mbar_init(&bar.pre_empty[i], S::kDzWarps);
         }
         for (uint32_t i = 0; i < 2u; ++i) {
             umma::mbar_init(&bar.d1_full[i], 1u);
@@ -159,9 +160,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_backward_narrow(const NarrowArg
             umma::commit(&bar.drain);
             tma::wait(&bar.drain, 0u);
         }
-    } else if (warp >= 4u && warp < 8u) {
+    } else if (warp >= 4u && warp < 4u + S::kDzWarps) {
         // ---- dz in place of dy; a thread keeps to one 8-column piece
-        constexpr uint32_t kPieces = OB / 8u, kStep = 128u / kPieces;
+        constexpr uint32_t kDzThreads = 32u * S::kDzWarps, kPieces = OB / 8u, kStep = kDzThreads / kPieces;
         const uint32_t t = threadIdx.x - 128u, p = t % kPieces, r0 = t / kPieces, box = (p >> 3) * kBoxBytes;
         float sums[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
         bool ok = true;
@@ -203,22 +204,22 @@ __global__ void __launch_bounds__(kThreads, 1) k_backward_narrow(const NarrowArg
             // A column's sums over the threads that kept to its piece, through the room of pre.  Every warp comes to
             // both barriers, also one whose wait ran out.
             float* acc = reinterpret_cast<float*>(pres);
-            asm volatile("bar.sync 1, 128;\n" ::: "memory");
+            asm volatile("bar.sync 1, %0;\n" ::"n"(kDzThreads) : "memory");
 #pragma unroll
             for (int j = 0; j < 8; ++j)
                 if (ok) acc[t * 9u + j] = sums[j];
-            asm volatile("bar.sync 1, 128;\n" ::: "memory");
-            for (uint32_t c = t; c < a.n_out && ok; c += 128u) {
+            asm volatile("bar.sync 1, %0;\n" ::"n"(kDzThreads) : "memory");
+            for (uint32_t c = t; c < a.n_out && ok; c += kDzThreads) {
                 float v = 0.0f;
                 for (uint32_t k = 0; k < kStep; ++k) v += acc[(k * kPieces + (c >> 3)) * 9u + (c & 7u)];
                 a.db_part[static_cast<uint64_t>(blockIdx.x) * a.n_out + c] = v;
             }
         }
-    } else if (warp >= 8u) {
+    } else if (warp >= 4u + S::kDzWarps) {
         // ---- epilogue: group h takes every other tile's dx, and half of the columns of every dW chunk
         constexpr uint32_t kHalf = IB / 2u;
-        const uint32_t q = warp & 3u, h = (warp >> 2) - 2u, row = 32u * q + lane, lane_base = (32u * q) << 16;
-        unsigned char* slab = slabs + (warp - 8u) * kSlabBytes;
+        const uint32_t e = warp - 4u - S::kDzWarps, q = warp & 3u, h = e >> 2, row = 32u * q + lane, lane_base = (32u * q) << 16;
+        unsigned char* slab = slabs + e * kSlabBytes;
         float s[kHalf];
 #pragma unroll
         for (uint32_t i = 0; i < kHalf; ++i) s[i] = 0.0f;
@@ -237,8 +238,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_backward_narrow(const NarrowArg
                     if (lane == 0u) {
                         tma::store_wait_read<0>();
                         if (a.res_tma && rows) {
-                            tma::expect_tx(&bar.res[warp - 8u], kSlabBytes);
-                            tma::load_2d(smem_u32(slab), &maps.res, c0, m0, &bar.res[warp - 8u]);
+                            tma::expect_tx(&bar.res[e], kSlabBytes);
+                            tma::load_2d(smem_u32(slab), &maps.res, c0, m0, &bar.res[e]);
                         }
                     }
                     __syncwarp();
@@ -248,7 +249,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_backward_narrow(const NarrowArg
                         __syncwarp();
                     }
                     if (a.res_tma && rows) {
-                        if (!tma::wait(&bar.res[warp - 8u], res_parity)) atomicOr(a.error, 1u);
+                        if (!tma::wait(&bar.res[e], res_parity)) atomicOr(a.error, 1u);
                         res_parity ^= 1u;
                         __syncwarp();
                     }
@@ -309,7 +310,7 @@ cudaError_t launch_t(const NarrowArgs& a, const NarrowMaps& maps, uint32_t block
         if (e != cudaSuccess) return e;
         done[dev] = true;
     }
-    return launch_after(k_backward_narrow<OB, IB, ACT>, dim3(blocks), kThreads, smem, 1u, s, a, maps);
+    return launch_after(k_backward_narrow<OB, IB, ACT>, dim3(blocks), NarrowShape<OB, IB>::kThreads, smem, 1u, s, a, maps);
 }
 template <uint32_t OB, uint32_t IB>
 cudaError_t launch_act(const NarrowArgs& a, const NarrowMaps& maps, uint32_t blocks, cudaStream_t s) {
