@@ -20,8 +20,9 @@
 //               and half of B, so the tensor cores read 8 KB of shared memory
 //               per 64 cycles of MMA and SM instead of 12 KB, more than it
 //               delivers (128 bytes a cycle).
-//   kFeedRaw    rows that do not start on 16-byte boundaries: copied raw,
-//               and moved into place by eight more warps.
+//   kFeedRaw, kFeedRawShort
+//               rows that do not start on 16-byte boundaries: copied raw, and
+//               moved into place by eight or four more warps.
 #include <atomic>
 
 #include "linear_common.cuh"
@@ -39,13 +40,12 @@ constexpr uint32_t kMaxStages = 8;
 // of any length are a multiple of 16 bytes, so the rows r, r + 8, r + 16, ...
 // all lie alike: one copy takes a box's rows of one residue mod 8, 72 (K-major)
 // or 136 (MN-major) values each from the 16-byte boundary before the first one
-// wanted.  Warp w moves the rows of residue w into the swizzled box: a
+// wanted.  Warps then move the rows of a residue each into the swizzled box: a
 // shared-memory read or two, a permute and a write a row, and no trip to memory.
 // The copies' price is by the copy (a thread gets one off about every 128
 // cycles), so the operands' are issued by a warp each.  2000 x 4000 -> 4000 with
 // rows 4001 apart took 356 us with loads to registers instead, and 430 us with
 // 16-byte asynchronous copies by the warps that move the rows.
-constexpr uint32_t kLoadWarps = 8;
 constexpr uint32_t kRawRing = 2;  // steps of raw copies in shared memory
 
 // Bytes of one residue's copy: of n rows (K-major), of 64 rows x 128 columns (MN-major).
@@ -143,19 +143,20 @@ NB_DEV void tile_of(const GemmArgs& g, uint32_t t, uint32_t& tm, uint32_t& tn) {
 
 template <uint32_t BN, int KIND, int FEED>
 struct GemmShape {
-    static constexpr bool kPair = FEED == kFeedPair, kRaw = FEED == kFeedRaw;
+    static constexpr bool kPair = FEED == kFeedPair, kRaw = FEED == kFeedRaw || FEED == kFeedRawShort;
+    static constexpr uint32_t kLoaders = FEED == kFeedRaw ? 8u : FEED == kFeedRawShort ? 4u : 0u;
     static constexpr uint32_t kBoxN = kPair ? BN / 2u : BN;  // rows of B in this CTA's shared memory
     static constexpr uint32_t kStageBytes = kStageBytesA + kBoxN * 128u;
     // Epilogue groups of four warps, an accumulator each: tiles of up to 128
     // columns are bound by memory and by the latency of their epilogues.
-    static constexpr uint32_t kGroups = KIND == kGemmRows && BN <= 128u && !kRaw ? 4u : 2u;
+    static constexpr uint32_t kGroups = KIND == kGemmRows && BN <= 128u && FEED != kFeedRaw ? 4u : 2u;
     static constexpr uint32_t kRawBytes = raw_bytes(kBM) + raw_bytes(kBoxN);  // raw copies of a step
     static constexpr uint32_t kRaws = kRaw ? kRawRing * kRawBytes : 0u;
     static constexpr uint32_t kStages = kRaw ? 2u : kPair ? 5u : BN >= 128u ? 3u : 4u;
-    static constexpr uint32_t kSlabs = 2u;  // per epilogue warp
+    static constexpr uint32_t kSlabs = FEED == kFeedRawShort ? 1u : 2u;  // per epilogue warp
     static constexpr uint32_t kSmem = 1024u + kStages * kStageBytes + kRaws + 4u * kGroups * kSlabs * kSlabBytes + kGroups * BN * 2u;
     static constexpr uint32_t kFirstLoader = 4u + 4u * kGroups;
-    static constexpr uint32_t kThreads = 32u * (kFirstLoader + (kRaw ? kLoadWarps : 0u));
+    static constexpr uint32_t kThreads = 32u * (kFirstLoader + kLoaders);
     // Weight gradients of 256 columns keep 128 sums a thread: registers move
     // from the copying and issuing warps to the two groups that sum.
     static constexpr bool kRegs = KIND == kGemmGrad && BN == 256u;
@@ -186,13 +187,13 @@ __global__ void __launch_bounds__(GemmShape<BN, KIND, FEED>::kThreads, 1) k_gemm
 
     if (threadIdx.x == 0u) {
         for (uint32_t i = 0; i < kStages; ++i) {
-            umma::mbar_init(&bar.full[i], S::kRaw ? kLoadWarps + (g.a_raw && g.b_raw ? 0u : 1u) : 1u);
+            umma::mbar_init(&bar.full[i], S::kRaw ? S::kLoaders + (g.a_raw && g.b_raw ? 0u : 1u) : 1u);
             umma::mbar_init(&bar.empty[i], 1u);
         }
         for (uint32_t i = 0; S::kRaw && i < kRawRing; ++i) {
             for (uint32_t o = 0; o < 2u; ++o) {
                 umma::mbar_init(&bar.raw_full[o][i], 1u);
-                umma::mbar_init(&bar.raw_empty[o][i], kLoadWarps);
+                umma::mbar_init(&bar.raw_empty[o][i], S::kLoaders);
             }
         }
         for (uint32_t i = 0; i < S::kGroups; ++i) {
@@ -243,11 +244,11 @@ __global__ void __launch_bounds__(GemmShape<BN, KIND, FEED>::kThreads, 1) k_gemm
         bool ok = true;
         for (uint32_t it = first_item; it < items && ok; it += item_step) {
             const uint32_t split = it / tiles;
+            const uint32_t ks0 = split * g.steps_per_split, ks1 = min(g.k_steps, ks0 + g.steps_per_split);
             uint32_t tm, tn;
             tile_of(g, it - split * tiles, tm, tn);
             const uint32_t at = op ? tn * BN + rank * S::kBoxN : (tm * kCtas + rank) * kBM;  // the box's rows or columns
-            const uint32_t ks1 = min(g.k_steps, (split + 1u) * g.steps_per_split);
-            for (uint32_t ks = split * g.steps_per_split; ks < ks1; ++ks) {
+            for (uint32_t ks = ks0; ks < ks1; ++ks) {
                 const uint32_t k0 = ks * kBK;
                 if (raw) {
                     const uint32_t r = issued % kRawRing;
@@ -290,10 +291,10 @@ __global__ void __launch_bounds__(GemmShape<BN, KIND, FEED>::kThreads, 1) k_gemm
         bool ok = true;
         for (uint32_t it = first_item; it < items && ok; it += item_step) {
             const uint32_t split = it / tiles;
+            const uint32_t ks0 = split * g.steps_per_split, ks1 = min(g.k_steps, ks0 + g.steps_per_split);
             uint32_t tm, tn;
             tile_of(g, it - split * tiles, tm, tn);
-            const uint32_t ks1 = min(g.k_steps, (split + 1u) * g.steps_per_split);
-            for (uint32_t ks = split * g.steps_per_split; ks < ks1; ++ks, ++i) {
+            for (uint32_t ks = ks0; ks < ks1; ++ks, ++i) {
                 const uint32_t stage = i % kStages, r = i % kRawRing, turn = (i / kRawRing) & 1u;
                 ok = tma::wait(&bar.empty[stage], (i / kStages + 1u) & 1u) && (!g.a_raw || tma::wait(&bar.raw_full[0][r], turn)) &&
                      (!g.b_raw || tma::wait(&bar.raw_full[1][r], turn));
@@ -302,12 +303,13 @@ __global__ void __launch_bounds__(GemmShape<BN, KIND, FEED>::kThreads, 1) k_gemm
                 unsigned char* sa = smem + stage * kStageBytes;
                 const unsigned char* src = raws + r * S::kRawBytes;
                 if (g.a_raw) {
-                    raw_box<kBM>(sa, src, g.a, g.a_mn, tm * kBM, ks * kBK, w, lane);
+                    for (uint32_t v = w; v < 8u; v += S::kLoaders) raw_box<kBM>(sa, src, g.a, g.a_mn, tm * kBM, ks * kBK, v, lane);
                     __syncwarp();
                     if (lane == 0u) tma::arrive(&bar.raw_empty[0][r]);
                 }
                 if (g.b_raw) {
-                    raw_box<BN>(sa + kStageBytesA, src + raw_bytes(kBM), g.b, g.b_mn, tn * BN, ks * kBK, w, lane);
+                    for (uint32_t v = w; v < 8u; v += S::kLoaders)
+                        raw_box<BN>(sa + kStageBytesA, src + raw_bytes(kBM), g.b, g.b_mn, tn * BN, ks * kBK, v, lane);
                     __syncwarp();
                     if (lane == 0u) tma::arrive(&bar.raw_empty[1][r]);
                 }
@@ -379,12 +381,12 @@ __global__ void __launch_bounds__(GemmShape<BN, KIND, FEED>::kThreads, 1) k_gemm
         uint32_t acc = 0, parity = 0;
         bool ok = true;
         for (uint32_t it = first_item; it < items && ok; it += item_step) {
-            const uint32_t split = it / tiles, tile = it - split * tiles;
+            const uint32_t split = it / tiles;
+            const uint32_t ks0 = split * g.steps_per_split, ks1 = min(g.k_steps, ks0 + g.steps_per_split);
             uint32_t tm, tn;
-            tile_of(g, tile, tm, tn);
+            tile_of(g, it - split * tiles, tm, tn);
             const uint32_t m0 = (tm * kCtas + rank) * kBM + 32u * q, n0 = tn * BN + h * kHalf;
             const uint32_t rows = m0 < g.M ? min(32u, g.M - m0) : 0u;
-            const uint32_t ks0 = split * g.steps_per_split, ks1 = min(g.k_steps, (split + 1u) * g.steps_per_split);
             float s[kHalf];
 #pragma unroll
             for (uint32_t i = 0; i < kHalf; ++i) s[i] = 0.0f;
@@ -506,7 +508,7 @@ __global__ void __launch_bounds__(GemmShape<BN, KIND, FEED>::kThreads, 1) k_gemm
         // The next slab, when no store of this warp still reads it (ahead: slabs taken since the last store).
         const auto next_slab = [&](uint32_t ahead) -> unsigned char* {
             if (lane == 0u) {
-                if (ahead) tma::store_wait_read<S::kSlabs - 2u>();
+                if (ahead) tma::store_wait_read<(S::kSlabs > 1u ? S::kSlabs - 2u : 0u)>();
                 else tma::store_wait_read<S::kSlabs - 1u>();
             }
             __syncwarp();
@@ -515,9 +517,8 @@ __global__ void __launch_bounds__(GemmShape<BN, KIND, FEED>::kThreads, 1) k_gemm
             return p;
         };
         for (uint32_t it = first_item + acc * item_step; it < items; it += S::kGroups * item_step) {
-            const uint32_t split = it / tiles, tile = it - split * tiles;
             uint32_t tm, tn;
-            tile_of(g, tile, tm, tn);
+            tile_of(g, it, tm, tn);
             const uint32_t m0 = (tm * kCtas + rank) * kBM + 32u * q, n0 = tn * BN;
             const uint32_t rows = m0 < g.M ? min(32u, g.M - m0) : 0u;
             if (n0 != bias_n) {  // the tile's bias, kept while the columns stay the same
@@ -550,7 +551,16 @@ __global__ void __launch_bounds__(GemmShape<BN, KIND, FEED>::kThreads, 1) k_gemm
             for (uint32_t c0 = 0; c0 < BN && n0 + c0 < g.N; c0 += 64u) {
                 const uint32_t cols = min(64u, g.N - n0 - c0);
                 unsigned char* slab_z = g.pre.ptr ? next_slab(0u) : nullptr;
-                unsigned char* slab = next_slab(g.pre.ptr ? 1u : 0u);
+                if (S::kSlabs == 1u && g.pre.ptr) {  // one slab for both: z by itself first
+#pragma unroll
+                    for (uint32_t h = 0; h < 2u; ++h) {
+                        float v[32];
+                        load_z(v, taddr + c0 + 32u * h, bias_s + c0 + 32u * h, bf16);
+                        slab_put32(slab_z, lane, h, v, bf16);
+                    }
+                    slab_out(slab_z, g.pre, g.pre_tma != 0u, &maps.pre, m0, n0 + c0, rows, cols, lane);
+                }
+                unsigned char* slab = next_slab(S::kSlabs > 1u && g.pre.ptr ? 1u : 0u);
                 // The residual's rows come straight into the slab of the output, where this thread's row replaces
                 // them; the copy runs while z is made.
                 if (g.res_tma && rows && lane == 0u) {
@@ -566,7 +576,7 @@ __global__ void __launch_bounds__(GemmShape<BN, KIND, FEED>::kThreads, 1) k_gemm
                 for (uint32_t h = 0; h < 2u; ++h) {
                     float v[32];
                     load_z(v, taddr + c0 + 32u * h, bias_s + c0 + 32u * h, bf16);
-                    if (g.pre.ptr) slab_put32(slab_z, lane, h, v, bf16);
+                    if (S::kSlabs > 1u && g.pre.ptr) slab_put32(slab_z, lane, h, v, bf16);
                     act_row(v, g.act);
                     if (h == 0u && g.res_tma && rows) {
                         if (!tma::wait(&bar.res[warp - 4u], res_parity)) atomicOr(g.error, 1u);
@@ -576,7 +586,7 @@ __global__ void __launch_bounds__(GemmShape<BN, KIND, FEED>::kThreads, 1) k_gemm
                     if (g.res.ptr) slab_add32(slab, lane, h, v, bf16);
                     slab_put32(slab, lane, h, v, bf16);
                 }
-                if (g.pre.ptr) slab_out(slab_z, g.pre, g.pre_tma != 0u, &maps.pre, m0, n0 + c0, rows, cols, lane);
+                if (S::kSlabs > 1u && g.pre.ptr) slab_out(slab_z, g.pre, g.pre_tma != 0u, &maps.pre, m0, n0 + c0, rows, cols, lane);
                 slab_out(slab, g.y, g.y_tma != 0u, &maps.y, m0, n0 + c0, rows, cols, lane);
             }
             umma::fence_before_sync();
@@ -613,7 +623,7 @@ struct ColsShape {
     static constexpr uint32_t kStages = RAW && BN == 128u ? 2u : 4u;  // two or three CTAs an SM: the next launch's start while this one's end
     static constexpr uint32_t kRawBytes = raw_bytes(kBM) + raw_bytes(BN);  // raw copies of a step
     static constexpr uint32_t kSmem = 1024u + kStages * kStageBytes + (RAW ? kRawRing * kRawBytes : 0u);
-    static constexpr uint32_t kThreads = RAW ? 256u + 32u * kLoadWarps : 256u;
+    static constexpr uint32_t kLoaders = 8u, kThreads = RAW ? 256u + 32u * kLoaders : 256u;
     static_assert(kSmem <= 232448u - 512u, "shared memory of one CTA");
     static_assert(BN * kBM * 4u <= kStages * kStageBytes, "the partial tile takes the stages' place");
 };
@@ -635,13 +645,13 @@ __global__ void __launch_bounds__(ColsShape<BN, RAW>::kThreads) k_gemm_cols(cons
 
     if (threadIdx.x == 0u) {
         for (uint32_t i = 0; i < kStages; ++i) {
-            umma::mbar_init(&full[i], RAW ? kLoadWarps + (g.a_raw && g.b_raw ? 0u : 1u) : 1u);
+            umma::mbar_init(&full[i], RAW ? S::kLoaders + (g.a_raw && g.b_raw ? 0u : 1u) : 1u);
             umma::mbar_init(&empty[i], 1u);
         }
         for (uint32_t i = 0; RAW && i < kRawRing; ++i) {
             for (uint32_t o = 0; o < 2u; ++o) {
                 umma::mbar_init(&raw_full[o][i], 1u);
-                umma::mbar_init(&raw_empty[o][i], kLoadWarps);
+                umma::mbar_init(&raw_empty[o][i], S::kLoaders);
             }
         }
         umma::mbar_init(&acc_full, 1u);
@@ -996,6 +1006,13 @@ template <int KIND>
 cudaError_t launch_gemm_kind(const GemmArgs& g, uint32_t bn, int feed, const GemmMaps& maps, uint32_t blocks, cudaStream_t s) {
     if (feed == kFeedPair)
         return bn == kGemmPairBN && !(blocks & 1u) ? launch_gemm_t<kGemmPairBN, KIND, kFeedPair>(g, maps, blocks, s) : cudaErrorInvalidValue;
+    if (feed == kFeedRawShort) {
+        if constexpr (KIND == kGemmRows)
+            return bn == 64u           ? launch_gemm_t<64u, KIND, kFeedRawShort>(g, maps, blocks, s)
+                   : bn == kGemmRawBN ? launch_gemm_t<kGemmRawBN, KIND, kFeedRawShort>(g, maps, blocks, s)
+                                      : cudaErrorInvalidValue;
+        return cudaErrorInvalidValue;
+    }
     if (feed == kFeedRaw) {
         if (bn == 64u) return launch_gemm_t<64u, KIND, kFeedRaw>(g, maps, blocks, s);
         return bn == kGemmRawBN ? launch_gemm_t<kGemmRawBN, KIND, kFeedRaw>(g, maps, blocks, s) : cudaErrorInvalidValue;

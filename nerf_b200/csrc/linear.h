@@ -52,8 +52,9 @@ struct GemmMaps {
 };
 // How a product's operands reach shared memory: copied for one CTA a tile,
 // copied for a pair of CTAs on one 256 x 256 tile, or (one of them at least)
-// copied raw and moved into place by warps.
-enum GemmFeed : int { kFeedTma = 0, kFeedPair = 1, kFeedRaw = 2 };
+// copied raw and moved into place by warps: eight of them, or four with a short
+// K, where the epilogues need the threads.
+enum GemmFeed : int { kFeedTma = 0, kFeedPair = 1, kFeedRaw = 2, kFeedRawShort = 3 };
 constexpr uint32_t kGemmPairBN = 256, kGemmRawBN = 128;  // the widest tile of raw copies
 // Values a row of a raw box: 64 or 128 and what rounding its start down adds.
 constexpr uint32_t kRawColsK = 72, kRawColsMn = 136;

@@ -259,7 +259,11 @@ cudaError_t run_gemm(GemmArgs& g, int kind, uint32_t bn, bool pair, uint32_t sms
     }
     const uint64_t items = static_cast<uint64_t>(g.tiles_m) * g.tiles_n * g.splits, slots = pair ? sms / 2u : sms;
     const uint32_t blocks = static_cast<uint32_t>(items < slots ? items : slots) * (pair ? 2u : 1u);
-    return launch_gemm(g, kind, bn, raw ? kFeedRaw : pair ? kFeedPair : kFeedTma, maps, blocks, s);
+    // Raw copies of one step of K a tile leave the time to the epilogues, of more steps to the warps that place them
+    // (100003 x 63 -> 255: 46 us with four of those and sixteen epilogue warps, 56 us with eight and eight;
+    // 50000 x 201 -> 333: 73 and 57 us).
+    const bool one_step = kind == kGemmRows && g.k_steps == 1u;
+    return launch_gemm(g, kind, bn, !raw ? (pair ? kFeedPair : kFeedTma) : one_step ? kFeedRawShort : kFeedRaw, maps, blocks, s);
 }
 // Few rows (run_cols) or tiles of 128 (run_rows)?  The first where every row
 // fits one column tile, or where the 128-row tiles would leave half of the SMs
