@@ -17,6 +17,7 @@
 #include <new>
 
 #include "../../include/nerf_b200.h"
+#include "reach.h"
 #include "tma.cuh"
 
 namespace nb {
@@ -27,6 +28,7 @@ constexpr uint32_t kThreads = 256;
 constexpr uint32_t kFlight = 4;        // 16-byte loads in flight a thread
 constexpr uint32_t kMaxBlocks = 1024;  // partial sums of one launch
 constexpr uint32_t kTable = 512;       // tensors of one launch
+constexpr uint32_t kMaxTensors = 1u << 24;
 constexpr uint32_t kSmallBlocks = 8, kSmallChunks = 32;
 
 struct GradEntry {
@@ -447,7 +449,7 @@ uint32_t groups_of(uint32_t n) { return n == 0u ? 1u : (n + kTable - 1u) / kTabl
 
 NerfStatus norm_and_clip(const NerfB200GradTensor* ts, uint32_t n, float loss_scale, bool clip, float max_norm, NerfB200GradNorm* info,
                          void* workspace, uint64_t workspace_bytes, cudaStream_t s) {
-    if ((n && !ts) || !info || !workspace || !(loss_scale > 0.0f) || std::isinf(loss_scale)) return NERF_STATUS_INVALID_USAGE;
+    if (n > kMaxTensors || (n && !ts) || !info || !workspace || !(loss_scale > 0.0f) || std::isinf(loss_scale)) return NERF_STATUS_INVALID_USAGE;
     if (clip && !(max_norm >= 0.0f)) return NERF_STATUS_INVALID_USAGE;
     if ((reinterpret_cast<uintptr_t>(info) & 3u) || (reinterpret_cast<uintptr_t>(workspace) & 15u)) return NERF_STATUS_INVALID_USAGE;
     const uint64_t need = nerf_b200_grad_workspace_bytes(n);
@@ -460,6 +462,12 @@ NerfStatus norm_and_clip(const NerfB200GradTensor* ts, uint32_t n, float loss_sc
         const int apart = outputs_apart(ts, n);
         if (apart != 1) return apart == 0 ? NERF_STATUS_INVALID_USAGE : NERF_STATUS_FAILURE;
     }
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return NERF_STATUS_CUDA_ERROR;
+    Reach usable(dev);
+    if (!usable(info) || !usable(workspace)) return NERF_STATUS_INVALID_USAGE;
+    for (uint32_t i = 0; i < n; ++i)
+        if (ts[i].count && (!usable(ts[i].grad) || (clip && !usable(ts[i].out)))) return NERF_STATUS_INVALID_USAGE;
     GradPartial* parts = static_cast<GradPartial*>(workspace);
     GradInfo* gi = reinterpret_cast<GradInfo*>(info);
     if (n <= kTable && group_chunks(ts, n) <= kSmallChunks) {
@@ -495,6 +503,7 @@ NerfStatus norm_and_clip(const NerfB200GradTensor* ts, uint32_t n, float loss_sc
 extern "C" {
 
 NERF_API uint64_t nerf_b200_grad_workspace_bytes(uint32_t n_tensors) {
+    if (n_tensors > nb::kMaxTensors) return 0u;
     return static_cast<uint64_t>(nb::groups_of(n_tensors)) * nb::kMaxBlocks * sizeof(nb::GradPartial);
 }
 

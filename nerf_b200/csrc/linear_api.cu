@@ -4,6 +4,7 @@
 
 #include "../../include/nerf_b200.h"
 #include "linear.h"
+#include "reach.h"
 
 namespace nb {
 namespace {
@@ -36,18 +37,6 @@ uint32_t current_sms() {
     return sms[dev];
 }
 
-// Whether a kernel of the current device may read or write p: its own device
-// memory or managed memory.
-bool usable(const void* p, int dev) {
-    if (!p) return true;
-    cudaPointerAttributes at{};
-    if (cudaPointerGetAttributes(&at, p) != cudaSuccess) {
-        cudaGetLastError();
-        return false;
-    }
-    return at.type == cudaMemoryTypeManaged || (at.type == cudaMemoryTypeDevice && at.device == dev);
-}
-
 MatrixView view(const void* p, uint64_t ld, uint64_t rows, uint32_t cols) {
     MatrixView v{};
     v.ptr = p;
@@ -63,16 +52,7 @@ using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, 
                                  const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 EncodeTiled encode_tiled() {
-    static const EncodeTiled fn = [] {
-        void* p = nullptr;
-        cudaDriverEntryPointQueryResult res{};
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &res) != cudaSuccess ||
-            res != cudaDriverEntryPointSuccess) {
-            cudaGetLastError();
-            p = nullptr;
-        }
-        return reinterpret_cast<EncodeTiled>(p);
-    }();
+    static const EncodeTiled fn = reinterpret_cast<EncodeTiled>(driver_function("cuTensorMapEncodeTiled"));
     return fn;
 }
 // Whether the copy unit can store into a matrix: it writes whole 16-byte
@@ -330,9 +310,10 @@ NERF_API NerfStatus nerf_b200_linear_forward(const NerfB200Linear* desc, const v
     if (!aligned(error_word, 4u)) return NERF_STATUS_INVALID_USAGE;
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess) return NERF_STATUS_CUDA_ERROR;
+    Reach usable(dev);
     for (const void* p : all)
-        if (!usable(p, dev)) return NERF_STATUS_INVALID_USAGE;
-    if (!usable(error_word, dev)) return NERF_STATUS_INVALID_USAGE;
+        if (!usable(p)) return NERF_STATUS_INVALID_USAGE;
+    if (!usable(error_word)) return NERF_STATUS_INVALID_USAGE;
 
     const uint32_t sms = current_sms();
     GemmArgs g{};
@@ -370,7 +351,8 @@ NERF_API NerfStatus nerf_b200_linear_backward(const NerfB200Linear* desc, const 
     int dev = 0;
     if (d.n_rows == 0u) {  // sums over no rows
         if (cudaGetDevice(&dev) != cudaSuccess) return NERF_STATUS_CUDA_ERROR;
-        if (!usable(dweight, dev) || !usable(dbias, dev)) return NERF_STATUS_INVALID_USAGE;
+        Reach usable(dev);
+        if (!usable(dweight) || !usable(dbias)) return NERF_STATUS_INVALID_USAGE;
         if (d.accumulate) return NERF_STATUS_OK;
         if (dweight && cudaMemsetAsync(dweight, 0, es * d.n_out * d.n_in, s) != cudaSuccess) return NERF_STATUS_CUDA_ERROR;
         if (dbias && cudaMemsetAsync(dbias, 0, es * d.n_out, s) != cudaSuccess) return NERF_STATUS_CUDA_ERROR;
@@ -385,9 +367,10 @@ NERF_API NerfStatus nerf_b200_linear_backward(const NerfB200Linear* desc, const 
     const BackwardPlan p = plan_backward(d);
     if (workspace_bytes < p.bytes) return NERF_STATUS_INVALID_USAGE;
     if (cudaGetDevice(&dev) != cudaSuccess) return NERF_STATUS_CUDA_ERROR;
+    Reach usable(dev);
     for (const void* q : all)
-        if (!usable(q, dev)) return NERF_STATUS_INVALID_USAGE;
-    if (!usable(workspace, dev) || !usable(error_word, dev)) return NERF_STATUS_INVALID_USAGE;
+        if (!usable(q)) return NERF_STATUS_INVALID_USAGE;
+    if (!usable(workspace) || !usable(error_word)) return NERF_STATUS_INVALID_USAGE;
 
     unsigned char* ws = static_cast<unsigned char*>(workspace);
     const uint32_t bf16 = d.dtype == NERF_B200_BF16;

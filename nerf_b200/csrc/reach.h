@@ -1,0 +1,56 @@
+// reach.h -- whether kernels of the current device may use a pointer.
+#pragma once
+#include <cuda.h>
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+namespace nb {
+
+// The address of a driver function, null without a driver.
+inline void* driver_function(const char* name) {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult res{};
+    if (cudaGetDriverEntryPoint(name, &p, cudaEnableDefault, &res) != cudaSuccess || res != cudaDriverEntryPointSuccess) {
+        cudaGetLastError();
+        return nullptr;
+    }
+    return p;
+}
+
+// Device memory of one device, or managed memory.  A call's tensors mostly lie
+// in a few allocations: the driver is asked once for each.
+class Reach {
+public:
+    explicit Reach(int device) : device_(device) {}
+    bool operator()(const void* p) {
+        if (!p) return true;
+        const uint64_t at = reinterpret_cast<uint64_t>(p);
+        for (uint32_t i = 0; i < kept_; ++i)
+            if (at - lo_[i] < size_[i]) return true;
+        using Query = CUresult (*)(unsigned int, CUpointer_attribute*, void**, CUdeviceptr);
+        static const Query query = reinterpret_cast<Query>(driver_function("cuPointerGetAttributes"));
+        if (!query) return false;
+        CUpointer_attribute what[5] = {CU_POINTER_ATTRIBUTE_MEMORY_TYPE, CU_POINTER_ATTRIBUTE_DEVICE_ORDINAL, CU_POINTER_ATTRIBUTE_IS_MANAGED,
+                                       CU_POINTER_ATTRIBUTE_RANGE_START_ADDR, CU_POINTER_ATTRIBUTE_RANGE_SIZE};
+        unsigned int type = 0, managed = 0;  // type 0: no memory that the driver knows
+        int device = -1;
+        CUdeviceptr lo = 0;
+        size_t size = 0;
+        void* into[5] = {&type, &device, &managed, &lo, &size};
+        if (query(5u, what, into, static_cast<CUdeviceptr>(at)) != CUDA_SUCCESS) return false;
+        if (!managed && (type != CU_MEMORYTYPE_DEVICE || device != device_)) return false;
+        const uint32_t slot = kept_ < kSlots ? kept_++ : next_++ % kSlots;
+        lo_[slot] = static_cast<uint64_t>(lo);
+        size_[slot] = static_cast<uint64_t>(size);
+        return true;
+    }
+
+private:
+    static constexpr uint32_t kSlots = 8;
+    int device_;
+    uint32_t kept_ = 0, next_ = 0;
+    uint64_t lo_[kSlots] = {}, size_[kSlots] = {};
+};
+
+}  // namespace nb

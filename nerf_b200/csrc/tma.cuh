@@ -73,11 +73,15 @@ NB_DEV void arrive(uint64_t* mbar) {
 }
 
 // Waits for the phase of the given parity; false after kWaitLimitNs.  The
-// clock is read every 64 polls only, so a wait that ends soon never reads it.
+// clock is read every 64 polls only, so a wait that ends soon never reads it;
+// it runs on while the GPU works for another process, so a wait that is late
+// polls on for a while before it gives up.
 constexpr uint64_t kWaitLimitNs = 1000000000ull;
+constexpr uint32_t kLatePolls = 64u * 64u;
 NB_DEV bool wait(uint64_t* mbar, uint32_t parity) {
     const uint32_t a = smem_u32(mbar);
     uint64_t t0 = 0u;
+    uint32_t late = 0u;
     for (uint32_t i = 0;; ++i) {
         uint32_t done;
         asm volatile(
@@ -93,7 +97,7 @@ NB_DEV bool wait(uint64_t* mbar, uint32_t parity) {
         if ((i & 63u) == 63u) {
             const uint64_t t = umma::globaltimer();
             if (t0 == 0u) t0 = t;
-            else if (t - t0 > kWaitLimitNs) return false;
+            else if (t - t0 > kWaitLimitNs && (late += 64u) > kLatePolls) return false;
         }
     }
 }

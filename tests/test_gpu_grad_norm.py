@@ -159,3 +159,22 @@ def test_clip_in_a_graph_on_a_stream(cuda):
         assert abs(float(info[0]) - norm) <= REL * norm
         for a, b in items:
             assert bool(((b.double() - a.double() / norm).abs() <= a.double().abs() / norm * (REL + 2.0 ** -23)).all())
+
+
+def test_host_memory_is_refused(cuda):
+    torch = cuda
+    from linear_util import ptr, tensors
+    from nerf_b200 import abi
+    lib = abi.load()
+    g, out = torch.ones(64, device="cuda"), torch.zeros(64, device="cuda")
+    info, ws = torch.zeros(4, device="cuda"), torch.zeros(lib.nerf_b200_grad_workspace_bytes(1), dtype=torch.uint8, device="cuda")
+    host = torch.zeros(65536, dtype=torch.uint8)
+    at = (host.data_ptr() + 255) // 256 * 256
+    for bad in ("grad", "out", "info", "ws"):
+        t = tensors([(g, out)])
+        if bad in ("grad", "out"):
+            setattr(t[0], bad, at)
+        pi, pw = at if bad == "info" else ptr(info), at if bad == "ws" else ptr(ws)
+        assert lib.nerf_b200_grad_clip(t, 1, 1.0, 1.0, pi, pw, ws.numel(), None) == abi.NERF_STATUS_INVALID_USAGE, bad
+    torch.cuda.synchronize()
+    assert not out.any()

@@ -18,6 +18,8 @@ pytestmark = pytest.mark.gpu
 # have enough 256 x 256 tiles for pairs of CTAs in the forward, the input gradient and the weight gradient
 SHAPES = [(1, 1, 1), (1, 64, 64), (2, 17, 9), (5, 64, 48), (63, 63, 65), (64, 128, 128), (127, 200, 256), (128, 64, 257), (129, 65, 64),
           (300, 320, 511), (1000, 63, 255), (257, 1024, 96), (19, 2048, 520), (4097, 32, 64), (20000, 64, 64), (2500, 520, 2056), (2500, 2049, 520), (700, 2328, 2312)]
+# rows of one to seven values, fewer rows than a group of eight and just behind one, steps of K that end in a group
+THIN = [(1000, 1, 3), (77, 3, 5), (7, 9, 129), (8, 65, 7), (9, 71, 130), (257, 5, 260), (135, 193, 15)]
 
 
 def _floor(torch, t):
@@ -28,7 +30,7 @@ def _gen(torch, seed):
     return torch.Generator(device="cuda").manual_seed(seed)
 
 
-@pytest.mark.parametrize("n,k,m", SHAPES)
+@pytest.mark.parametrize("n,k,m", SHAPES + THIN)
 @pytest.mark.parametrize("dtype,pad,shift", [("f16", 0, 0), ("bf16", 8, 8), ("f16", 1, 3), ("bf16", 2, 2)])
 def test_forward_whole_numbers(cuda, n, k, m, dtype, pad, shift):
     torch = cuda
@@ -109,7 +111,7 @@ def test_residual_in_place_and_zero_rows(cuda):
     assert torch.equal(y, keep)
 
 
-@pytest.mark.parametrize("n,k,m", SHAPES)
+@pytest.mark.parametrize("n,k,m", SHAPES + THIN)
 @pytest.mark.parametrize("dtype,grad,pad,shift", [("f16", "f32", 0, 0), ("bf16", "bf16", 8, 8), ("f16", "f16", 1, 3), ("bf16", "f32", 2, 2)])
 def test_backward_whole_numbers(cuda, n, k, m, dtype, grad, pad, shift):
     torch = cuda
@@ -323,5 +325,12 @@ def test_host_memory_is_refused(cuda):
         p = {key: ptr(v) for key, v in dev.items()}
         p[bad] = torch.zeros(16, 16, dtype=torch.float16).data_ptr()
         assert lib.nerf_b200_linear_forward(C.byref(d), *(p[c] for c in "xwbryz"), ptr(err), None) == abi.NERF_STATUS_INVALID_USAGE, bad
+    ws = torch.zeros(1 << 20, dtype=torch.uint8, device="cuda")
+    for bad in ("x", "w", "z", "dy", "dx", "dw", "db", "ws"):
+        p = dict(x=ptr(dev["x"]), w=ptr(dev["w"]), z=ptr(dev["z"]), dy=ptr(dev["y"]), r=None, dx=ptr(dev["r"]), dw=ptr(ws), db=ptr(ws) + 4096, ws=ptr(ws) + 65536)
+        host = torch.zeros(1 << 20, dtype=torch.uint8)
+        p[bad] = (host.data_ptr() + 255) // 256 * 256
+        assert lib.nerf_b200_linear_backward(C.byref(d), p["x"], p["w"], p["z"], p["dy"], p["r"], p["dx"], p["dw"], p["db"], p["ws"],
+                                             1 << 19, ptr(err), None) == abi.NERF_STATUS_INVALID_USAGE, bad
     torch.cuda.synchronize()
-    assert SENTINEL == 77.0 and not any(bool(v.any()) for v in dev.values())
+    assert SENTINEL == 77.0 and not ws.any() and not any(bool(v.any()) for v in dev.values())

@@ -92,6 +92,8 @@ def test_gradient_refusals():
             assert _clip(good, clip=clip, **kw) == INVALID, kw
         for kw in (dict(grad=None), dict(grad=OK + 2, out=OK + 2), dict(dtype=3), dict(count=1 << 41)):
             assert _clip([_tensor(**kw)], clip=clip) == INVALID, kw
+        assert _clip(good, n=(1 << 24) + 1, clip=clip) == INVALID
+    assert abi.load().nerf_b200_grad_workspace_bytes((1 << 24) + 1) == 0
     for most in (-1.0, float("nan")):
         assert _clip(good, most=most) == INVALID
     for kw in (dict(out=None), dict(out=OK + 2), dict(dtype=abi.NERF_B200_F32, out_dtype=abi.NERF_B200_F16),
