@@ -911,10 +911,13 @@ NB_DEV void grad_out(void* p, uint64_t i, float v, const GradReduceArgs& a) {
     }
 }
 // Blocks below n_dw: 32 rows x 4 columns of dw; the others: 32 columns of db.
-// Eight warps take an eighth of the parts each, all of a batch's loads in
-// flight, and the first adds the eight sums: a fixed order.
-__global__ void __launch_bounds__(256) k_grad_reduce(const GradReduceArgs a, uint32_t n_dw) {
-    __shared__ float4 ws[8][32];
+// Sixteen warps take a sixteenth of the parts each, with the loads of a batch
+// in flight together (148 parts, one a CTA, are one batch), and the first adds
+// the sixteen sums: a fixed order.  With eight warps and batches of eight the
+// sums of 148 parts of a 64 x 64 layer took 14 us, most of it waiting.
+constexpr uint32_t kSumWarps = 16;
+__global__ void __launch_bounds__(32 * kSumWarps, 1) k_grad_reduce(const GradReduceArgs a, uint32_t n_dw) {
+    __shared__ float4 ws[kSumWarps][32];
     const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
     after_previous();
     let_next_start();
@@ -926,29 +929,28 @@ __global__ void __launch_bounds__(256) k_grad_reduce(const GradReduceArgs a, uin
         const uint32_t per = 16u * a.tiles_n, group = tile / per, first = 16u * group;
         const uint32_t gm = min(16u, a.tiles_m - first), r = tile - group * per;
         const uint32_t m = ((first + r % gm) * a.ctas + half % a.ctas) * kBM + row, n = (r / gm) * a.bn + 4u * c4;
+        if (m - lane >= a.n_out || n >= a.n_in) return;  // the whole block
         const float4* src = reinterpret_cast<const float4*>(a.partials) + (static_cast<uint64_t>(half) * per_tile + c4) * kBM + row;
         const uint64_t step = static_cast<uint64_t>(tiles) * a.ctas * per_tile * kBM;
-        const uint32_t each = (a.splits + 7u) / 8u, k0 = min(a.splits, warp * each), k1 = min(a.splits, k0 + each);
+        const uint32_t each = (a.splits + kSumWarps - 1u) / kSumWarps, k0 = min(a.splits, warp * each), k1 = min(a.splits, k0 + each);
         float4 t = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (n < a.n_in) {
-            for (uint32_t k = k0; k < k1; k += 8u) {
-                float4 v[8];
+        for (uint32_t k = k0; k < k1; k += 10u) {
+            float4 v[10];
 #pragma unroll
-                for (uint32_t j = 0; j < 8u; ++j) v[j] = k + j < k1 ? __ldcs(src + (k + j) * step) : make_float4(0.f, 0.f, 0.f, 0.f);
+            for (uint32_t j = 0; j < 10u; ++j) v[j] = k + j < k1 ? __ldcs(src + (k + j) * step) : make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-                for (uint32_t j = 0; j < 8u; ++j) {
-                    t.x += v[j].x;
-                    t.y += v[j].y;
-                    t.z += v[j].z;
-                    t.w += v[j].w;
-                }
+            for (uint32_t j = 0; j < 10u; ++j) {
+                t.x += v[j].x;
+                t.y += v[j].y;
+                t.z += v[j].z;
+                t.w += v[j].w;
             }
         }
         ws[warp][lane] = t;
         __syncthreads();
-        if (warp != 0u || m >= a.n_out || n >= a.n_in) return;
+        if (warp != 0u || m >= a.n_out) return;
 #pragma unroll
-        for (uint32_t w = 1; w < 8u; ++w) {
+        for (uint32_t w = 1; w < kSumWarps; ++w) {
             const float4 v = ws[w][lane];
             t.x += v.x;
             t.y += v.y;
@@ -962,22 +964,22 @@ __global__ void __launch_bounds__(256) k_grad_reduce(const GradReduceArgs a, uin
         return;
     }
     const uint32_t c = 32u * (blockIdx.x - n_dw) + lane;
-    const uint32_t per = (a.parts + 7u) / 8u, p0 = min(a.parts, warp * per), p1 = min(a.parts, p0 + per);
+    const uint32_t per = (a.parts + kSumWarps - 1u) / kSumWarps, p0 = min(a.parts, warp * per), p1 = min(a.parts, p0 + per);
     float t = 0.0f;
     if (c < a.n_out) {
-        for (uint32_t p = p0; p < p1; p += 16u) {
-            float v[16];
+        for (uint32_t p = p0; p < p1; p += 20u) {
+            float v[20];
 #pragma unroll
-            for (uint32_t j = 0; j < 16u; ++j) v[j] = p + j < p1 ? a.db_part[static_cast<uint64_t>(p + j) * a.n_out + c] : 0.0f;
+            for (uint32_t j = 0; j < 20u; ++j) v[j] = p + j < p1 ? a.db_part[static_cast<uint64_t>(p + j) * a.n_out + c] : 0.0f;
 #pragma unroll
-            for (uint32_t j = 0; j < 16u; ++j) t += v[j];
+            for (uint32_t j = 0; j < 20u; ++j) t += v[j];
         }
     }
     ws[warp][lane].x = t;
     __syncthreads();
     if (warp == 0u && c < a.n_out) {
 #pragma unroll
-        for (uint32_t w = 1; w < 8u; ++w) t += ws[w][lane].x;
+        for (uint32_t w = 1; w < kSumWarps; ++w) t += ws[w][lane].x;
         grad_out(a.db, c, t, a);
     }
 }
@@ -1062,7 +1064,7 @@ cudaError_t launch_grad_reduce(const GradReduceArgs& a, cudaStream_t s) {
     const uint32_t n_dw = a.dw ? a.tiles_m * a.tiles_n * a.ctas * (a.bn / 4u) * 4u : 0u;
     const uint32_t n_db = a.db ? (a.n_out + 31u) / 32u : 0u;
     if (n_dw + n_db == 0u) return cudaSuccess;
-    return launch_after(k_grad_reduce, dim3(n_dw + n_db), 256u, 0u, 1u, s, a, n_dw);
+    return launch_after(k_grad_reduce, dim3(n_dw + n_db), 32u * kSumWarps, 0u, 1u, s, a, n_dw);
 }
 
 }  // namespace nb

@@ -102,9 +102,9 @@ struct NarrowMaps {
     CUtensorMap dy, pre, x, w, dx, res;
 };
 // The input gradient of a layer with n_in, n_out <= 256, making dz on the way
-// (linear_dx.cu): dx, dz (null: dy itself), and eight parts of db a CTA.  Of the
+// (linear_dx.cu): dx, dz (null: dy itself), and a part of db a CTA.  Of the
 // maps w has boxes of 64 x 64, the others as for the narrow backward.
-constexpr uint32_t kDxMaxWidth = 256, kDxPartsPerBlock = 8;
+constexpr uint32_t kDxMaxWidth = 256;
 struct DxArgs {
     uint32_t n, n_in, n_out, act, bf16;
     MatrixView dx, res;  // res.ptr null: none

@@ -183,7 +183,7 @@ BackwardPlan plan_backward(const NerfB200Linear& d) {
     if (p.dz_needed) at += up(static_cast<uint64_t>(d.n_rows) * p.dz_ld * 2u, 256u);
     p.o_db = at;
     const uint32_t blocks = dz_on_the_way(d) ? row_blocks(d, p.sms) : 0u;
-    at += up(static_cast<uint64_t>(p.parts > kDxPartsPerBlock * blocks ? p.parts : kDxPartsPerBlock * blocks) * d.n_out * 4u, 256u);
+    at += up(static_cast<uint64_t>(p.parts > blocks ? p.parts : blocks) * d.n_out * 4u, 256u);
     p.o_dw = at;
     // How the operands can be fed depends on the pointers: room for every way.
     const uint64_t tma = plan_grad(d, false, p.sms).bytes, raw = plan_grad(d, true, p.sms).bytes;
@@ -439,7 +439,7 @@ NERF_API NerfStatus nerf_b200_linear_backward(const NerfB200Linear* desc, const 
         a.error = error_word;
         if (!make_maps(64u)) return NERF_STATUS_CUDA_ERROR;
         if (launch_dx(a, maps, blocks, s) != cudaSuccess) return NERF_STATUS_CUDA_ERROR;
-        r.parts = kDxPartsPerBlock * blocks;
+        r.parts = blocks;
     }
     const bool dz_written = p.dz_needed && (dx || dweight);
     const MatrixView dzv = p.dz_needed ? view(ws + p.o_dz, p.dz_ld, d.n_rows, d.n_out) : dyv;

@@ -22,7 +22,6 @@ namespace {
 constexpr uint32_t kRows = 128, kBox = kRows * 128u;  // 128 rows x 64 values
 constexpr uint32_t kDzWarps = 8, kThreads = 32u * (4u + kDzWarps + 8u);
 constexpr uint32_t kMaxK = 4;  // 64-value steps of n_out
-static_assert(kDxPartsPerBlock == kDzWarps, "one part of db a warp");
 
 template <uint32_t IB>
 struct DxShape {
@@ -174,8 +173,11 @@ __global__ void __launch_bounds__(kThreads, 1) k_dx(const DxArgs a, const __grid
             }
         }
         if (!ok) atomicOr(a.error, 1u);
-        if (a.db_part) {  // one part a warp: four of its lanes hold each column
-            float* part = a.db_part + static_cast<uint64_t>(kDzWarps * blockIdx.x + warp - 4u) * a.n_out;
+        if (a.db_part) {
+            // Four lanes of each warp hold a column: their sums meet in the last stage's room, once its MMAs have read
+            // it.  Every warp comes to the barrier, also one whose wait ran out.
+            if (ok && steps) ok = __all_sync(0xffffffffu, tma::wait(&bar.empty[(steps - 1u) % S::kStages], ((steps - 1u) / S::kStages) & 1u));
+            float* acc = reinterpret_cast<float*>(smem + (steps - 1u) % S::kStages * S::kStage);
 #pragma unroll
             for (uint32_t k = 0; k < kMaxK; ++k) {
 #pragma unroll
@@ -183,9 +185,15 @@ __global__ void __launch_bounds__(kThreads, 1) k_dx(const DxArgs a, const __grid
                     float v = sums[k][j];
                     v += __shfl_xor_sync(0xffffffffu, v, 8);
                     v += __shfl_xor_sync(0xffffffffu, v, 16);
-                    const uint32_t c = 64u * k + 8u * p + j;
-                    if (lane < 8u && c < a.n_out) part[c] = v;
+                    if (lane < 8u && ok) acc[(warp - 4u) * 64u * kMaxK + 64u * k + 8u * p + j] = v;
                 }
+            }
+            asm volatile("bar.sync 1, %0;\n" ::"n"(32u * kDzWarps) : "memory");
+            for (uint32_t c = t; c < a.n_out && ok; c += 32u * kDzWarps) {
+                float v = 0.0f;
+#pragma unroll
+                for (uint32_t w = 0; w < kDzWarps; ++w) v += acc[w * 64u * kMaxK + c];
+                a.db_part[static_cast<uint64_t>(blockIdx.x) * a.n_out + c] = v;
             }
         }
     } else if (warp >= 4u + kDzWarps) {
