@@ -226,6 +226,16 @@ __global__ void __launch_bounds__(GemmShape<BN, KIND, FEED>::kThreads, 1) k_gemm
     let_next_start();
     const uint32_t tmem = bar.tmem_base;
     const uint32_t tiles = g.tiles_m * g.tiles_n, items = tiles * g.splits;
+    // With one step of K a CTA that keeps to one column of tiles keeps B: its box is brought to each stage once.
+    const bool keep_b = KIND == kGemmRows && g.k_steps == 1u && item_step % g.tiles_n == 0u;
+    const auto locate = [&](uint32_t tile, uint32_t& tm, uint32_t& tn) {
+        if (keep_b) {
+            tm = tile / g.tiles_n;
+            tn = tile - tm * g.tiles_n;
+        } else {
+            tile_of(g, tile, tm, tn);
+        }
+    };
     if (S::kRegs && warp < 4u) tma::registers_down<S::kRegsDown>();
 
     if ((warp == 0u || warp == 3u) && lane == 0u) {
@@ -246,11 +256,13 @@ __global__ void __launch_bounds__(GemmShape<BN, KIND, FEED>::kThreads, 1) k_gemm
             const uint32_t split = it / tiles;
             const uint32_t ks0 = split * g.steps_per_split, ks1 = min(g.k_steps, ks0 + g.steps_per_split);
             uint32_t tm, tn;
-            tile_of(g, it - split * tiles, tm, tn);
+            locate(it - split * tiles, tm, tn);
             const uint32_t at = op ? tn * BN + rank * S::kBoxN : (tm * kCtas + rank) * kBM;  // the box's rows or columns
             for (uint32_t ks = ks0; ks < ks1; ++ks) {
                 const uint32_t k0 = ks * kBK;
+                const bool kept = op && keep_b && issued >= kStages;
                 if (raw) {
+                    if (kept) break;  // placed for good
                     const uint32_t r = issued % kRawRing;
                     ok = tma::wait(&bar.raw_empty[op][r], (issued / kRawRing + 1u) & 1u);
                     if (!ok) break;
@@ -259,9 +271,9 @@ __global__ void __launch_bounds__(GemmShape<BN, KIND, FEED>::kThreads, 1) k_gemm
                     ok = tma::wait(&bar.empty[stage], parity);
                     if (!ok) break;
                     unsigned char* dst = smem + stage * kStageBytes + op * kStageBytesA;
-                    if (announce) tma::expect_tx(&bar.full[stage], kCtas * bytes);
+                    if (announce) tma::expect_tx(&bar.full[stage], keep_b && issued >= kStages ? (op ? 0u : bytes_a) : kCtas * bytes);
                     const uint32_t full = S::kPair ? tma::peer_addr(smem_u32(&bar.full[stage]), 0u) : 0u;
-                    for (uint32_t j = 0; j < (mn ? width / 64u : 1u); ++j) {
+                    for (uint32_t j = 0; j < (kept ? 0u : mn ? width / 64u : 1u); ++j) {
                         const uint32_t x = mn ? at + 64u * j : k0, y = mn ? k0 : at;
                         if (S::kPair) tma::load_2d_pair(smem_u32(dst + j * 8192u), map, x, y, full);
                         else tma::load_2d(smem_u32(dst + j * 8192u), map, x, y, &bar.full[stage]);
@@ -293,11 +305,12 @@ __global__ void __launch_bounds__(GemmShape<BN, KIND, FEED>::kThreads, 1) k_gemm
             const uint32_t split = it / tiles;
             const uint32_t ks0 = split * g.steps_per_split, ks1 = min(g.k_steps, ks0 + g.steps_per_split);
             uint32_t tm, tn;
-            tile_of(g, it - split * tiles, tm, tn);
+            locate(it - split * tiles, tm, tn);
             for (uint32_t ks = ks0; ks < ks1; ++ks, ++i) {
                 const uint32_t stage = i % kStages, r = i % kRawRing, turn = (i / kRawRing) & 1u;
+                const bool place_b = g.b_raw && !(keep_b && i >= kStages);
                 ok = tma::wait(&bar.empty[stage], (i / kStages + 1u) & 1u) && (!g.a_raw || tma::wait(&bar.raw_full[0][r], turn)) &&
-                     (!g.b_raw || tma::wait(&bar.raw_full[1][r], turn));
+                     (!place_b || tma::wait(&bar.raw_full[1][r], turn));
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
                 unsigned char* sa = smem + stage * kStageBytes;
@@ -307,7 +320,7 @@ __global__ void __launch_bounds__(GemmShape<BN, KIND, FEED>::kThreads, 1) k_gemm
                     __syncwarp();
                     if (lane == 0u) tma::arrive(&bar.raw_empty[0][r]);
                 }
-                if (g.b_raw) {
+                if (place_b) {
                     for (uint32_t v = w; v < 8u; v += S::kLoaders)
                         raw_box<BN>(sa + kStageBytesA, src + raw_bytes(kBM), g.b, g.b_mn, tn * BN, ks * kBK, v, lane);
                     __syncwarp();
@@ -384,7 +397,7 @@ __global__ void __launch_bounds__(GemmShape<BN, KIND, FEED>::kThreads, 1) k_gemm
             const uint32_t split = it / tiles;
             const uint32_t ks0 = split * g.steps_per_split, ks1 = min(g.k_steps, ks0 + g.steps_per_split);
             uint32_t tm, tn;
-            tile_of(g, it - split * tiles, tm, tn);
+            locate(it - split * tiles, tm, tn);
             const uint32_t m0 = (tm * kCtas + rank) * kBM + 32u * q, n0 = tn * BN + h * kHalf;
             const uint32_t rows = m0 < g.M ? min(32u, g.M - m0) : 0u;
             float s[kHalf];
@@ -518,7 +531,7 @@ __global__ void __launch_bounds__(GemmShape<BN, KIND, FEED>::kThreads, 1) k_gemm
         };
         for (uint32_t it = first_item + acc * item_step; it < items; it += S::kGroups * item_step) {
             uint32_t tm, tn;
-            tile_of(g, it, tm, tn);
+            locate(it, tm, tn);
             const uint32_t m0 = (tm * kCtas + rank) * kBM + 32u * q, n0 = tn * BN;
             const uint32_t rows = m0 < g.M ? min(32u, g.M - m0) : 0u;
             if (n0 != bias_n) {  // the tile's bias, kept while the columns stay the same
@@ -534,7 +547,7 @@ __global__ void __launch_bounds__(GemmShape<BN, KIND, FEED>::kThreads, 1) k_gemm
                     const uint32_t jt = it + S::kGroups * w * item_step;
                     if (jt >= items) break;
                     uint32_t jm, jn;
-                    tile_of(g, jt, jm, jn);
+                    locate(jt, jm, jn);
                     const uint32_t jr = (jm * kCtas + rank) * kBM + 32u * q;
                     for (uint32_t c = jn * BN; jr < g.M && c < min(jn * BN + BN, g.N); c += 64u)
                         tma::prefetch_2d(&maps.res, static_cast<int32_t>(c), static_cast<int32_t>(jr));
