@@ -399,7 +399,8 @@ typedef struct NerfB200Linear {
  * pre may be NULL.  Products are summed in fp32, y and pre are rounded once.
  * residual may be y itself; otherwise outputs overlap nothing.  Any alignment
  * of the dtype is accepted; rows that start on 16-byte boundaries (pointer
- * and ld) are the fast path.  error_word: one device uint32; bit 0 is set
+ * and ld) are the fast path (x and weight of another alignment are read from
+ * the 16-byte boundary before their first value on).  error_word: one device uint32; bit 0 is set
  * when a wait inside the kernel ran out after a second (outputs are then
  * incomplete). */
 NERF_API NerfStatus nerf_b200_linear_forward(const NerfB200Linear* desc, const void* x, const void* weight, const void* bias,

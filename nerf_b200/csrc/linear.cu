@@ -842,6 +842,16 @@ cudaError_t launch_cols_t(const GemmArgs& g, const GemmMaps& maps, cudaStream_t 
 }
 
 // ------------------------------------------------- dz and its column sums
+// A finished sum into its place in dw or db.
+NB_DEV void grad_out(void* p, uint64_t i, float v, bool f32, bool bf16, bool accumulate) {
+    if (f32) {
+        float* q = static_cast<float*>(p) + i;
+        *q = accumulate ? *q + v : v;
+    } else {
+        uint16_t* q = static_cast<uint16_t*>(p) + i;
+        *q = to_16(accumulate ? from_16(*q, bf16) + v : v, bf16);
+    }
+}
 // 256 threads: 8 columns a thread, `cg` column groups side by side (a power of
 // two up to 32), 256 / cg rows at a time.
 NB_DEV void dz_row(uint32_t (&w)[4], const uint16_t* q, uint32_t have, bool vec) {
@@ -909,20 +919,12 @@ __global__ void __launch_bounds__(256, 4) k_dz(const DzArgs a, uint32_t cg_log2)
         if (col >= a.dy.cols) break;
         float t = 0.0f;
         for (uint32_t y = 0; y < ny; ++y) t += sums[(y << cg_log2) + (c >> 3)][c & 7u];
-        a.db_part[static_cast<uint64_t>(blockIdx.y) * a.dy.cols + col] = t;
+        if (a.parts == 1u) grad_out(a.db, col, t, a.f32 != 0u, bf16, a.accumulate != 0u);
+        else a.db_part[static_cast<uint64_t>(blockIdx.y) * a.dy.cols + col] = t;
     }
 }
 
 // -------------------------------------------- sums of the partial gradients
-NB_DEV void grad_out(void* p, uint64_t i, float v, const GradReduceArgs& a) {
-    if (a.f32) {
-        float* q = static_cast<float*>(p) + i;
-        *q = a.accumulate ? *q + v : v;
-    } else {
-        uint16_t* q = static_cast<uint16_t*>(p) + i;
-        *q = to_16(a.accumulate ? from_16(*q, a.bf16 != 0u) + v : v, a.bf16 != 0u);
-    }
-}
 // Blocks below n_dw: 32 rows x 4 columns of dw; the others: 32 columns of db.
 // Sixteen warps take a sixteenth of the parts each, with the loads of a batch
 // in flight together (148 parts, one a CTA, are one batch), and the first adds
@@ -973,7 +975,7 @@ __global__ void __launch_bounds__(32 * kSumWarps, 1) k_grad_reduce(const GradRed
         const float o[4] = {t.x, t.y, t.z, t.w};
 #pragma unroll
         for (uint32_t i = 0; i < 4u; ++i)
-            if (n + i < a.n_in) grad_out(a.dw, static_cast<uint64_t>(m) * a.n_in + n + i, o[i], a);
+            if (n + i < a.n_in) grad_out(a.dw, static_cast<uint64_t>(m) * a.n_in + n + i, o[i], a.f32 != 0u, a.bf16 != 0u, a.accumulate != 0u);
         return;
     }
     const uint32_t c = 32u * (blockIdx.x - n_dw) + lane;
@@ -993,7 +995,7 @@ __global__ void __launch_bounds__(32 * kSumWarps, 1) k_grad_reduce(const GradRed
     if (warp == 0u && c < a.n_out) {
 #pragma unroll
         for (uint32_t w = 1; w < kSumWarps; ++w) t += ws[w][lane].x;
-        grad_out(a.db, c, t, a);
+        grad_out(a.db, c, t, a.f32 != 0u, a.bf16 != 0u, a.accumulate != 0u);
     }
 }
 

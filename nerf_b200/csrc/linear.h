@@ -74,6 +74,8 @@ struct DzArgs {
     float* db_part;
     uint32_t parts, rows_per_part;
     uint32_t bf16, act;
+    void* db;  // one part: the sums go here at once
+    uint32_t f32, accumulate;
 };
 cudaError_t launch_dz(const DzArgs& a, cudaStream_t s);
 // dw (+)= sum of the splits' partial tiles, db (+)= sum of the row parts.

@@ -454,6 +454,10 @@ NERF_API NerfStatus nerf_b200_linear_backward(const NerfB200Linear* desc, const 
         a.rows_per_part = p.rows_per_part;
         a.bf16 = bf16;
         a.act = d.activation;
+        a.db = dbias;
+        a.f32 = r.f32;
+        a.accumulate = d.accumulate;
+        if (p.parts == 1u) r.db = nullptr;  // nothing is left to add up
         if (launch_dz(a, s) != cudaSuccess) return NERF_STATUS_CUDA_ERROR;
     }
     if (dx && !on_the_way) {
