@@ -798,25 +798,40 @@ __global__ void __launch_bounds__(ColsShape<BN, RAW>::kThreads) k_gemm_cols(cons
     __syncthreads();
     if (g.splits > 1u) tma::cluster_sync();
     if (mine && failed == 0u) {
-        const uint32_t part_at = smem_u32(part);
-        for (uint32_t i = rank * 256u + t; i < rows * kBM; i += g.splits * 256u) {
-            const uint64_t j = n0 + (i >> 7);
-            float z = 0.0f, r = 0.0f;
-            if (g.res.ptr) r = from_16(static_cast<const uint16_t*>(g.res.ptr)[j * g.res.ld + m], bf16);
-            if (g.splits == 1u) {
-                z = part[i];
-            } else {
-                float p[kColsMaxCluster];
+        const uint32_t part_at = smem_u32(part), step = g.splits * 256u, end = rows * kBM;
+        constexpr uint32_t kAtOnce = 4;  // values a thread: the trips to the other CTAs overlap
+#pragma unroll 1
+        for (uint32_t i0 = rank * 256u + t; i0 < end; i0 += kAtOnce * step) {
+            float z[kAtOnce], r[kAtOnce];
 #pragma unroll
-                for (uint32_t c = 0; c < kColsMaxCluster; ++c) p[c] = c < g.splits ? tma::peer_f32(part_at + 4u * i, c) : 0.0f;
+            for (uint32_t v = 0; v < kAtOnce; ++v) {
+                const uint32_t i = i0 + v * step;
+                const uint64_t j = n0 + (i >> 7);
+                r[v] = g.res.ptr && i < end ? from_16(static_cast<const uint16_t*>(g.res.ptr)[j * g.res.ld + m], bf16) : 0.0f;
+                z[v] = 0.0f;
+                if (g.splits == 1u) {
+                    if (i < end) z[v] = part[i];
+                } else if (i < end) {
+                    float p[kColsMaxCluster];
 #pragma unroll
-                for (uint32_t c = 0; c < kColsMaxCluster; ++c) z += p[c];
+                    for (uint32_t c = 0; c < kColsMaxCluster; ++c) p[c] = c < g.splits ? tma::peer_f32(part_at + 4u * i, c) : 0.0f;
+#pragma unroll
+                    for (uint32_t c = 0; c < kColsMaxCluster; ++c) z[v] += p[c];
+                }
+                z[v] += bias;
             }
-            z += bias;
-            if (g.pre.ptr) static_cast<uint16_t*>(const_cast<void*>(g.pre.ptr))[j * g.pre.ld + m] = to_16(z, bf16);
-            float v[1] = {z};
-            act_row(v, g.act);
-            static_cast<uint16_t*>(const_cast<void*>(g.y.ptr))[j * g.y.ld + m] = to_16(v[0] + r, bf16);
+            float y[kAtOnce];
+#pragma unroll
+            for (uint32_t v = 0; v < kAtOnce; ++v) y[v] = z[v];
+            act_row(y, g.act);
+#pragma unroll
+            for (uint32_t v = 0; v < kAtOnce; ++v) {
+                const uint32_t i = i0 + v * step;
+                const uint64_t j = n0 + (i >> 7);
+                if (i >= end) break;
+                if (g.pre.ptr) static_cast<uint16_t*>(const_cast<void*>(g.pre.ptr))[j * g.pre.ld + m] = to_16(z[v], bf16);
+                static_cast<uint16_t*>(const_cast<void*>(g.y.ptr))[j * g.y.ld + m] = to_16(y[v] + r[v], bf16);
+            }
         }
     }
     umma::fence_before_sync();
@@ -868,7 +883,7 @@ NB_DEV void dz_row(uint32_t (&w)[4], const uint16_t* q, uint32_t have, bool vec)
     }
 }
 template <uint32_t ACT, bool VEC>
-__global__ void __launch_bounds__(256, 4) k_dz(const DzArgs a, uint32_t cg_log2) {
+__global__ void __launch_bounds__(256, 3) k_dz(const DzArgs a, uint32_t cg_log2) {
     __shared__ float sums[256][8];
     after_previous();
     let_next_start();
@@ -925,48 +940,51 @@ __global__ void __launch_bounds__(256, 4) k_dz(const DzArgs a, uint32_t cg_log2)
 }
 
 // -------------------------------------------- sums of the partial gradients
-// Blocks below n_dw: 32 rows x 4 columns of dw; the others: 32 columns of db.
-// Sixteen warps take a sixteenth of the parts each, with the loads of a batch
-// in flight together (148 parts, one a CTA, are one batch), and the first adds
-// the sixteen sums: a fixed order.  With eight warps and batches of eight the
-// sums of 148 parts of a 64 x 64 layer took 14 us, most of it waiting.
-constexpr uint32_t kSumWarps = 16;
-__global__ void __launch_bounds__(32 * kSumWarps, 1) k_grad_reduce(const GradReduceArgs a, uint32_t n_dw) {
+// Blocks below n_dw: groups of 32 rows x 4 columns of dw, `share` of a block's
+// sixteen warps a group; the others: 32 columns of db.  The warps of a group take
+// equal ranges of the parts, with the loads of a batch in flight together (148
+// parts, one a CTA, are one batch for sixteen), and the first adds their sums: a
+// fixed order.  With eight warps and batches of eight the sums of 148 parts of a
+// 64 x 64 layer took 14 us, most of it waiting; now 6.
+constexpr uint32_t kSumWarps = 16, kSumBatch = 10;
+__global__ void __launch_bounds__(32 * kSumWarps, 1) k_grad_reduce(const GradReduceArgs a, uint32_t n_dw, uint32_t share) {
     __shared__ float4 ws[kSumWarps][32];
     const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
     after_previous();
     let_next_start();
     if (blockIdx.x < n_dw) {
-        const uint32_t per_tile = a.bn / 4u, quarter = blockIdx.x & 3u, idx = blockIdx.x >> 2;
+        const uint32_t per_tile = a.bn / 4u, sub = warp & (share - 1u), group = blockIdx.x * (kSumWarps / share) + warp / share;
+        const uint32_t quarter = group & 3u, idx = group >> 2;
         // half: 128 rows of a tile (a pair of CTAs leaves two)
         const uint32_t half = idx / per_tile, c4 = idx - half * per_tile, row = 32u * quarter + lane;
         const uint32_t tiles = a.tiles_m * a.tiles_n, tile = half / a.ctas;
-        const uint32_t per = 16u * a.tiles_n, group = tile / per, first = 16u * group;
-        const uint32_t gm = min(16u, a.tiles_m - first), r = tile - group * per;
+        const uint32_t per = 16u * a.tiles_n, set = tile / per, first = 16u * set;
+        const uint32_t gm = min(16u, a.tiles_m - first), r = tile - set * per;
         const uint32_t m = ((first + r % gm) * a.ctas + half % a.ctas) * kBM + row, n = (r / gm) * a.bn + 4u * c4;
-        if (m - lane >= a.n_out || n >= a.n_in) return;  // the whole block
-        const float4* src = reinterpret_cast<const float4*>(a.partials) + (static_cast<uint64_t>(half) * per_tile + c4) * kBM + row;
-        const uint64_t step = static_cast<uint64_t>(tiles) * a.ctas * per_tile * kBM;
-        const uint32_t each = (a.splits + kSumWarps - 1u) / kSumWarps, k0 = min(a.splits, warp * each), k1 = min(a.splits, k0 + each);
+        const bool live = half < tiles * a.ctas && m - lane < a.n_out && n < a.n_in;  // the same in the whole warp
         float4 t = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (uint32_t k = k0; k < k1; k += 10u) {
-            float4 v[10];
+        if (live) {
+            const float4* src = reinterpret_cast<const float4*>(a.partials) + (static_cast<uint64_t>(half) * per_tile + c4) * kBM + row;
+            const uint64_t step = static_cast<uint64_t>(tiles) * a.ctas * per_tile * kBM;
+            const uint32_t each = (a.splits + share - 1u) / share, k0 = min(a.splits, sub * each), k1 = min(a.splits, k0 + each);
+            for (uint32_t k = k0; k < k1; k += kSumBatch) {
+                float4 v[kSumBatch];
 #pragma unroll
-            for (uint32_t j = 0; j < 10u; ++j) v[j] = k + j < k1 ? __ldcs(src + (k + j) * step) : make_float4(0.f, 0.f, 0.f, 0.f);
+                for (uint32_t j = 0; j < kSumBatch; ++j) v[j] = k + j < k1 ? __ldcs(src + (k + j) * step) : make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-            for (uint32_t j = 0; j < 10u; ++j) {
-                t.x += v[j].x;
-                t.y += v[j].y;
-                t.z += v[j].z;
-                t.w += v[j].w;
+                for (uint32_t j = 0; j < kSumBatch; ++j) {
+                    t.x += v[j].x;
+                    t.y += v[j].y;
+                    t.z += v[j].z;
+                    t.w += v[j].w;
+                }
             }
         }
         ws[warp][lane] = t;
         __syncthreads();
-        if (warp != 0u || m >= a.n_out) return;
-#pragma unroll
-        for (uint32_t w = 1; w < kSumWarps; ++w) {
-            const float4 v = ws[w][lane];
+        if (sub != 0u || !live || m >= a.n_out) return;
+        for (uint32_t w = 1; w < share; ++w) {
+            const float4 v = ws[warp + w][lane];
             t.x += v.x;
             t.y += v.y;
             t.z += v.z;
@@ -1076,10 +1094,13 @@ cudaError_t launch_dz(const DzArgs& a, cudaStream_t s) {
 }
 
 cudaError_t launch_grad_reduce(const GradReduceArgs& a, cudaStream_t s) {
-    const uint32_t n_dw = a.dw ? a.tiles_m * a.tiles_n * a.ctas * (a.bn / 4u) * 4u : 0u;
+    uint32_t share = 1u;  // warps a group: one batch of loads each
+    while (share < kSumWarps && share * kSumBatch < a.splits) share *= 2u;
+    const uint32_t groups = a.dw ? a.tiles_m * a.tiles_n * a.ctas * (a.bn / 4u) * 4u : 0u, per_block = kSumWarps / share;
+    const uint32_t n_dw = (groups + per_block - 1u) / per_block;
     const uint32_t n_db = a.db ? (a.n_out + 31u) / 32u : 0u;
     if (n_dw + n_db == 0u) return cudaSuccess;
-    return launch_after(k_grad_reduce, dim3(n_dw + n_db), 32u * kSumWarps, 0u, 1u, s, a, n_dw);
+    return launch_after(k_grad_reduce, dim3(n_dw + n_db), 32u * kSumWarps, 0u, 1u, s, a, n_dw, share);
 }
 
 }  // namespace nb

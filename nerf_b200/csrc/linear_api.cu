@@ -136,11 +136,11 @@ GradPlan plan_grad(const NerfB200Linear& d, bool raw, uint32_t sms) {
     p.tiles_m = ceil_div(d.n_out, p.pair ? 2u * kGemmBM : kGemmBM);
     p.tiles_n = ceil_div(d.n_in, p.bn);
     p.k_steps = ceil_div(d.n_rows, kGemmBK);
-    // One wave of (tile, row range) items, each range at least four steps.
+    // One wave of (tile, row range) items, each range at least eight steps, 512 rows.
     const uint64_t tiles = static_cast<uint64_t>(p.tiles_m) * p.tiles_n;
     const uint32_t slots = p.pair ? sms / 2u : sms;
     uint64_t splits = tiles >= slots ? 1u : slots / tiles;
-    if (splits > ceil_div(p.k_steps, 4u)) splits = ceil_div(p.k_steps, 4u);
+    if (splits > ceil_div(p.k_steps, 8u)) splits = ceil_div(p.k_steps, 8u);
     if (splits < 1u) splits = 1u;
     p.steps_per_split = ceil_div(p.k_steps, splits);
     p.splits = p.steps_per_split ? ceil_div(p.k_steps, p.steps_per_split) : 1u;
@@ -170,9 +170,9 @@ BackwardPlan plan_backward(const NerfB200Linear& d) {
     p.sms = current_sms();
     p.dz_needed = d.activation != kActNone;
     p.dz_ld = up(d.n_out, 8u);
-    // One wave of four 256-thread blocks an SM, each with at least 128 rows.
+    // One wave of three 256-thread blocks an SM, each with at least 128 rows.
     const uint32_t groups = ceil_div(d.n_out, 8u), gx = ceil_div(groups, 32u);
-    uint64_t parts = 4ull * p.sms / gx;
+    uint64_t parts = 3ull * p.sms / gx;
     if (parts > ceil_div(d.n_rows, 128u)) parts = ceil_div(d.n_rows, 128u);
     if (parts < 1u) parts = 1u;
     p.rows_per_part = ceil_div(d.n_rows, parts);
