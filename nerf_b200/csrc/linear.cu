@@ -626,14 +626,14 @@ __global__ void __launch_bounds__(GemmShape<BN, KIND, FEED>::kThreads, 1) k_gemm
 // With few activation rows the weight's read is what takes the time: as many
 // CTAs as there are SMs have to read it, which the 128-row tiles of k_gemm
 // leave too few of.  Here the weight's rows fill the tensor core's 128 rows
-// and BN (16 to 128) activation rows its columns, and a cluster of `splits`
+// and BN (16 to 64) activation rows its columns, and a cluster of `splits`
 // CTAs takes one tile, each a part of K.  Every CTA leaves its partial tile in
 // its own shared memory, and the cluster adds them in rank order over
 // distributed shared memory: no workspace, and the same bits every time.
 template <uint32_t BN, bool RAW>
 struct ColsShape {
     static constexpr uint32_t kStageBytes = kStageBytesA + BN * 128u;
-    static constexpr uint32_t kStages = RAW && BN == 128u ? 2u : 4u;  // two or three CTAs an SM: the next launch's start while this one's end
+    static constexpr uint32_t kStages = 4u;  // two or three CTAs an SM: the next launch's start while this one's end
     static constexpr uint32_t kRawBytes = raw_bytes(kBM) + raw_bytes(BN);  // raw copies of a step
     static constexpr uint32_t kSmem = 1024u + kStages * kStageBytes + (RAW ? kRawRing * kRawBytes : 0u);
     static constexpr uint32_t kLoaders = 8u, kThreads = RAW ? 256u + 32u * kLoaders : 256u;
@@ -1073,7 +1073,6 @@ cudaError_t launch_gemm_cols(const GemmArgs& g, uint32_t bn, bool raw, const Gem
         case 16u: return raw ? launch_cols_t<16u, true>(g, maps, s) : launch_cols_t<16u, false>(g, maps, s);
         case 32u: return raw ? launch_cols_t<32u, true>(g, maps, s) : launch_cols_t<32u, false>(g, maps, s);
         case 64u: return raw ? launch_cols_t<64u, true>(g, maps, s) : launch_cols_t<64u, false>(g, maps, s);
-        case 128u: return raw ? launch_cols_t<128u, true>(g, maps, s) : launch_cols_t<128u, false>(g, maps, s);
         default: return cudaErrorInvalidValue;
     }
 }

@@ -247,9 +247,10 @@ cudaError_t run_gemm(GemmArgs& g, int kind, uint32_t bn, bool pair, uint32_t sms
 }
 // Few rows (run_cols) or tiles of 128 (run_rows)?  The first where every row
 // fits one column tile, or where the 128-row tiles would leave half of the SMs
-// without work and K is long enough to be split.
+// without work and K is long enough to be split (128 x 1024 -> 1024: 6.9 us
+// against 9.8; 100 x 256 -> 256: 8.7 against 5.7).
 bool cols_pay(uint64_t m, uint64_t n, uint64_t k, uint32_t sms) {
-    return m <= 128u || (k >= 512u && static_cast<uint64_t>(ceil_div(m, 128u)) * ceil_div(n, 64u) <= sms / 2u);
+    return m <= 64u || (k >= 512u && static_cast<uint64_t>(ceil_div(m, 128u)) * ceil_div(n, 64u) <= sms / 2u);
 }
 cudaError_t run_cols(const GemmArgs& rows, cudaStream_t s, uint32_t sms) {
     GemmArgs g = rows;  // the weight as A, the activations as B
@@ -259,13 +260,15 @@ cudaError_t run_cols(const GemmArgs& rows, cudaStream_t s, uint32_t sms) {
     g.b_mn = 0u;
     g.M = rows.N;
     g.N = rows.M;
-    const uint32_t bn = g.N <= 16u ? 16u : g.N <= 32u ? 32u : g.N <= 64u ? 64u : 128u;
+    // (tiles of 128 rows instead of two of 64 took 15.5 us against 14.7 at 100 x 4096 -> 4096, 9.0 against 7.9 at
+    // 100 x 512 -> 4096: their output work is by the CTA)
+    const uint32_t bn = g.N <= 16u ? 16u : g.N <= 32u ? 32u : 64u;
     g.tiles_m = ceil_div(g.M, kGemmBM);
     g.tiles_n = ceil_div(g.N, bn);
     g.k_steps = ceil_div(g.K, kGemmBK);
-    // As many parts of K as fill the SMs, which hold two CTAs each but of the widest tile, and each part at least two
-    // steps (19 rows through 4096 x 4096: 10.0 us with 256 CTAs, 11.1 with 128; 100 rows: 28 us with 256, 15 with 128).
-    const uint64_t tiles = static_cast<uint64_t>(g.tiles_m) * g.tiles_n, room = bn <= 64u ? 2u * sms : sms;
+    // As many parts of K as fill the SMs, which hold two CTAs each, and each part at least two steps (19 rows through
+    // 4096 x 4096: 10.0 us with 256 CTAs, 11.1 with 128).
+    const uint64_t tiles = static_cast<uint64_t>(g.tiles_m) * g.tiles_n, room = 2u * sms;
     uint64_t splits = tiles >= room ? 1u : room / tiles;
     if (splits > kColsMaxCluster) splits = kColsMaxCluster;
     if (splits > ceil_div(g.k_steps, 2u)) splits = ceil_div(g.k_steps, 2u);
