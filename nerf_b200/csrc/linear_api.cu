@@ -118,9 +118,11 @@ uint32_t pick_bn(uint32_t tiles_m, uint32_t n, uint32_t k, bool raw, uint32_t sm
 }
 
 // Whether a product is worth a pair of CTAs on 256 x 256 tiles: enough tiles
-// for every pair, and a K long enough for the MMAs to be what takes the time.
+// for every pair, more than half of a tile's rows and a quarter of its columns
+// in use (100 x 4096 -> 20480: 59 us with pairs, 43 without; 20000 x 4096 -> 64:
+// 64 and 58), and a K long enough for the MMAs to be what takes the time.
 bool pair_pays(uint64_t m, uint64_t n, uint64_t k, uint32_t sms) {
-    return k >= 512u && static_cast<uint64_t>(ceil_div(m, 256u)) * ceil_div(n, 256u) >= sms / 2u;
+    return k >= 512u && m > 128u && n > 64u && static_cast<uint64_t>(ceil_div(m, 256u)) * ceil_div(n, 256u) >= sms / 2u;
 }
 
 // The weight gradient's tiles, and the row ranges that each is split into.
@@ -131,7 +133,7 @@ struct GradPlan {
 };
 GradPlan plan_grad(const NerfB200Linear& d, bool raw, uint32_t sms) {
     GradPlan p{};
-    p.pair = !raw && pair_pays(d.n_out, d.n_in, d.n_rows, sms);
+    p.pair = !raw && d.n_in > 128u && pair_pays(d.n_out, d.n_in, d.n_rows, sms);  // its tiles are 256 wide
     p.bn = d.n_in <= 64u ? 64u : d.n_in <= 128u || raw ? kGemmRawBN : 256u;
     p.tiles_m = ceil_div(d.n_out, p.pair ? 2u * kGemmBM : kGemmBM);
     p.tiles_n = ceil_div(d.n_in, p.bn);

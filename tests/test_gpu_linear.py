@@ -20,6 +20,9 @@ SHAPES = [(1, 1, 1), (1, 64, 64), (2, 17, 9), (5, 64, 48), (63, 63, 65), (64, 12
           (300, 320, 511), (1000, 63, 255), (257, 1024, 96), (19, 2048, 520), (4097, 32, 64), (20000, 64, 64), (2500, 520, 2056), (2500, 2049, 520), (700, 2328, 2312)]
 # rows of one to seven values, fewer rows than a group of eight and just behind one, steps of K that end in a group
 THIN = [(1000, 1, 3), (77, 3, 5), (7, 9, 129), (8, 65, 7), (9, 71, 130), (257, 5, 260), (135, 193, 15)]
+# one long axis beside short ones: enough 256 x 256 tiles for pairs of CTAs, but most of each empty
+LONG = [(600, 64, 19200), (600, 128, 19200), (520, 130, 19200), (600, 19200, 64), (520, 19200, 130), (40, 576, 19200), (70, 576, 19200),
+        (19200, 576, 64), (19200, 520, 72)]
 
 
 def _floor(torch, t):
@@ -30,7 +33,7 @@ def _gen(torch, seed):
     return torch.Generator(device="cuda").manual_seed(seed)
 
 
-@pytest.mark.parametrize("n,k,m", SHAPES + THIN)
+@pytest.mark.parametrize("n,k,m", SHAPES + THIN + LONG)
 @pytest.mark.parametrize("dtype,pad,shift", [("f16", 0, 0), ("bf16", 8, 8), ("f16", 1, 3), ("bf16", 2, 2)])
 def test_forward_whole_numbers(cuda, n, k, m, dtype, pad, shift):
     torch = cuda
@@ -111,7 +114,7 @@ def test_residual_in_place_and_zero_rows(cuda):
     assert torch.equal(y, keep)
 
 
-@pytest.mark.parametrize("n,k,m", SHAPES + THIN)
+@pytest.mark.parametrize("n,k,m", SHAPES + THIN + LONG)
 @pytest.mark.parametrize("dtype,grad,pad,shift", [("f16", "f32", 0, 0), ("bf16", "bf16", 8, 8), ("f16", "f16", 1, 3), ("bf16", "f32", 2, 2)])
 def test_backward_whole_numbers(cuda, n, k, m, dtype, grad, pad, shift):
     torch = cuda
