@@ -136,8 +136,9 @@ GradPlan plan_grad(const NerfB200Linear& d, bool raw, uint32_t sms) {
     p.pair = !raw && d.n_in > 128u && pair_pays(d.n_out, d.n_in, d.n_rows, sms);  // its tiles are 256 wide
     p.bn = d.n_in <= 64u ? 64u : d.n_in <= 128u || raw ? kGemmRawBN : 256u;
     p.tiles_m = ceil_div(d.n_out, p.pair ? 2u * kGemmBM : kGemmBM);
-    p.tiles_n = ceil_div(d.n_in, p.bn);
     p.k_steps = ceil_div(d.n_rows, kGemmBK);
+    while (!p.pair && p.bn > 64u && static_cast<uint64_t>(p.tiles_m) * ceil_div(d.n_in, p.bn / 2u) * ceil_div(p.k_steps, 8u) <= sms) p.bn /= 2u;
+    p.tiles_n = ceil_div(d.n_in, p.bn);
     // One wave of (tile, row range) items, each range at least eight steps, 512 rows.
     const uint64_t tiles = static_cast<uint64_t>(p.tiles_m) * p.tiles_n;
     const uint32_t slots = p.pair ? sms / 2u : sms;
@@ -264,10 +265,13 @@ cudaError_t run_cols(const GemmArgs& rows, cudaStream_t s, uint32_t sms) {
     g.N = rows.M;
     // (tiles of 128 rows instead of two of 64 took 15.5 us against 14.7 at 100 x 4096 -> 4096, 9.0 against 7.9 at
     // 100 x 512 -> 4096: their output work is by the CTA)
-    const uint32_t bn = g.N <= 16u ? 16u : g.N <= 32u ? 32u : 64u;
+    uint32_t bn = g.N <= 16u ? 16u : g.N <= 32u ? 32u : 64u;
     g.tiles_m = ceil_div(g.M, kGemmBM);
-    g.tiles_n = ceil_div(g.N, bn);
     g.k_steps = ceil_div(g.K, kGemmBK);
+    // Narrower tiles while even twice as many leave SMs without work.
+    const uint32_t most = g.k_steps < 2u * kColsMaxCluster ? (g.k_steps + 1u) / 2u : kColsMaxCluster;
+    while (bn > 16u && static_cast<uint64_t>(g.tiles_m) * ceil_div(g.N, bn / 2u) * most <= sms) bn /= 2u;
+    g.tiles_n = ceil_div(g.N, bn);
     // As many parts of K as fill the SMs, which hold two CTAs each, and each part at least two steps (19 rows through
     // 4096 x 4096: 10.0 us with 256 CTAs, 11.1 with 128).
     const uint64_t tiles = static_cast<uint64_t>(g.tiles_m) * g.tiles_n, room = 2u * sms;
@@ -426,7 +430,7 @@ NERF_API NerfStatus nerf_b200_linear_backward(const NerfB200Linear* desc, const 
         r.parts = blocks;
         return launch_grad_reduce(r, s) == cudaSuccess ? NERF_STATUS_OK : NERF_STATUS_CUDA_ERROR;
     }
-    const bool on_the_way = dx && dz_on_the_way(d) && copied && (p.dz_needed || dbias);
+    const bool on_the_way = dx && d.n_rows > 64u && dz_on_the_way(d) && copied && (p.dz_needed || dbias);
     if (on_the_way) {
         DxArgs a{};
         a.n = d.n_rows;
