@@ -943,36 +943,49 @@ __global__ void __launch_bounds__(256, 3) k_dz(const DzArgs a, uint32_t cg_log2)
 // Blocks below n_dw: groups of 32 rows x 4 columns of dw, `share` of a block's
 // sixteen warps a group; the others: 32 columns of db.  The warps of a group take
 // equal ranges of the parts, with the loads of a batch in flight together (148
-// parts, one a CTA, are one batch for sixteen), and the first adds their sums: a
-// fixed order.  With eight warps and batches of eight the sums of 148 parts of a
-// 64 x 64 layer took 14 us, most of it waiting; now 6.
-constexpr uint32_t kSumWarps = 16, kSumBatch = 10;
-__global__ void __launch_bounds__(32 * kSumWarps, 1) k_grad_reduce(const GradReduceArgs a, uint32_t n_dw, uint32_t share) {
+// parts, one a CTA, are one batch for sixteen), and their sums are added in their
+// order: the same bits every time.  With eight warps and batches of eight the sums
+// of 148 parts of a 64 x 64 layer took 14 us, most of it waiting; now 6.  Of few
+// parts a batch is four, so that an SM holds three blocks, and groups side by side
+// in a block let it write up to 64 bytes of a row at once (two parts of 1536 x 1536:
+// 32 us with batches of ten, four scattered values a thread; now 13).
+constexpr uint32_t kSumWarps = 16, kSumBatch = 10, kSumFew = 4;
+template <uint32_t BATCH>
+__global__ void __launch_bounds__(32 * kSumWarps, BATCH == kSumFew ? 3 : 1) k_grad_reduce(const GradReduceArgs a, uint32_t n_dw, uint32_t share) {
     __shared__ float4 ws[kSumWarps][32];
     const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
     after_previous();
     let_next_start();
     if (blockIdx.x < n_dw) {
-        const uint32_t per_tile = a.bn / 4u, sub = warp & (share - 1u), group = blockIdx.x * (kSumWarps / share) + warp / share;
-        const uint32_t quarter = group & 3u, idx = group >> 2;
-        // half: 128 rows of a tile (a pair of CTAs leaves two)
-        const uint32_t half = idx / per_tile, c4 = idx - half * per_tile, row = 32u * quarter + lane;
-        const uint32_t tiles = a.tiles_m * a.tiles_n, tile = half / a.ctas;
-        const uint32_t per = 16u * a.tiles_n, set = tile / per, first = 16u * set;
-        const uint32_t gm = min(16u, a.tiles_m - first), r = tile - set * per;
-        const uint32_t m = ((first + r % gm) * a.ctas + half % a.ctas) * kBM + row, n = (r / gm) * a.bn + 4u * c4;
-        const bool live = half < tiles * a.ctas && m - lane < a.n_out && n < a.n_in;  // the same in the whole warp
+        const bool bf16 = a.bf16 != 0u;
+        const uint32_t per_tile = a.bn / 4u, here = kSumWarps / share, tiles = a.tiles_m * a.tiles_n;
+        // Group i: columns 4 (i mod 4) .. of 16, then rows 32 (i / 4 mod 4) .. of 128, then the 16 columns and the tile.
+        const auto place = [&](uint32_t i, uint32_t& half, uint32_t& c4, uint32_t& row0) {
+            half = (i >> 4) / (per_tile / 4u);  // 128 rows of a tile (a pair of CTAs leaves two)
+            c4 = 4u * ((i >> 4) - half * (per_tile / 4u)) + (i & 3u);
+            row0 = 32u * ((i >> 2) & 3u);
+        };
+        const auto corner = [&](uint32_t half, uint32_t& m0, uint32_t& n0) {  // of the half's tile
+            const uint32_t tile = half / a.ctas, per = 16u * a.tiles_n, set = tile / per, first = 16u * set;
+            const uint32_t gm = min(16u, a.tiles_m - first), r = tile - set * per;
+            m0 = ((first + r % gm) * a.ctas + half % a.ctas) * kBM;
+            n0 = (r / gm) * a.bn;
+        };
+        const uint32_t sub = warp & (share - 1u);
+        uint32_t half, c4, row0, m0, n0;
+        place(blockIdx.x * here + warp / share, half, c4, row0);
+        corner(half, m0, n0);
         float4 t = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (live) {
-            const float4* src = reinterpret_cast<const float4*>(a.partials) + (static_cast<uint64_t>(half) * per_tile + c4) * kBM + row;
+        if (half < tiles * a.ctas && m0 + row0 < a.n_out && n0 + 4u * c4 < a.n_in) {  // the same in the whole warp
+            const float4* src = reinterpret_cast<const float4*>(a.partials) + (static_cast<uint64_t>(half) * per_tile + c4) * kBM + row0 + lane;
             const uint64_t step = static_cast<uint64_t>(tiles) * a.ctas * per_tile * kBM;
             const uint32_t each = (a.splits + share - 1u) / share, k0 = min(a.splits, sub * each), k1 = min(a.splits, k0 + each);
-            for (uint32_t k = k0; k < k1; k += kSumBatch) {
-                float4 v[kSumBatch];
+            for (uint32_t k = k0; k < k1; k += BATCH) {
+                float4 v[BATCH];
 #pragma unroll
-                for (uint32_t j = 0; j < kSumBatch; ++j) v[j] = k + j < k1 ? __ldcs(src + (k + j) * step) : make_float4(0.f, 0.f, 0.f, 0.f);
+                for (uint32_t j = 0; j < BATCH; ++j) v[j] = k + j < k1 ? __ldcs(src + (k + j) * step) : make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-                for (uint32_t j = 0; j < kSumBatch; ++j) {
+                for (uint32_t j = 0; j < BATCH; ++j) {
                     t.x += v[j].x;
                     t.y += v[j].y;
                     t.z += v[j].z;
@@ -982,18 +995,45 @@ __global__ void __launch_bounds__(32 * kSumWarps, 1) k_grad_reduce(const GradRed
         }
         ws[warp][lane] = t;
         __syncthreads();
-        if (sub != 0u || !live || m >= a.n_out) return;
+        // Thread i takes four values of a row: neighbours those of the groups side by side.
+        const uint32_t beside = min(here, 4u), i = threadIdx.x;
+        if (i >= 32u * here) return;
+        const uint32_t g = i % beside + beside * (i / (32u * beside)), from = (i / beside) & 31u;
+        place(blockIdx.x * here + g, half, c4, row0);
+        corner(half, m0, n0);
+        const uint32_t m = m0 + row0 + from, n = n0 + 4u * c4;
+        if (half >= tiles * a.ctas || m >= a.n_out || n >= a.n_in) return;
+        t = ws[g * share][from];
         for (uint32_t w = 1; w < share; ++w) {
-            const float4 v = ws[warp + w][lane];
+            const float4 v = ws[g * share + w][from];
             t.x += v.x;
             t.y += v.y;
             t.z += v.z;
             t.w += v.w;
         }
+        const uint64_t at = static_cast<uint64_t>(m) * a.n_in + n;
+        if (a.f32 && a.dw_vec) {
+            float4* q = reinterpret_cast<float4*>(static_cast<float*>(a.dw) + at);
+            if (a.accumulate) {
+                const float4 v = *q;
+                t = make_float4(v.x + t.x, v.y + t.y, v.z + t.z, v.w + t.w);
+            }
+            *q = t;
+            return;
+        }
+        if (a.dw_vec) {
+            uint2* q = reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.dw) + at);
+            if (a.accumulate) {
+                const float2 lo = unpack_16(q->x, bf16), hi = unpack_16(q->y, bf16);
+                t = make_float4(lo.x + t.x, lo.y + t.y, hi.x + t.z, hi.y + t.w);
+            }
+            *q = make_uint2(pack_16(t.x, t.y, bf16), pack_16(t.z, t.w, bf16));
+            return;
+        }
         const float o[4] = {t.x, t.y, t.z, t.w};
 #pragma unroll
-        for (uint32_t i = 0; i < 4u; ++i)
-            if (n + i < a.n_in) grad_out(a.dw, static_cast<uint64_t>(m) * a.n_in + n + i, o[i], a.f32 != 0u, a.bf16 != 0u, a.accumulate != 0u);
+        for (uint32_t j = 0; j < 4u; ++j)
+            if (n + j < a.n_in) grad_out(a.dw, at + j, o[j], a.f32 != 0u, bf16, a.accumulate != 0u);
         return;
     }
     const uint32_t c = 32u * (blockIdx.x - n_dw) + lane;
@@ -1094,12 +1134,13 @@ cudaError_t launch_dz(const DzArgs& a, cudaStream_t s) {
 
 cudaError_t launch_grad_reduce(const GradReduceArgs& a, cudaStream_t s) {
     uint32_t share = 1u;  // warps a group: one batch of loads each
+    const bool few = a.splits <= kSumFew;
     while (share < kSumWarps && share * kSumBatch < a.splits) share *= 2u;
     const uint32_t groups = a.dw ? a.tiles_m * a.tiles_n * a.ctas * (a.bn / 4u) * 4u : 0u, per_block = kSumWarps / share;
     const uint32_t n_dw = (groups + per_block - 1u) / per_block;
     const uint32_t n_db = a.db ? (a.n_out + 31u) / 32u : 0u;
     if (n_dw + n_db == 0u) return cudaSuccess;
-    return launch_after(k_grad_reduce, dim3(n_dw + n_db), 32u * kSumWarps, 0u, 1u, s, a, n_dw, share);
+    return launch_after(few ? k_grad_reduce<kSumFew> : k_grad_reduce<kSumBatch>, dim3(n_dw + n_db), 32u * kSumWarps, 0u, 1u, s, a, n_dw, share);
 }
 
 }  // namespace nb

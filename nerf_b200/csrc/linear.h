@@ -86,6 +86,7 @@ struct GradReduceArgs {
     uint32_t parts;
     void *dw, *db;  // null: none
     uint32_t f32, bf16, accumulate;
+    uint32_t dw_vec;  // four values of dw at once: aligned rows of a multiple of four
 };
 cudaError_t launch_grad_reduce(const GradReduceArgs& a, cudaStream_t s);
 

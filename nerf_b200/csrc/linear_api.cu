@@ -395,6 +395,7 @@ NERF_API NerfStatus nerf_b200_linear_backward(const NerfB200Linear* desc, const 
     r.f32 = d.grad_dtype == NERF_B200_F32;
     r.bf16 = bf16;
     r.accumulate = d.accumulate;
+    r.dw_vec = aligned(dweight, 4u * es) && d.n_in % 4u == 0u;
     if (dbias) {
         r.db_part = reinterpret_cast<float*>(ws + p.o_db);
         r.parts = p.parts;
