@@ -147,14 +147,15 @@ struct GemmShape {
     static constexpr uint32_t kLoaders = FEED == kFeedRaw ? 8u : FEED == kFeedRawShort ? 4u : 0u;
     static constexpr uint32_t kBoxN = kPair ? BN / 2u : BN;  // rows of B in this CTA's shared memory
     static constexpr uint32_t kStageBytes = kStageBytesA + kBoxN * 128u;
-    // Epilogue groups of four warps, an accumulator each: tiles of up to 128
-    // columns are bound by memory and by the latency of their epilogues.
-    static constexpr uint32_t kGroups = KIND == kGemmRows && BN <= 128u && FEED != kFeedRaw ? 4u : 2u;
+    // Epilogue groups of four warps: the epilogues' latency is what bounds short products.  Up to 128 columns a tile
+    // each has an accumulator, of 256 two share one, a half each.
+    static constexpr uint32_t kGroups = KIND == kGemmRows && FEED != kFeedRaw ? 4u : 2u;
+    static constexpr uint32_t kAccs = BN == 256u ? 2u : kGroups, kColsGroup = KIND == kGemmRows ? BN * kAccs / kGroups : BN;
     static constexpr uint32_t kRawBytes = raw_bytes(kBM) + raw_bytes(kBoxN);  // raw copies of a step
     static constexpr uint32_t kRaws = kRaw ? kRawRing * kRawBytes : 0u;
     static constexpr uint32_t kStages = kRaw ? 2u : kPair ? 5u : BN >= 128u ? 3u : 4u;
-    static constexpr uint32_t kSlabs = FEED == kFeedRawShort ? 1u : 2u;  // per epilogue warp
-    static constexpr uint32_t kSmem = 1024u + kStages * kStageBytes + kRaws + 4u * kGroups * kSlabs * kSlabBytes + kGroups * BN * 2u;
+    static constexpr uint32_t kSlabs = FEED == kFeedRawShort || (KIND == kGemmRows && BN == 256u) ? 1u : 2u;  // per epilogue warp
+    static constexpr uint32_t kSmem = 1024u + kStages * kStageBytes + kRaws + 4u * kGroups * kSlabs * kSlabBytes + kAccs * BN * 2u;
     static constexpr uint32_t kFirstLoader = 4u + 4u * kGroups;
     static constexpr uint32_t kThreads = 32u * (kFirstLoader + kLoaders);
     // Weight gradients of 256 columns keep 128 sums a thread: registers move
@@ -166,13 +167,13 @@ struct GemmShape {
 };
 
 // Warps: 0 operand copies, 1 MMA, 2 tensor-memory allocation, from 4 on the
-// epilogue groups of four, which take turns (item i of the CTA: group and
-// accumulator i % kGroups), then the ones that place raw copies (kFeedRaw).
+// epilogue groups of four, which take turns (item i of the CTA: accumulator
+// i % kAccs and its groups), then the ones that place raw copies (kFeedRaw).
 template <uint32_t BN, int KIND, int FEED>
 __global__ void __launch_bounds__(GemmShape<BN, KIND, FEED>::kThreads, 1) k_gemm(const GemmArgs g, const __grid_constant__ GemmMaps maps) {
     using S = GemmShape<BN, KIND, FEED>;
     constexpr uint32_t kStages = S::kStages, kStageBytes = S::kStageBytes;
-    constexpr uint32_t kCols = tmem_cols(S::kGroups * BN);
+    constexpr uint32_t kCols = tmem_cols(S::kAccs * BN);
     constexpr uint32_t kCtas = S::kPair ? 2u : 1u;
     extern __shared__ unsigned char smem_raw[];
     __shared__ Barriers bar;
@@ -196,9 +197,9 @@ __global__ void __launch_bounds__(GemmShape<BN, KIND, FEED>::kThreads, 1) k_gemm
                 umma::mbar_init(&bar.raw_empty[o][i], S::kLoaders);
             }
         }
-        for (uint32_t i = 0; i < S::kGroups; ++i) {
+        for (uint32_t i = 0; i < S::kAccs; ++i) {
             umma::mbar_init(&bar.acc_full[i], 1u);
-            umma::mbar_init(&bar.acc_empty[i], (KIND == kGemmGrad ? 8u : 4u) * kCtas);
+            umma::mbar_init(&bar.acc_empty[i], (KIND == kGemmGrad ? 8u : 4u * S::kGroups / S::kAccs) * kCtas);
         }
         for (uint32_t i = 0; i < 4u * S::kGroups; ++i) umma::mbar_init(&bar.res[i], 1u);
         umma::mbar_init(&bar.drain, 1u);
@@ -373,7 +374,7 @@ __global__ void __launch_bounds__(GemmShape<BN, KIND, FEED>::kThreads, 1) k_gemm
                 if (S::kPair) tma::commit_pair(&bar.acc_full[acc]);
                 else umma::commit(&bar.acc_full[acc]);
             }
-            acc = acc + 1u == S::kGroups ? 0u : acc + 1u;
+            acc = acc + 1u == S::kAccs ? 0u : acc + 1u;
             if (acc == 0u) acc_parity ^= 1u;
             }
         }
@@ -511,10 +512,10 @@ __global__ void __launch_bounds__(GemmShape<BN, KIND, FEED>::kThreads, 1) k_gemm
         if (lane == 0u) tma::store_wait_all();
     } else if (KIND == kGemmRows && warp >= 4u && warp < S::kFirstLoader) {
         // ---- epilogue: warp q of a group drains rows 32 q .. 32 q + 31 of the tile
-        const uint32_t q = warp & 3u, acc = (warp >> 2) - 1u;
+        const uint32_t q = warp & 3u, group = (warp >> 2) - 1u, acc = group % S::kAccs, c_first = group / S::kAccs * S::kColsGroup;
         unsigned char* my_slabs = slabs + (warp - 4u) * S::kSlabs * kSlabBytes;
-        uint16_t* bias_s = bias_all + acc * BN;
-        const uint32_t taddr = tmem + acc * BN + ((32u * q) << 16);
+        uint16_t* bias_s = bias_all + acc * BN + c_first;
+        const uint32_t taddr = tmem + acc * BN + c_first + ((32u * q) << 16);
         const uint32_t acc_empty = S::kPair ? tma::peer_addr(smem_u32(&bar.acc_empty[acc]), 0u) : 0u;
         uint32_t parity = 0, res_parity = 0, slab_i = 0, bias_n = ~0u;
         bool ok = true;  // after a wait that ran out the warp only keeps the named barriers' count
@@ -529,27 +530,27 @@ __global__ void __launch_bounds__(GemmShape<BN, KIND, FEED>::kThreads, 1) k_gemm
             slab_i = slab_i + 1u == S::kSlabs ? 0u : slab_i + 1u;
             return p;
         };
-        for (uint32_t it = first_item + acc * item_step; it < items; it += S::kGroups * item_step) {
+        for (uint32_t it = first_item + acc * item_step; it < items; it += S::kAccs * item_step) {
             uint32_t tm, tn;
             locate(it, tm, tn);
-            const uint32_t m0 = (tm * kCtas + rank) * kBM + 32u * q, n0 = tn * BN;
+            const uint32_t m0 = (tm * kCtas + rank) * kBM + 32u * q, n0 = tn * BN + c_first;
             const uint32_t rows = m0 < g.M ? min(32u, g.M - m0) : 0u;
             if (n0 != bias_n) {  // the tile's bias, kept while the columns stay the same
-                asm volatile("bar.sync %0, 128;\n" ::"r"(1u + acc) : "memory");
-                for (uint32_t c = threadIdx.x & 127u; c < BN; c += 128u)
+                asm volatile("bar.sync %0, 128;\n" ::"r"(1u + group) : "memory");
+                for (uint32_t c = threadIdx.x & 127u; c < S::kColsGroup; c += 128u)
                     bias_s[c] = g.bias && n0 + c < g.N ? static_cast<const uint16_t*>(g.bias)[n0 + c] : static_cast<uint16_t>(0);
-                asm volatile("bar.sync %0, 128;\n" ::"r"(1u + acc) : "memory");
+                asm volatile("bar.sync %0, 128;\n" ::"r"(1u + group) : "memory");
                 bias_n = n0;
             }
             if (g.res_tma && lane == 0u) {
                 // The residual of this group's next tile (and of its first) on its way to the L2 cache.
                 for (uint32_t w = it == first_item + acc * item_step ? 0u : 1u; w < 2u; ++w) {
-                    const uint32_t jt = it + S::kGroups * w * item_step;
+                    const uint32_t jt = it + S::kAccs * w * item_step;
                     if (jt >= items) break;
                     uint32_t jm, jn;
                     locate(jt, jm, jn);
                     const uint32_t jr = (jm * kCtas + rank) * kBM + 32u * q;
-                    for (uint32_t c = jn * BN; jr < g.M && c < min(jn * BN + BN, g.N); c += 64u)
+                    for (uint32_t c = jn * BN + c_first; jr < g.M && c < min(jn * BN + c_first + S::kColsGroup, g.N); c += 64u)
                         tma::prefetch_2d(&maps.res, static_cast<int32_t>(c), static_cast<int32_t>(jr));
                 }
             }
@@ -561,7 +562,7 @@ __global__ void __launch_bounds__(GemmShape<BN, KIND, FEED>::kThreads, 1) k_gemm
             if (!ok) continue;
             umma::fence_after_sync();
 #pragma unroll 1
-            for (uint32_t c0 = 0; c0 < BN && n0 + c0 < g.N; c0 += 64u) {
+            for (uint32_t c0 = 0; c0 < S::kColsGroup && n0 + c0 < g.N; c0 += 64u) {
                 const uint32_t cols = min(64u, g.N - n0 - c0);
                 unsigned char* slab_z = g.pre.ptr ? next_slab(0u) : nullptr;
                 if (S::kSlabs == 1u && g.pre.ptr) {  // one slab for both: z by itself first
