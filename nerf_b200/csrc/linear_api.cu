@@ -97,18 +97,16 @@ bool make_operand_map(CUtensorMap* map, const MatrixView& m, uint32_t raw, bool 
 // ------------------------------------------------------------------- plans
 // Tile width of an activation product: the number of waves of 128 x bn tiles
 // times the time of one, which grows with bn and has a part (the row panel's
-// copy) that does not.
-// Up to K = 256 the epilogues take the time, and 128 columns have twice the
-// epilogue warps (65536 x 256 -> 256 with residual 27.9 us with 128 columns and
-// 31.5 with 256; at K = 512 both take 29.2).
-uint32_t pick_bn(uint32_t tiles_m, uint32_t n, uint32_t k, bool raw, uint32_t sms) {
-    const uint32_t widest = raw ? kGemmRawBN : k <= 256u ? 128u : 256u;
+// copy, the accumulator's round trip) that does not: 65536 x 384 -> 384 38.1 us
+// with a part of 64 columns, 31.6 with one of 128.
+uint32_t pick_bn(uint32_t tiles_m, uint32_t n, bool raw, uint32_t sms) {
+    const uint32_t widest = raw ? kGemmRawBN : 256u;
     uint32_t best = widest;
     uint64_t cost = ~0ull;
     for (uint32_t bn = widest; bn >= 64u; bn /= 2u) {
         if (bn > 64u && bn / 2u >= n) continue;  // half of it holds every column
         const uint64_t tiles = static_cast<uint64_t>(tiles_m) * ceil_div(n, bn);
-        const uint64_t c = ((tiles + sms - 1u) / sms) * (bn + 64u);
+        const uint64_t c = ((tiles + sms - 1u) / sms) * (bn + 128u);
         if (c < cost) {
             cost = c;
             best = bn;
@@ -301,7 +299,7 @@ cudaError_t run_rows(GemmArgs& g, uint32_t sms, cudaStream_t s) {
     const bool pair = g.a.vec >= 8u && g.b.vec >= 8u && pair_pays(g.M, g.N, g.K, sms);
     if (!pair && cols_pay(g.M, g.N, g.K, sms)) return run_cols(g, s, sms);
     g.tiles_m = ceil_div(g.M, pair ? 2u * kGemmBM : kGemmBM);
-    const uint32_t bn = pair ? kGemmPairBN : pick_bn(g.tiles_m, g.N, g.K, g.a.vec < 8u || g.b.vec < 8u, sms);
+    const uint32_t bn = pair ? kGemmPairBN : pick_bn(g.tiles_m, g.N, g.a.vec < 8u || g.b.vec < 8u, sms);
     g.tiles_n = ceil_div(g.N, bn);
     g.splits = 1u;
     g.k_steps = g.steps_per_split = ceil_div(g.K, kGemmBK);
