@@ -46,7 +46,7 @@ constexpr uint32_t kMaxStages = 8;
 // cycles), so the operands' are issued by a warp each.  2000 x 4000 -> 4000 with
 // rows 4001 apart took 356 us with loads to registers instead, and 430 us with
 // 16-byte asynchronous copies by the warps that move the rows.
-constexpr uint32_t kRawRing = 2;  // steps of raw copies in shared memory
+constexpr uint32_t kRawRing = 2, kMaxRing = 3;  // steps of raw copies in shared memory
 
 // Bytes of one residue's copy: of n rows (K-major), of 64 rows x 128 columns (MN-major).
 constexpr uint32_t kRawMn = 8u * kRawColsMn * 2u;
@@ -125,7 +125,7 @@ NB_DEV void raw_box(unsigned char* box, const unsigned char* raw, const MatrixVi
 // ------------------------------------------------------------------ the GEMM
 struct Barriers {
     uint64_t full[kMaxStages], empty[kMaxStages];
-    uint64_t raw_full[2][kRawRing], raw_empty[2][kRawRing];  // of A and of B
+    uint64_t raw_full[2][kMaxRing], raw_empty[2][kMaxRing];  // of A and of B
     uint64_t acc_full[4], acc_empty[4];
     uint64_t res[16];  // an epilogue warp's residual rows have arrived
     uint64_t drain;
@@ -151,10 +151,11 @@ struct GemmShape {
     // each has an accumulator, of 256 two share one, a half each.
     static constexpr uint32_t kGroups = KIND == kGemmRows && FEED != kFeedRaw ? 4u : 2u;
     static constexpr uint32_t kAccs = BN == 256u ? 2u : kGroups, kColsGroup = KIND == kGemmRows ? BN * kAccs / kGroups : BN;
+    static constexpr uint32_t kRing = FEED == kFeedRaw ? kMaxRing : kRawRing;
     static constexpr uint32_t kRawBytes = raw_bytes(kBM) + raw_bytes(kBoxN);  // raw copies of a step
-    static constexpr uint32_t kRaws = kRaw ? kRawRing * kRawBytes : 0u;
+    static constexpr uint32_t kRaws = kRaw ? kRing * kRawBytes : 0u;
     static constexpr uint32_t kStages = kRaw ? 2u : kPair ? 5u : BN >= 128u ? 3u : 4u;
-    static constexpr uint32_t kSlabs = FEED == kFeedRawShort || (KIND == kGemmRows && BN == 256u) ? 1u : 2u;  // per epilogue warp
+    static constexpr uint32_t kSlabs = kRaw || (KIND == kGemmRows && BN == 256u) ? 1u : 2u;  // per epilogue warp
     static constexpr uint32_t kSmem = 1024u + kStages * kStageBytes + kRaws + 4u * kGroups * kSlabs * kSlabBytes + kAccs * BN * 2u;
     static constexpr uint32_t kFirstLoader = 4u + 4u * kGroups;
     static constexpr uint32_t kThreads = 32u * (kFirstLoader + kLoaders);
@@ -191,7 +192,7 @@ __global__ void __launch_bounds__(GemmShape<BN, KIND, FEED>::kThreads, 1) k_gemm
             umma::mbar_init(&bar.full[i], S::kRaw ? S::kLoaders + (g.a_raw && g.b_raw ? 0u : 1u) : 1u);
             umma::mbar_init(&bar.empty[i], 1u);
         }
-        for (uint32_t i = 0; S::kRaw && i < kRawRing; ++i) {
+        for (uint32_t i = 0; S::kRaw && i < S::kRing; ++i) {
             for (uint32_t o = 0; o < 2u; ++o) {
                 umma::mbar_init(&bar.raw_full[o][i], 1u);
                 umma::mbar_init(&bar.raw_empty[o][i], S::kLoaders);
@@ -264,8 +265,8 @@ __global__ void __launch_bounds__(GemmShape<BN, KIND, FEED>::kThreads, 1) k_gemm
                 const bool kept = op && keep_b && issued >= kStages;
                 if (raw) {
                     if (kept) break;  // placed for good
-                    const uint32_t r = issued % kRawRing;
-                    ok = tma::wait(&bar.raw_empty[op][r], (issued / kRawRing + 1u) & 1u);
+                    const uint32_t r = issued % S::kRing;
+                    ok = tma::wait(&bar.raw_empty[op][r], (issued / S::kRing + 1u) & 1u);
                     if (!ok) break;
                     raw_load(raws + r * S::kRawBytes + op * raw_bytes(kBM), map, m, mn, width, at, k0, &bar.raw_full[op][r]);
                 } else {
@@ -290,8 +291,8 @@ __global__ void __launch_bounds__(GemmShape<BN, KIND, FEED>::kThreads, 1) k_gemm
         if (!ok) {  // copies in flight: wait for them before the shared memory goes
             atomicOr(g.error, 1u);
             if (raw) {
-                for (uint32_t i = issued > kRawRing ? issued - kRawRing : 0u; i < issued; ++i)
-                    tma::wait(&bar.raw_full[op][i % kRawRing], (i / kRawRing) & 1u);
+                for (uint32_t i = issued > S::kRing ? issued - S::kRing : 0u; i < issued; ++i)
+                    tma::wait(&bar.raw_full[op][i % S::kRing], (i / S::kRing) & 1u);
             } else if (rank == 0u) {
                 for (uint32_t i = issued > kStages ? issued - kStages : 0u; i < issued; ++i)
                     tma::wait(&bar.full[i % kStages], (i / kStages) & 1u);
@@ -308,7 +309,7 @@ __global__ void __launch_bounds__(GemmShape<BN, KIND, FEED>::kThreads, 1) k_gemm
             uint32_t tm, tn;
             locate(it - split * tiles, tm, tn);
             for (uint32_t ks = ks0; ks < ks1; ++ks, ++i) {
-                const uint32_t stage = i % kStages, r = i % kRawRing, turn = (i / kRawRing) & 1u;
+                const uint32_t stage = i % kStages, r = i % S::kRing, turn = (i / S::kRing) & 1u;
                 const bool place_b = g.b_raw && !(keep_b && i >= kStages);
                 ok = tma::wait(&bar.empty[stage], (i / kStages + 1u) & 1u) && (!g.a_raw || tma::wait(&bar.raw_full[0][r], turn)) &&
                      (!place_b || tma::wait(&bar.raw_full[1][r], turn));
@@ -468,7 +469,7 @@ __global__ void __launch_bounds__(GemmShape<BN, KIND, FEED>::kThreads, 1) k_gemm
             const auto free_slab = [&]() -> unsigned char* {
                 if (lane == 0u) tma::store_wait_read<S::kSlabs - 1u>();
                 __syncwarp();
-                slab_i ^= 1u;
+                slab_i = S::kSlabs > 1u ? slab_i ^ 1u : 0u;
                 return my_slabs + slab_i * kSlabBytes;
             };
             if (g.dw_f32) {
