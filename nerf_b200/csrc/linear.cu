@@ -555,6 +555,18 @@ __global__ void __launch_bounds__(GemmShape<BN, KIND, FEED>::kThreads, 1) k_gemm
                         tma::prefetch_2d(&maps.res, static_cast<int32_t>(c), static_cast<int32_t>(jr));
                 }
             }
+            if (g.res.ptr && !g.res_tma) {
+                // Likewise of rows that the copy unit cannot read: a lane asks for its row's columns, 128 bytes at a time.
+                for (uint32_t w = it == first_item + acc * item_step ? 0u : 1u; w < 2u; ++w) {
+                    const uint32_t jt = it + S::kAccs * w * item_step;
+                    if (jt >= items) break;
+                    uint32_t jm, jn;
+                    locate(jt, jm, jn);
+                    const uint32_t jr = (jm * kCtas + rank) * kBM + 32u * q + lane, end = min(jn * BN + c_first + S::kColsGroup, g.N);
+                    for (uint32_t c = jn * BN + c_first; jr < g.M && c < end; c += 64u)
+                        prefetch_l2(static_cast<const uint16_t*>(g.res.ptr) + jr * g.res.ld + c);
+                }
+            }
             if (ok && !tma::wait(&bar.acc_full[acc], parity)) {
                 atomicOr(g.error, 1u);
                 ok = false;

@@ -144,6 +144,9 @@ NB_DEV uint32_t load_32(const void* q, bool on) {
     return v;
 }
 
+// The line at q on its way to the L2 cache.
+NB_DEV void prefetch_l2(const void* q) { asm volatile("prefetch.global.L2 [%0];\n" ::"l"(q)); }
+
 // ------------------------------------------------- slabs: 32 rows x 128 bytes
 // A warp's shared-memory slab, 16-byte pieces swizzled by the row so that both
 // "one row a thread" and "eight threads a row" accesses are conflict-free.
@@ -195,43 +198,67 @@ NB_DEV void slab_copy(unsigned char* slab, unsigned char* g, uint64_t ld, uint32
         }
         return;
     }
-    // A row is 32 words of the slab: lane i moves word i, as one or two values.
+    // Rows that start on words: a row is 32 words of the slab, lane i moves word i.  Others of 16-bit values: lane i
+    // moves values i and 32 + i, so that an instruction takes 64 bytes in a row.
     const bool words = ES == 4 || ((reinterpret_cast<uintptr_t>(g) & 3u) == 0u && (ld & 1u) == 0u);
-    const bool lo = ES == 4 ? lane < cols : 2u * lane < cols, hi = ES == 4 ? lane < cols : 2u * lane + 1u < cols;
     const uint64_t step = ld * ES;
-    unsigned char* q = g + 4u * lane;
     constexpr uint32_t kBatch = 8;
+    if (ES == 2 && !(words && !(cols & 1u))) {
+        const bool lo = lane < cols, hi = lane + 32u < cols;
+        uint16_t* q = reinterpret_cast<uint16_t*>(g) + lane;
+        const uint32_t in_piece = 2u * (lane & 7u);
+#pragma unroll 1
+        for (uint32_t r0 = 0; r0 < rows; r0 += kBatch) {
+            const uint32_t in = rows - r0;
+            uint32_t w[kBatch], v[kBatch];
+            const auto at = [&](uint32_t j, uint32_t h) { return reinterpret_cast<uint16_t*>(slab + slab_at(r0 + j, (lane >> 3) + 4u * h) + in_piece); };
+            if (kStore) {
+#pragma unroll
+                for (uint32_t j = 0; j < kBatch; ++j) {
+                    w[j] = *at(j, 0u);
+                    v[j] = *at(j, 1u);
+                }
+#pragma unroll
+                for (uint32_t j = 0; j < kBatch; ++j) {
+                    uint16_t* p = reinterpret_cast<uint16_t*>(reinterpret_cast<unsigned char*>(q) + j * step);
+                    if (lo && j < in) p[0] = static_cast<uint16_t>(w[j]);
+                    if (hi && j < in) p[32] = static_cast<uint16_t>(v[j]);
+                }
+            } else {
+#pragma unroll
+                for (uint32_t j = 0; j < kBatch; ++j) {
+                    const uint16_t* p = reinterpret_cast<const uint16_t*>(reinterpret_cast<const unsigned char*>(q) + j * step);
+                    w[j] = load_16(p, lo && j < in);
+                    v[j] = load_16(p + 32, hi && j < in);
+                }
+#pragma unroll
+                for (uint32_t j = 0; j < kBatch; ++j) {
+                    *at(j, 0u) = static_cast<uint16_t>(w[j]);
+                    *at(j, 1u) = static_cast<uint16_t>(v[j]);
+                }
+            }
+            q = reinterpret_cast<uint16_t*>(reinterpret_cast<unsigned char*>(q) + kBatch * step);
+        }
+        return;
+    }
+    const bool on = ES == 4 ? lane < cols : 2u * lane < cols;
+    unsigned char* q = g + 4u * lane;
 #pragma unroll 1
     for (uint32_t r0 = 0; r0 < rows; r0 += kBatch) {
         const uint32_t in = rows - r0;
         uint32_t w[kBatch];
-        unsigned char* l[kBatch];
-#pragma unroll
-        for (uint32_t j = 0; j < kBatch; ++j) l[j] = slab + slab_at(r0 + j, lane >> 2) + 4u * (lane & 3u);
+        const auto at = [&](uint32_t j) { return reinterpret_cast<uint32_t*>(slab + slab_at(r0 + j, lane >> 2) + 4u * (lane & 3u)); };
         if (kStore) {
 #pragma unroll
-            for (uint32_t j = 0; j < kBatch; ++j) w[j] = *reinterpret_cast<const uint32_t*>(l[j]);
+            for (uint32_t j = 0; j < kBatch; ++j) w[j] = *at(j);
 #pragma unroll
-            for (uint32_t j = 0; j < kBatch; ++j) {
-                unsigned char* p = q + j * step;
-                if (words && !(cols & 1u)) {
-                    if (hi && j < in) *reinterpret_cast<uint32_t*>(p) = w[j];
-                } else if (ES == 4) {
-                    if (lo && j < in) *reinterpret_cast<uint32_t*>(p) = w[j];
-                } else {
-                    if (lo && j < in) *reinterpret_cast<uint16_t*>(p) = static_cast<uint16_t>(w[j]);
-                    if (hi && j < in) reinterpret_cast<uint16_t*>(p)[1] = static_cast<uint16_t>(w[j] >> 16);
-                }
-            }
+            for (uint32_t j = 0; j < kBatch; ++j)
+                if (on && j < in) *reinterpret_cast<uint32_t*>(q + j * step) = w[j];
         } else {
 #pragma unroll
-            for (uint32_t j = 0; j < kBatch; ++j) {
-                const uint16_t* p = reinterpret_cast<const uint16_t*>(q + j * step);
-                if (ES == 4 || (words && !(cols & 1u))) w[j] = load_32(p, hi && j < in);
-                else w[j] = load_16(p, lo && j < in) | (load_16(p + 1, hi && j < in) << 16);
-            }
+            for (uint32_t j = 0; j < kBatch; ++j) w[j] = load_32(q + j * step, on && j < in);
 #pragma unroll
-            for (uint32_t j = 0; j < kBatch; ++j) *reinterpret_cast<uint32_t*>(l[j]) = w[j];
+            for (uint32_t j = 0; j < kBatch; ++j) *at(j) = w[j];
         }
         q += kBatch * step;
     }
