@@ -144,7 +144,9 @@ NB_DEV void tile_of(const GemmArgs& g, uint32_t t, uint32_t& tm, uint32_t& tn) {
 template <uint32_t BN, int KIND, int FEED>
 struct GemmShape {
     static constexpr bool kPair = FEED == kFeedPair, kRaw = FEED == kFeedRaw || FEED == kFeedRawShort;
+    // Warps that place the raw copies of a step, and teams of them that take the steps in turn.
     static constexpr uint32_t kLoaders = FEED == kFeedRaw ? 8u : FEED == kFeedRawShort ? 4u : 0u;
+    static constexpr uint32_t kTeams = FEED == kFeedRaw && KIND == kGemmRows ? 2u : 1u;
     static constexpr uint32_t kBoxN = kPair ? BN / 2u : BN;  // rows of B in this CTA's shared memory
     static constexpr uint32_t kStageBytes = kStageBytesA + kBoxN * 128u;
     // Epilogue groups of four warps: the epilogues' latency is what bounds short products.  Up to 128 columns a tile
@@ -158,7 +160,7 @@ struct GemmShape {
     static constexpr uint32_t kSlabs = kRaw || (KIND == kGemmRows && BN == 256u) ? 1u : 2u;  // per epilogue warp
     static constexpr uint32_t kSmem = 1024u + kStages * kStageBytes + kRaws + 4u * kGroups * kSlabs * kSlabBytes + kAccs * BN * 2u;
     static constexpr uint32_t kFirstLoader = 4u + 4u * kGroups;
-    static constexpr uint32_t kThreads = 32u * (kFirstLoader + kLoaders);
+    static constexpr uint32_t kThreads = 32u * (kFirstLoader + kTeams * kLoaders);
     // Weight gradients of 256 columns keep 128 sums a thread: registers move
     // from the copying and issuing warps to the two groups that sum.
     static constexpr bool kRegs = KIND == kGemmGrad && BN == 256u;
@@ -300,7 +302,8 @@ __global__ void __launch_bounds__(GemmShape<BN, KIND, FEED>::kThreads, 1) k_gemm
         }
     } else if (S::kRaw && warp >= S::kFirstLoader) {
         // ---- raw copies into place
-        const uint32_t w = warp - S::kFirstLoader;
+        constexpr uint32_t kTeam = S::kLoaders ? S::kLoaders : 1u;
+        const uint32_t w = (warp - S::kFirstLoader) % kTeam, team = (warp - S::kFirstLoader) / kTeam;
         uint32_t i = 0;
         bool ok = true;
         for (uint32_t it = first_item; it < items && ok; it += item_step) {
@@ -309,6 +312,7 @@ __global__ void __launch_bounds__(GemmShape<BN, KIND, FEED>::kThreads, 1) k_gemm
             uint32_t tm, tn;
             locate(it - split * tiles, tm, tn);
             for (uint32_t ks = ks0; ks < ks1; ++ks, ++i) {
+                if (S::kTeams > 1u && i % S::kTeams != team) continue;
                 const uint32_t stage = i % kStages, r = i % S::kRing, turn = (i / S::kRing) & 1u;
                 const bool place_b = g.b_raw && !(keep_b && i >= kStages);
                 ok = tma::wait(&bar.empty[stage], (i / kStages + 1u) & 1u) && (!g.a_raw || tma::wait(&bar.raw_full[0][r], turn)) &&
