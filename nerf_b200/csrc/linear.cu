@@ -12,9 +12,9 @@
 //
 // k_gemm: persistent CTAs, one 128 x BN tile (or one part of its K range) at
 // a time.  Warp 0 copies operand boxes into a ring of shared-memory stages,
-// one thread of warp 1 issues the MMAs into one of two tensor-memory
-// accumulators, and two groups of four warps drain them in turn: the copies,
-// the products and the epilogues of the two tiles before overlap.
+// one thread of warp 1 issues the MMAs into one of two or four tensor-memory
+// accumulators, and two or four groups of four warps drain them in turn: the
+// copies, the products and the epilogues of the tiles before overlap.
 //   kFeedTma    one CTA a tile.
 //   kFeedPair   two CTAs on one 256 x 256 tile: each holds its 128 rows of A
 //               and half of B, so the tensor cores read 8 KB of shared memory
@@ -22,7 +22,7 @@
 //               delivers (128 bytes a cycle).
 //   kFeedRaw, kFeedRawShort
 //               rows that do not start on 16-byte boundaries: copied raw, and
-//               moved into place by eight or four more warps.
+//               moved into place by four to sixteen more warps.
 #include <atomic>
 
 #include "linear_common.cuh"
@@ -42,10 +42,11 @@ constexpr uint32_t kMaxStages = 8;
 // or 136 (MN-major) values each from the 16-byte boundary before the first one
 // wanted.  Warps then move the rows of a residue each into the swizzled box: a
 // shared-memory read or two, a permute and a write a row, and no trip to memory.
-// The copies' price is by the copy (a thread gets one off about every 128
-// cycles), so the operands' are issued by a warp each.  2000 x 4000 -> 4000 with
-// rows 4001 apart took 356 us with loads to registers instead, and 430 us with
-// 16-byte asynchronous copies by the warps that move the rows.
+// A thread gets a copy off about every 128 cycles: the operands' are issued by a
+// warp each.  2000 x 4000 -> 4000 with
+// rows 4001 apart takes 220 us, 356 us with loads to registers instead, and 430 us with
+// 16-byte asynchronous copies by the warps that move the rows.  Their shared-memory traffic
+// bounds it: 244 us without the copies, 150 without the moves (one team of warps, in all 245).
 constexpr uint32_t kRawRing = 2, kMaxRing = 3;  // steps of raw copies in shared memory
 
 // Bytes of one residue's copy: of n rows (K-major), of 64 rows x 128 columns (MN-major).
@@ -144,13 +145,15 @@ NB_DEV void tile_of(const GemmArgs& g, uint32_t t, uint32_t& tm, uint32_t& tn) {
 template <uint32_t BN, int KIND, int FEED>
 struct GemmShape {
     static constexpr bool kPair = FEED == kFeedPair, kRaw = FEED == kFeedRaw || FEED == kFeedRawShort;
-    // Warps that place the raw copies of a step, and teams of them that take the steps in turn.
+    // Warps that place the raw copies of a step, and teams of them that take the steps in turn (a weight gradient's
+    // epilogue has no registers to spare for a second).
     static constexpr uint32_t kLoaders = FEED == kFeedRaw ? 8u : FEED == kFeedRawShort ? 4u : 0u;
     static constexpr uint32_t kTeams = FEED == kFeedRaw && KIND == kGemmRows ? 2u : 1u;
     static constexpr uint32_t kBoxN = kPair ? BN / 2u : BN;  // rows of B in this CTA's shared memory
     static constexpr uint32_t kStageBytes = kStageBytesA + kBoxN * 128u;
-    // Epilogue groups of four warps: the epilogues' latency is what bounds short products.  Up to 128 columns a tile
-    // each has an accumulator, of 256 two share one, a half each.
+    // Epilogue groups of four warps: the epilogues' instructions and latency bound short products (65536 x 512 -> 512
+    // with GELU: 86 us with two groups, 66 with four).  Up to 128 columns a tile each has an accumulator, of 256 two
+    // share one, a half each.
     static constexpr uint32_t kGroups = KIND == kGemmRows && FEED != kFeedRaw ? 4u : 2u;
     static constexpr uint32_t kAccs = BN == 256u ? 2u : kGroups, kColsGroup = KIND == kGemmRows ? BN * kAccs / kGroups : BN;
     static constexpr uint32_t kRing = FEED == kFeedRaw ? kMaxRing : kRawRing;
