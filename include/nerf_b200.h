@@ -397,7 +397,8 @@ typedef struct NerfB200Linear {
 /* z = x weight^T + bias, y = act(z) + residual; pre = z where given (what the
  * backward needs unless the activation is NONE).  bias [n_out], residual and
  * pre may be NULL.  Products are summed in fp32, y and pre are rounded once.
- * residual may be y itself; otherwise outputs overlap nothing.  Any alignment
+ * residual may be y itself (with its ld); otherwise outputs overlap nothing (the
+ * same pointer for an output and another matrix is refused).  Any alignment
  * of the dtype is accepted; rows that start on 16-byte boundaries (pointer
  * and ld) are the fast path (x and weight of another alignment are read from
  * the 16-byte boundary before their first value on).  error_word: one device uint32; bit 0 is set
@@ -408,7 +409,7 @@ NERF_API NerfStatus nerf_b200_linear_forward(const NerfB200Linear* desc, const v
 /* dz = dy act'(pre); dx = dz weight + dx_residual; dweight [n_out][n_in]
  * (tight) and dbias [n_out] are dz^T x and the column sums of dz, written or
  * added to.  dx, dweight, dbias, dx_residual may be NULL (dx_residual may be
- * dx itself, or dy where the widths agree: the gradient of the forward's
+ * dx itself, with its ld, or dy where the widths agree: the gradient of the forward's
  * residual is dy).  ReLU passes nothing where pre <= 0, whatever dy holds.
  * dz is rounded to dtype before the two products (exact for NONE and RELU);
  * dbias sums it before the rounding.  Sums are fp32 in a fixed order: the

@@ -320,6 +320,8 @@ NERF_API NerfStatus nerf_b200_linear_forward(const NerfB200Linear* desc, const v
     if (residual && d.ld_residual && d.ld_residual < d.n_out) return NERF_STATUS_INVALID_USAGE;
     if (d.n_rows == 0u) return NERF_STATUS_OK;
     if (!x || !weight || !y || !error_word) return NERF_STATUS_INVALID_USAGE;
+    if (y == x || y == weight || y == pre || pre == x || (pre && pre == residual)) return NERF_STATUS_INVALID_USAGE;
+    if (residual == y && d.n_rows > 1u && ld_or(d.ld_residual, d.n_out) != ld_or(d.ld_y, d.n_out)) return NERF_STATUS_INVALID_USAGE;
     const void* all[] = {x, weight, bias, residual, y, pre};
     for (const void* p : all)
         if (!aligned(p, 2u)) return NERF_STATUS_INVALID_USAGE;
@@ -376,6 +378,8 @@ NERF_API NerfStatus nerf_b200_linear_backward(const NerfB200Linear* desc, const 
     }
     if (!dy || !error_word || !workspace || (dx && !weight) || (dweight && !x) || (d.activation != kActNone && !pre))
         return NERF_STATUS_INVALID_USAGE;
+    if (dx && (dx == dy || dx == weight || (dx == pre && d.activation != kActNone) || (dx == x && dweight))) return NERF_STATUS_INVALID_USAGE;
+    if (dx && dx_residual == dx && d.n_rows > 1u && ld_or(d.ld_residual, d.n_in) != ld_or(d.ld_dx, d.n_in)) return NERF_STATUS_INVALID_USAGE;
     const void* all[] = {x, weight, pre, dy, dx_residual, dx, dweight, dbias};
     for (const void* p : all)
         if (!aligned(p, 2u)) return NERF_STATUS_INVALID_USAGE;

@@ -52,6 +52,18 @@ def test_missing_and_misaligned_arguments():
     assert size > 0 and _backward(d, size=size - 1) == INVALID
 
 
+def test_outputs_over_operands_are_refused():
+    d, at = _desc(), [OK + 0x1000 * i for i in range(12)]
+    good = dict(x=at[0], w=at[1], b=at[2], r=at[3], y=at[4], z=at[5], e=at[6])
+    for change in (dict(y=at[0]), dict(y=at[1]), dict(y=at[5]), dict(z=at[0]), dict(z=at[3])):
+        assert _forward(d, **{**good, **change}) == INVALID, change
+    assert _forward(_desc(ld_residual=16), **{**good, "r": at[4]}) == INVALID  # in place with another distance between rows
+    good = dict(x=at[0], w=at[1], z=at[2], dy=at[3], r=None, dx=at[4], dw=at[5], db=at[6], ws=at[7], e=at[8])
+    for change in (dict(dx=at[0]), dict(dx=at[1]), dict(dx=at[2]), dict(dx=at[3])):
+        assert _backward(d, **{**good, **change}) == INVALID, change
+    assert _backward(_desc(ld_residual=16), **{**good, "r": at[4]}) == INVALID
+
+
 def test_nothing_to_do_needs_no_device():
     d = _desc(n_rows=0)
     assert _forward(d, x=None, w=None, y=None, e=None) == abi.NERF_STATUS_OK
